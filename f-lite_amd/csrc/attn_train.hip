@@ -1,0 +1,680 @@
+// Attention for training on gfx950: the forward pass that keeps its log-sum-exp, and the backward pass that makes the
+// probabilities again from it. Packed sequences (cu_seqlens), no mask, head sizes 64, 128 and 256, bf16, K/V heads
+// shared by groups of query heads.
+//
+//   S = scale q k^T, lse = log sum exp S, P = exp(S - lse), out = P v
+//   delta = sum_d dout * out,  dP = dout v^T,  dS = P * (dP - delta)
+//   dv = P^T dout,  dk = scale dS^T q,  dq = scale dS k
+//
+// Backward = three launches. (1) delta and lse * log2(e) per query row. (2) Two kinds of workgroups in one launch: a
+// "key" workgroup owns 128 keys of one K/V head and sweeps the queries of its group of heads (4 products: S, dP, dv,
+// dk); a "query" workgroup owns 128 queries of one head and sweeps the keys (3 products: S, dP, dq). S and dP are made
+// twice (7 products instead of 5), and in return every gradient is summed by one workgroup in registers, in a fixed
+// order: no atomics, no fp32 gradient in memory. (3) Where too few workgroups would run, the sweeps are cut into
+// ranges whose fp32 partial gradients a last kernel adds in range order.
+//
+// A wave owns 32 of the workgroup's rows ("stationary": fragments in registers, row on the lane) and reads tiles of
+// the swept rows from LDS: row-wise (ds_read_b128, A operand of S and dP) and transposed (ds_read_b64_tr_b16, A operand
+// of the gradients). P and dS go from the S accumulators straight into the B operand: no LDS round trip.
+#include <math.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "attn_common.h"
+#include "common.h"
+#include "kernels.h"
+
+namespace flite {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int WROWS = 128;  // stationary rows of a workgroup
+constexpr int TR = 64;      // swept rows of an LDS tile
+constexpr int kThreads = 256;
+constexpr int kMaxSplit = 16;
+
+struct TrainDev {
+  AttnTrainParams p;
+  int tiles_q, tiles_k;    // upper bounds of the packed batch's 128-row tiles
+  int split_q, split_k;    // ranges that a query / key workgroup's sweep is cut into
+  int n_key_blocks;        // backward: the first blocks of the launch are key workgroups
+  float2* ld;              // [H][total_q] (lse * log2 e, delta)
+  float* part_q;           // [split_q][total_q][H][D] fp32, with split_q > 1
+  float* part_k;           // [split_k][total_k][HK][D]
+  float* part_v;
+};
+
+// One sequence's rows [start, start + len) of `total`, from a cumulative array that a caller may have filled wrongly:
+// clamped, so that nothing outside the tensors is touched.
+__device__ __forceinline__ void seq_range(const int* cu, int b, int total, int* start, int* len) {
+  const int s = min(max(cu[b], 0), total);
+  const int e = min(max(cu[b + 1], s), total);
+  *start = s;
+  *len = e - s;
+}
+
+// Tile t of the packed batch -> (sequence, first row); false past the last tile. Tiles number the sequences' 128-row
+// pieces in order.
+__device__ __forceinline__ bool find_tile(const int* cu, int B, int total, int t, int* b, int* row0) {
+  const int lane = threadIdx.x & 63;
+  for (int base = 0; base < B; base += 64) {
+    int s, len = 0;
+    if (base + lane < B) seq_range(cu, base + lane, total, &s, &len);
+    const int n = (len + WROWS - 1) / WROWS;
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += up;
+    }
+    const unsigned long long hit = __ballot(t < sum);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      *b = base + l;
+      *row0 = (t - (__shfl(sum, l, 64) - __shfl(n, l, 64))) * WROWS;
+      return true;
+    }
+    t -= __shfl(sum, 63, 64);
+  }
+  return false;
+}
+
+// XOR of the 16-B chunk index of tile row r. The low 4 bits of a row map one to one onto the XOR (row reads of 16 lanes
+// hit 16 different chunks), and rows 0..3 of a group land in different 64-B blocks (transposed reads). 128-B rows
+// (D = 64): two rows share the 256 B of banks, so bit 0 of the row needs no XOR.
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+  if constexpr (D == 64)
+    return ((r & 2) << 1) | ((r >> 2) & 3);
+  else
+    return ((r & 3) << 2) | ((r >> 2) & 3);
+}
+
+// Copies TR rows of D elements from `base` (row stride `stride` elements) into LDS at `lds`, swizzled; rows >= rows_left
+// become zeros (the buffer range check).
+template <int D>
+__device__ __forceinline__ void stage(const bf16_t* base, long stride, long rows_left, unsigned lds, int wave, int lane) {
+  constexpr int CPR = D / 8;                 // 16-B chunks per row
+  constexpr int PIECES = TR * D * 2 / 1024;  // 1-KiB copies per tile
+  const i32x4 rs = make_rsrc(base, (unsigned)min(max(rows_left, 0L) * stride * 2, 0x7fffffffL));
+#pragma unroll
+  for (int i = 0; i < PIECES / 4; ++i) {
+    const int piece = wave * (PIECES / 4) + i;
+    const int pos = piece * 64 + lane;
+    const int row = pos / CPR, ch = (pos % CPR) ^ swz<D>(row);
+    blds16(rs, (unsigned)(row * stride * 2 + ch * 16), lds + piece * 1024);
+  }
+}
+
+// Fragments of the stationary rows: lane (row lq, half hh) holds elements 16 s + 8 hh .. + 7
+template <int D>
+__device__ __forceinline__ void load_frags(const bf16_t* row, int hh, bf16x8 (&f)[D / 16]) {
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) f[s] = *(const bf16x8*)(row + 16 * s + 8 * hh);
+}
+
+// LDS offsets of a lane's reads, relative to a 32-row half tile
+template <int D>
+struct LaneOff {
+  int row[D / 16];  // row-wise: chunk 2 s + hh of row lq
+  int tr[2][D / 32];  // transposed: columns 32 dt .., rows 4 (G >> 1) + vq of an even / odd 8-row group
+  __device__ __forceinline__ LaneOff(int lane) {
+    const int lq = lane & 31, hh = lane >> 5;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) row[s] = lq * D * 2 + (((2 * s + hh) ^ swz<D>(lq)) << 4);
+    const int G = lane >> 4, vq = (lane & 15) >> 2, vp = lane & 3;
+    const int r0 = 4 * (G >> 1) + vq;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int o = 0; o < 2; ++o)
+        tr[o][dt] = (r0 + 8 * o) * D * 2 + (((4 * dt + 2 * (G & 1) + (vp >> 1)) ^ swz<D>(r0 + 8 * o)) << 4) + (vp & 1) * 8;
+  }
+};
+
+// acc[32 tile rows x 32 stationary rows] = tile rows . stationary rows
+template <int D>
+__device__ __forceinline__ f32x16 row_product(const char* half, const LaneOff<D>& o, const bf16x8 (&f)[D / 16]) {
+  f32x16 acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s)
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(half + o.row[s]), f[s], acc, 0, 0, 0);
+  return acc;
+}
+
+// acc[D x 32 stationary rows] += (tile half)^T . m, m[32 tile rows x 32 stationary rows] in the accumulator layout
+template <int D>
+__device__ __forceinline__ void tr_product(const char* half, const LaneOff<D>& o, const f32x16& m, f32x16 (&acc)[D / 32]) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    // rounded to bf16 for the matrix unit (relative 2^-9); accumulators, P and dS themselves are fp32
+    bf16x8 b;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = (__bf16)m[8 * s + j];
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) {
+      const s16x4 lo = ds_tr16(half + 16 * s * D * 2 + o.tr[0][dt]);
+      const s16x4 hi = ds_tr16(half + 16 * s * D * 2 + o.tr[1][dt]);
+      const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc[dt], 0, 0, 0);
+    }
+  }
+}
+
+// The lane's stationary row of acc[D x rows], times f: bf16 to `dst` (the row's start)
+template <int D>
+__device__ __forceinline__ void store_row(bf16_t* dst, const f32x16 (&acc)[D / 32], float f, int hh, bool live) {
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int rp = 0; rp < 2; ++rp) {
+      const int a = 8 * rp, b = 8 * rp + 4;
+      const auto x0 = __builtin_amdgcn_permlane32_swap(pack2bf(acc[i][a] * f, acc[i][a + 1] * f),
+                                                       pack2bf(acc[i][b] * f, acc[i][b + 1] * f), false, false);
+      const auto x1 = __builtin_amdgcn_permlane32_swap(pack2bf(acc[i][a + 2] * f, acc[i][a + 3] * f),
+                                                       pack2bf(acc[i][b + 2] * f, acc[i][b + 3] * f), false, false);
+      const u32x4 w = {x0[0], x1[0], x0[1], x1[1]};
+      if (live) *(u32x4*)(dst + i * 32 + 16 * rp + 8 * hh) = w;
+    }
+}
+
+// the same as an fp32 partial
+template <int D>
+__device__ __forceinline__ void store_part(float* dst, const f32x16 (&acc)[D / 32], float f, int hh, bool live) {
+  if (!live) return;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4)
+      *(f32x4*)(dst + i * 32 + 8 * r4 + 4 * hh) =
+          f32x4{acc[i][4 * r4] * f, acc[i][4 * r4 + 1] * f, acc[i][4 * r4 + 2] * f, acc[i][4 * r4 + 3] * f};
+}
+
+#define TILE_SYNC()                                  \
+  do {                                               \
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); \
+    __syncthreads();                                 \
+  } while (0)
+
+// ------------------------------------------------------------------------------------------------ forward
+template <int D>
+__global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const AttnTrainParams& p = d.p;
+  constexpr int TB = TR * D * 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int lq = lane & 31, hh = lane >> 5;
+  const int v = xcd_remap(blockIdx.x, gridDim.x);
+  const int h = v / d.tiles_q;
+  int b, row0;
+  if (!find_tile(p.cu_q, p.B, p.total_q, v % d.tiles_q, &b, &row0)) return;
+  int q_start, q_len, k_start, k_len;
+  seq_range(p.cu_q, b, p.total_q, &q_start, &q_len);
+  seq_range(p.cu_k, b, p.total_k, &k_start, &k_len);
+  const int hk = h / (p.H / p.HK);
+  const int row = row0 + wave * 32 + lq;
+  const bool live = row < q_len;
+
+  bf16x8 qf[D / 16];
+  load_frags<D>(p.q + (long)(q_start + min(row, q_len - 1)) * p.q_row + (long)h * p.q_head, hh, qf);
+  const LaneOff<D> off(lane);
+  const unsigned lds0 = lds_addr_of(smem);
+  const bf16_t* kp = p.k + (long)k_start * p.k_row + (long)hk * p.k_head;
+  const bf16_t* vp = p.v + (long)k_start * p.v_row + (long)hk * p.v_head;
+  auto fetch = [&](int t, int buf) {
+    const long r = (long)t * TR;
+    stage<D>(kp + r * p.k_row, p.k_row, k_len - r, lds0 + buf * 2 * TB, wave, lane);
+    stage<D>(vp + r * p.v_row, p.v_row, k_len - r, lds0 + buf * 2 * TB + TB, wave, lane);
+  };
+  const float sl2 = p.scale * kLog2e;
+  float m = -INFINITY, l = 0.f;
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+
+  const int nt = (k_len + TR - 1) / TR;
+  if (nt > 0) fetch(0, 0);
+  TILE_SYNC();
+  for (int t = 0; t < nt; ++t) {
+    if (t + 1 < nt) fetch(t + 1, (t + 1) & 1);
+    const char* kt = smem + (t & 1) * 2 * TB;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      f32x16 s = row_product<D>(kt + hf * 32 * D * 2, off, qf);
+      float top = -INFINITY;
+      const int k_left = k_len - t * TR - hf * 32 - 4 * hh;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = 8 * (r >> 2) + (r & 3) < k_left ? s[r] * sl2 : -INFINITY;
+        top = fmaxf(top, s[r]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float m_new = fmaxf(m, top);
+      if (__any(m_new > m)) {
+        const float alpha = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+        l *= alpha;
+        m = m_new;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][r] *= alpha;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        // a half tile without keys, before the first key, has m = -inf: its scores are -inf too
+        s[r] = s[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s[r] - m);
+        l += s[r];
+      }
+      tr_product<D>(kt + TB + hf * 32 * D * 2, off, s, acc);
+    }
+    TILE_SYNC();
+  }
+  l += __shfl_xor(l, 32, 64);
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no keys: zeros; NaN stays
+  store_row<D>(p.o + (long)(q_start + row) * p.o_row + (long)h * p.o_head, acc, inv, hh, live);
+  if (live && hh == 0)
+    p.lse[(long)h * p.total_q + q_start + row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+// (lse * log2 e, delta) of every query row; rows outside all sequences are not read by anyone
+template <int D>
+__global__ __launch_bounds__(kThreads) void attn_delta_kernel(TrainDev d) {
+  const AttnTrainParams& p = d.p;
+  constexpr int LANES = D / 8;
+  const long item = ((long)blockIdx.x * kThreads + threadIdx.x) / LANES;
+  const int c = threadIdx.x % LANES;
+  if (item >= (long)p.total_q * p.H) return;
+  const int row = (int)(item / p.H), h = (int)(item % p.H);
+  const bf16x8 a = *(const bf16x8*)(p.dout + (long)row * p.do_row + (long)h * p.do_head + 8 * c);
+  const bf16x8 b = *(const bf16x8*)(p.o + (long)row * p.o_row + (long)h * p.o_head + 8 * c);
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s += (float)a[j] * (float)b[j];
+#pragma unroll
+  for (int o = 1; o < LANES; o <<= 1) s += __shfl_xor(s, o, 64);
+  if (c == 0) {
+    const long at = (long)h * p.total_q + row;
+    const float lse = p.lse[at];
+    // a row without keys (or with -inf scores alone) has P = 0: exp2(x - inf)
+    d.ld[at] = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e, s);
+  }
+}
+
+// A query workgroup: dq of 128 queries of head h
+template <int D>
+__device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem) {
+  const AttnTrainParams& p = d.p;
+  constexpr int TB = TR * D * 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int lq = lane & 31, hh = lane >> 5;
+  const int part = v % d.split_q;
+  v /= d.split_q;
+  const int h = v / d.tiles_q;
+  int b, row0;
+  if (!find_tile(p.cu_q, p.B, p.total_q, v % d.tiles_q, &b, &row0)) return;
+  int q_start, q_len, k_start, k_len;
+  seq_range(p.cu_q, b, p.total_q, &q_start, &q_len);
+  seq_range(p.cu_k, b, p.total_k, &k_start, &k_len);
+  const int hk = h / (p.H / p.HK);
+  const int row = row0 + wave * 32 + lq;
+  const bool live = row < q_len;
+  const int rc = q_start + min(row, q_len - 1);
+
+  bf16x8 qf[D / 16], df[D / 16];
+  load_frags<D>(p.q + (long)rc * p.q_row + (long)h * p.q_head, hh, qf);
+  load_frags<D>(p.dout + (long)rc * p.do_row + (long)h * p.do_head, hh, df);
+  const float2 ld = d.ld[(long)h * p.total_q + rc];
+  const LaneOff<D> off(lane);
+  const unsigned lds0 = lds_addr_of(smem);
+  const bf16_t* kp = p.k + (long)k_start * p.k_row + (long)hk * p.k_head;
+  const bf16_t* vp = p.v + (long)k_start * p.v_row + (long)hk * p.v_head;
+  auto fetch = [&](int t, int buf) {
+    const long r = (long)t * TR;
+    stage<D>(kp + r * p.k_row, p.k_row, k_len - r, lds0 + buf * 2 * TB, wave, lane);
+    stage<D>(vp + r * p.v_row, p.v_row, k_len - r, lds0 + buf * 2 * TB + TB, wave, lane);
+  };
+  const float sl2 = p.scale * kLog2e;
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+
+  const int all = (k_len + TR - 1) / TR, per = (all + d.split_q - 1) / d.split_q;
+  const int t0 = min(part * per, all), t1 = min(t0 + per, all);
+  if (t0 < t1) fetch(t0, 0);
+  TILE_SYNC();
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    if (t + 1 < t1) fetch(t + 1, buf ^ 1);
+    const char* kt = smem + buf * 2 * TB;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      f32x16 s = row_product<D>(kt + hf * 32 * D * 2, off, qf);
+      const f32x16 dp = row_product<D>(kt + TB + hf * 32 * D * 2, off, df);
+      // keys past the end are zero rows: they add nothing to dq, but exp2(-lse) could overflow (inf * 0)
+      const int k_left = k_len - t * TR - hf * 32 - 4 * hh;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sl2, -ld.x)) * (dp[r] - ld.y);
+        s[r] = 8 * (r >> 2) + (r & 3) < k_left ? e : 0.f;
+      }
+      tr_product<D>(kt + hf * 32 * D * 2, off, s, acc);
+    }
+    TILE_SYNC();
+  }
+  if (d.split_q > 1)
+    store_part<D>(d.part_q + (((long)part * p.total_q + rc) * p.H + h) * D, acc, p.scale, hh, live);
+  else
+    store_row<D>(p.dq + (long)rc * p.dq_row + (long)h * p.dq_head, acc, p.scale, hh, live);
+}
+
+// A key workgroup: dk and dv of 128 keys of K/V head hk
+template <int D>
+__device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) {
+  const AttnTrainParams& p = d.p;
+  constexpr int TB = TR * D * 2;
+  constexpr int LDB = TR * 8;  // (lse, delta) of a tile
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int lq = lane & 31, hh = lane >> 5;
+  const int part = v % d.split_k;
+  v /= d.split_k;
+  const int hk = v / d.tiles_k;
+  int b, row0;
+  if (!find_tile(p.cu_k, p.B, p.total_k, v % d.tiles_k, &b, &row0)) return;
+  int q_start, q_len, k_start, k_len;
+  seq_range(p.cu_q, b, p.total_q, &q_start, &q_len);
+  seq_range(p.cu_k, b, p.total_k, &k_start, &k_len);
+  const int group = p.H / p.HK;
+  const int row = row0 + wave * 32 + lq;
+  const bool live = row < k_len;
+  const int rc = k_start + min(row, k_len - 1);
+
+  bf16x8 kf[D / 16], vf[D / 16];
+  load_frags<D>(p.k + (long)rc * p.k_row + (long)hk * p.k_head, hh, kf);
+  load_frags<D>(p.v + (long)rc * p.v_row + (long)hk * p.v_head, hh, vf);
+  const LaneOff<D> off(lane);
+  const unsigned lds0 = lds_addr_of(smem);
+  const int tiles = (q_len + TR - 1) / TR;  // tiles of one head
+  char* const ld_s = smem + 4 * TB;
+  // tile i of the sweep over the group's heads and their query tiles. Rows past the sequence end are zeros, (lse,
+  // delta) included: P = exp2(0 - 0) = 1 meets zero rows of q and dout and adds nothing
+  auto fetch = [&](int i, int buf) {
+    const int h = hk * group + i / tiles;
+    const long r = (long)(i % tiles) * TR;
+    const long at = q_start + r;
+    stage<D>(p.q + at * p.q_row + (long)h * p.q_head, p.q_row, q_len - r, lds0 + buf * 2 * TB, wave, lane);
+    stage<D>(p.dout + at * p.do_row + (long)h * p.do_head, p.do_row, q_len - r, lds0 + buf * 2 * TB + TB, wave, lane);
+    if (threadIdx.x < TR) {
+      float2 x = make_float2(0.f, 0.f);
+      if (r + (int)threadIdx.x < q_len) x = d.ld[(long)h * p.total_q + at + threadIdx.x];
+      *(float2*)(ld_s + buf * LDB + threadIdx.x * 8) = x;
+    }
+  };
+  const float sl2 = p.scale * kLog2e;
+  f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
+
+  const int all = tiles * group, per = (all + d.split_k - 1) / d.split_k;
+  const int t0 = min(part * per, all), t1 = min(t0 + per, all);
+  if (t0 < t1) fetch(t0, 0);
+  TILE_SYNC();
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    if (t + 1 < t1) fetch(t + 1, buf ^ 1);
+    const char* qt = smem + buf * 2 * TB;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const char* qh = qt + hf * 32 * D * 2;
+      f32x16 s = row_product<D>(qh, off, kf);
+      f32x16 dp = row_product<D>(qh + TB, off, vf);
+      const f32x4* ld = (const f32x4*)(ld_s + buf * LDB + (hf * 32 + 4 * hh) * 8);
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {  // rows 8 (r >> 2) + 4 hh + (r & 3): two per 16 B
+        const f32x4 x = ld[4 * (r >> 2) + ((r & 3) >> 1)];
+        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sl2, -x[0]));
+        s[r + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], sl2, -x[2]));
+        dp[r] = s[r] * (dp[r] - x[1]);
+        dp[r + 1] = s[r + 1] * (dp[r + 1] - x[3]);
+      }
+      tr_product<D>(qh + TB, off, s, dv);
+      tr_product<D>(qh, off, dp, dk);
+    }
+    TILE_SYNC();
+  }
+  if (d.split_k > 1) {
+    const long at = (((long)part * p.total_k + rc) * p.HK + hk) * D;
+    store_part<D>(d.part_k + at, dk, p.scale, hh, live);
+    store_part<D>(d.part_v + at, dv, 1.f, hh, live);
+  } else {
+    store_row<D>(p.dk + (long)rc * p.dk_row + (long)hk * p.dk_head, dk, p.scale, hh, live);
+    store_row<D>(p.dv + (long)rc * p.dv_row + (long)hk * p.dv_head, dv, 1.f, hh, live);
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads, 1) void attn_bwd_kernel(TrainDev d) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  if ((int)blockIdx.x < d.n_key_blocks)
+    key_block<D>(d, xcd_remap(blockIdx.x, d.n_key_blocks), smem);
+  else
+    query_block<D>(d, xcd_remap(blockIdx.x - d.n_key_blocks, gridDim.x - d.n_key_blocks), smem);
+}
+
+// Adds the ranges' partial gradients in order. Rows outside all sequences have no partials and are left alone.
+template <int D>
+__global__ __launch_bounds__(kThreads) void attn_join_kernel(const float* part, int n, bf16_t* out, long row_stride,
+                                                             long head_stride, const int* cu, int B, int total, int H) {
+  constexpr int LANES = D / 8;
+  const long item = ((long)blockIdx.x * kThreads + threadIdx.x) / LANES;
+  const int c = threadIdx.x % LANES;
+  if (item >= (long)total * H) return;
+  const int row = (int)(item / H), h = (int)(item % H);
+  bool inside = false;
+  for (int b = 0; b < B && !inside; ++b) {
+    int s, len;
+    seq_range(cu, b, total, &s, &len);
+    inside = row >= s && row < s + len;
+  }
+  if (!inside) return;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+  const long step = (long)total * H * D;
+  const float* src = part + item * D + 8 * c;
+  for (int i = 0; i < n; ++i) {
+    a += *(const f32x4*)(src + i * step);
+    b += *(const f32x4*)(src + i * step + 4);
+  }
+  const u32x4 w = {pack2bf(a[0], a[1]), pack2bf(a[2], a[3]), pack2bf(b[0], b[1]), pack2bf(b[2], b[3])};
+  *(u32x4*)(out + (long)row * row_stride + (long)h * head_stride + 8 * c) = w;
+}
+
+// zeros (lse: -inf) in the rows outside all sequences
+__global__ __launch_bounds__(kThreads) void attn_zero_kernel(bf16_t* out, long row_stride, long head_stride, const int* cu,
+                                                             int B, int total, int H, int D, float* lse) {
+  const long item = ((long)blockIdx.x * kThreads + threadIdx.x) * 8;
+  if (item >= (long)total * H * D) return;
+  const int row = (int)(item / ((long)H * D)), h = (int)(item / D % H), c = (int)(item % D);
+  for (int b = 0; b < B; ++b) {
+    int s, len;
+    seq_range(cu, b, total, &s, &len);
+    if (row >= s && row < s + len) return;
+  }
+  *(u32x4*)(out + (long)row * row_stride + (long)h * head_stride + c) = u32x4{0u, 0u, 0u, 0u};
+  if (lse != nullptr && c == 0) lse[(long)h * total + row] = -INFINITY;
+}
+
+constexpr int kCus = 256;
+
+struct Plan {
+  int tiles_q, tiles_k, split_q, split_k;
+  long ld_bytes, part_q_bytes, part_k_bytes;  // part_k_bytes: dk and dv each
+};
+
+// Ranges per sweep: as many as fill the CUs (a workgroup takes a whole CU), none shorter than two tiles of the average
+// sequence.
+Plan make_plan(const AttnTrainParams& p) {
+  Plan x;
+  x.tiles_q = p.total_q / WROWS + p.B;
+  x.tiles_k = p.total_k / WROWS + p.B;
+  const long nq = (long)(p.total_q / WROWS + 1) * p.H, nk = (long)(p.total_k / WROWS + 1) * p.HK;
+  const long sweep_q = p.total_k / p.B / TR, sweep_k = (long)(p.total_q / p.B / TR) * (p.H / p.HK);
+  auto ranges = [&](long tiles) {
+    return (int)std::max(1L, std::min({(long)kMaxSplit, kCus / (nq + nk), tiles / 2}));
+  };
+  x.split_q = ranges(sweep_q);
+  x.split_k = ranges(sweep_k);
+  auto pad = [](long n) { return (n + 255) / 256 * 256; };
+  x.ld_bytes = pad((long)p.H * p.total_q * 8);
+  x.part_q_bytes = x.split_q > 1 ? pad((long)x.split_q * p.total_q * p.H * p.dim * 4) : 0;
+  x.part_k_bytes = x.split_k > 1 ? pad((long)x.split_k * p.total_k * p.HK * p.dim * 4) : 0;
+  return x;
+}
+
+int check(const AttnTrainParams& p) {
+  FLITE_REQUIRE(p.dim == 64 || p.dim == 128 || p.dim == 256, "attention: head size must be 64, 128 or 256");
+  FLITE_REQUIRE(p.B > 0 && p.H > 0 && p.HK > 0 && p.H % p.HK == 0,
+                "attention: batch, heads and kv heads must be positive, heads a multiple of kv heads");
+  FLITE_REQUIRE(p.total_q >= 0 && p.total_k >= 0, "attention: rows must not be negative");
+  FLITE_REQUIRE(((long)p.total_q / WROWS + p.B) * p.H < (1L << 30) / kMaxSplit &&
+                    ((long)p.total_k / WROWS + p.B) * p.HK < (1L << 30) / kMaxSplit,
+                "attention: too many rows, sequences or heads");
+  FLITE_REQUIRE(p.cu_q && p.cu_k, "attention: cu_seqlens missing");
+  return 0;
+}
+
+int check_rows(const void* ptr, long row, long head, int dim, bool any, const char* what) {
+  FLITE_REQUIRE(!any || ptr, std::string("attention: missing ") + what);
+  FLITE_REQUIRE(((uintptr_t)ptr & 15) == 0 && row % 8 == 0 && head % 8 == 0 && row >= dim && head >= 0 && row <= (1 << 22),
+                std::string("attention: ") + what +
+                    " must be 16-byte aligned, its row and head strides multiples of 8, the row stride dim to 2^22");
+  return 0;
+}
+
+template <typename F>
+int lds_limit(F* f, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  FLITE_HIP_CHECK(hipGetDevice(&dev));
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done.load() & bit) return 0;
+  FLITE_HIP_CHECK(hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit);
+  return 0;
+}
+
+template <int D>
+int launch_fwd(const TrainDev& d, hipStream_t s) {
+  constexpr int lds = 4 * TR * D * 2;
+  static std::atomic<unsigned long long> done{0};
+  if (lds_limit(attn_lse_kernel<D>, lds, done)) return 1;
+  hipLaunchKernelGGL(attn_lse_kernel<D>, dim3(d.tiles_q * d.p.H), dim3(kThreads), lds, s, d);
+  FLITE_HIP_CHECK(hipGetLastError());
+  return 0;
+}
+
+template <int D>
+int launch_bwd(const TrainDev& d, hipStream_t s) {
+  const AttnTrainParams& p = d.p;
+  constexpr int lds = 4 * TR * D * 2 + 2 * TR * 8;
+  static std::atomic<unsigned long long> done{0};
+  if (lds_limit(attn_bwd_kernel<D>, lds, done)) return 1;
+  auto blocks = [](long rows_heads) { return dim3((unsigned)((rows_heads * (D / 8) + kThreads - 1) / kThreads)); };
+  if (p.total_q > 0)
+    hipLaunchKernelGGL(attn_delta_kernel<D>, blocks((long)p.total_q * p.H), dim3(kThreads), 0, s, d);
+  const int n = d.n_key_blocks + (p.total_q > 0 ? d.tiles_q * p.H * d.split_q : 0);
+  if (n > 0) hipLaunchKernelGGL(attn_bwd_kernel<D>, dim3(n), dim3(kThreads), lds, s, d);
+  if (d.split_q > 1 && p.total_q > 0)
+    hipLaunchKernelGGL(attn_join_kernel<D>, blocks((long)p.total_q * p.H), dim3(kThreads), 0, s, d.part_q, d.split_q,
+                       p.dq, p.dq_row, p.dq_head, p.cu_q, p.B, p.total_q, p.H);
+  if (d.split_k > 1 && p.total_k > 0) {
+    hipLaunchKernelGGL(attn_join_kernel<D>, blocks((long)p.total_k * p.HK), dim3(kThreads), 0, s, d.part_k, d.split_k,
+                       p.dk, p.dk_row, p.dk_head, p.cu_k, p.B, p.total_k, p.HK);
+    hipLaunchKernelGGL(attn_join_kernel<D>, blocks((long)p.total_k * p.HK), dim3(kThreads), 0, s, d.part_v, d.split_k,
+                       p.dv, p.dv_row, p.dv_head, p.cu_k, p.B, p.total_k, p.HK);
+  }
+  FLITE_HIP_CHECK(hipGetLastError());
+  return 0;
+}
+
+void zero_outside(bf16_t* out, long row, long head, const int* cu, int B, int total, int H, int D, float* lse,
+                  hipStream_t s) {
+  if (total <= 0) return;
+  const long n = (long)total * H * D / 8;
+  hipLaunchKernelGGL(attn_zero_kernel, dim3((unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, out, row,
+                     head, cu, B, total, H, D, lse);
+}
+
+}  // namespace
+
+long attn_train_workspace_bytes(const AttnTrainParams& p) {
+  if (check(p)) return -1;
+  const Plan x = make_plan(p);
+  return x.ld_bytes + x.part_q_bytes + 2 * x.part_k_bytes;
+}
+
+int attn_train_fwd(const AttnTrainParams& p, hipStream_t s) {
+  if (int rc = check(p)) return rc;
+  const bool any_q = p.total_q > 0, any_k = p.total_k > 0;
+  if (int rc = check_rows(p.q, p.q_row, p.q_head, p.dim, any_q, "q")) return rc;
+  if (int rc = check_rows(p.k, p.k_row, p.k_head, p.dim, any_k, "k")) return rc;
+  if (int rc = check_rows(p.v, p.v_row, p.v_head, p.dim, any_k, "v")) return rc;
+  if (int rc = check_rows(p.o, p.o_row, p.o_head, p.dim, any_q, "out")) return rc;
+  FLITE_REQUIRE(p.lse || !any_q, "attention: missing lse");
+  if (!any_q) return 0;
+  TrainDev d{};
+  d.p = p;
+  d.tiles_q = make_plan(p).tiles_q;
+  if (p.zero_outside) zero_outside(p.o, p.o_row, p.o_head, p.cu_q, p.B, p.total_q, p.H, p.dim, p.lse, s);
+  if (p.dim == 64) return launch_fwd<64>(d, s);
+  if (p.dim == 128) return launch_fwd<128>(d, s);
+  return launch_fwd<256>(d, s);
+}
+
+int attn_train_bwd(const AttnTrainParams& p, void* ws, long ws_bytes, hipStream_t s) {
+  if (int rc = check(p)) return rc;
+  const bool any_q = p.total_q > 0, any_k = p.total_k > 0;
+  if (int rc = check_rows(p.q, p.q_row, p.q_head, p.dim, any_q, "q")) return rc;
+  if (int rc = check_rows(p.k, p.k_row, p.k_head, p.dim, any_k, "k")) return rc;
+  if (int rc = check_rows(p.v, p.v_row, p.v_head, p.dim, any_k, "v")) return rc;
+  if (int rc = check_rows(p.o, p.o_row, p.o_head, p.dim, any_q, "out")) return rc;
+  if (int rc = check_rows(p.dout, p.do_row, p.do_head, p.dim, any_q, "dout")) return rc;
+  if (int rc = check_rows(p.dq, p.dq_row, p.dq_head, p.dim, any_q, "dq")) return rc;
+  if (int rc = check_rows(p.dk, p.dk_row, p.dk_head, p.dim, any_k, "dk")) return rc;
+  if (int rc = check_rows(p.dv, p.dv_row, p.dv_head, p.dim, any_k, "dv")) return rc;
+  FLITE_REQUIRE(p.lse || !any_q, "attention: missing lse");
+  const Plan x = make_plan(p);
+  FLITE_REQUIRE((ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= x.ld_bytes + x.part_q_bytes + 2 * x.part_k_bytes) ||
+                    x.ld_bytes + x.part_q_bytes + 2 * x.part_k_bytes == 0,
+                "attention backward: workspace missing, not 256-byte aligned, or too small");
+  TrainDev d{};
+  d.p = p;
+  d.tiles_q = x.tiles_q;
+  d.tiles_k = x.tiles_k;
+  d.split_q = x.split_q;
+  d.split_k = x.split_k;
+  d.n_key_blocks = any_k ? x.tiles_k * p.HK * x.split_k : 0;
+  d.ld = (float2*)ws;
+  d.part_q = (float*)((char*)ws + x.ld_bytes);
+  d.part_k = (float*)((char*)ws + x.ld_bytes + x.part_q_bytes);
+  d.part_v = (float*)((char*)ws + x.ld_bytes + x.part_q_bytes + x.part_k_bytes);
+  if (p.zero_outside) {
+    zero_outside(p.dq, p.dq_row, p.dq_head, p.cu_q, p.B, p.total_q, p.H, p.dim, nullptr, s);
+    zero_outside(p.dk, p.dk_row, p.dk_head, p.cu_k, p.B, p.total_k, p.HK, p.dim, nullptr, s);
+    zero_outside(p.dv, p.dv_row, p.dv_head, p.cu_k, p.B, p.total_k, p.HK, p.dim, nullptr, s);
+  }
+  if (p.dim == 64) return launch_bwd<64>(d, s);
+  if (p.dim == 128) return launch_bwd<128>(d, s);
+  return launch_bwd<256>(d, s);
+}
+
+}  // namespace flite

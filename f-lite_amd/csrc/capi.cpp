@@ -177,6 +177,139 @@ int flite_rope_qknorm(void* stream, void* x, long ldx, long rows, int heads, int
   return rope_qknorm(p, (hipStream_t)stream);
 }
 
+// ---- training operators ----
+static AttnTrainParams attn_train_params(const flite_attn_train& a) {
+  AttnTrainParams p;
+  p.q = (const bf16_t*)a.q;
+  p.k = (const bf16_t*)a.k;
+  p.v = (const bf16_t*)a.v;
+  p.o = (bf16_t*)a.out;
+  p.lse = a.lse;
+  p.dout = (const bf16_t*)a.dout;
+  p.dq = (bf16_t*)a.dq;
+  p.dk = (bf16_t*)a.dk;
+  p.dv = (bf16_t*)a.dv;
+  p.q_row = a.q_row;
+  p.q_head = a.q_head;
+  p.k_row = a.k_row;
+  p.k_head = a.k_head;
+  p.v_row = a.v_row;
+  p.v_head = a.v_head;
+  p.o_row = a.out_row;
+  p.o_head = a.out_head;
+  p.do_row = a.dout_row;
+  p.do_head = a.dout_head;
+  p.dq_row = a.dq_row;
+  p.dq_head = a.dq_head;
+  p.dk_row = a.dk_row;
+  p.dk_head = a.dk_head;
+  p.dv_row = a.dv_row;
+  p.dv_head = a.dv_head;
+  p.cu_q = a.cu_q;
+  p.cu_k = a.cu_k;
+  p.B = a.batch;
+  p.H = a.heads;
+  p.HK = a.kv_heads;
+  p.dim = a.head_dim;
+  p.total_q = a.total_q;
+  p.total_k = a.total_k;
+  p.scale = a.scale;
+  p.zero_outside = a.zero_outside;
+  return p;
+}
+
+int flite_attn_lse_fwd(void* stream, const flite_attn_train* args) {
+  FLITE_REQUIRE(args, "flite_attn_lse_fwd: null argument");
+  return attn_train_fwd(attn_train_params(*args), (hipStream_t)stream);
+}
+
+long flite_attn_lse_bwd_workspace_bytes(const flite_attn_train* args) {
+  if (args == nullptr) {
+    set_last_error("flite: flite_attn_lse_bwd_workspace_bytes: null argument");
+    return -1;
+  }
+  return attn_train_workspace_bytes(attn_train_params(*args));
+}
+
+int flite_attn_lse_bwd(void* stream, const flite_attn_train* args, void* workspace, long workspace_bytes) {
+  FLITE_REQUIRE(args, "flite_attn_lse_bwd: null argument");
+  return attn_train_bwd(attn_train_params(*args), workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+static int rope_axes_call(void* stream, const flite_rope_axes_args* a, bool bwd) {
+  FLITE_REQUIRE(a, "flite_rope_axes: null argument");
+  RopeAxesParams p;
+  p.x = a->x;
+  p.x_row = a->x_row;
+  p.x_head = a->x_head;
+  p.out = a->out;
+  p.o_row = a->out_row;
+  p.o_head = a->out_head;
+  p.y = a->y;
+  p.y_row = a->y_row;
+  p.y_head = a->y_head;
+  p.rstd = a->rstd;
+  p.positions = a->positions;
+  p.pos_is_f32 = a->positions_f32;
+  p.axes = a->axes;
+  p.tokens = a->tokens;
+  p.rows = a->rows;
+  p.heads = a->heads;
+  p.rope_heads = a->rope_heads;
+  p.dim = a->head_dim;
+  p.eps = a->eps;
+  return rope_axes(p, a->axis_pairs, a->bases, a->is_bf16 != 0, a->interleaved != 0, a->norm != 0, bwd,
+                   (hipStream_t)stream);
+}
+
+int flite_rope_axes_fwd(void* stream, const flite_rope_axes_args* args) { return rope_axes_call(stream, args, false); }
+
+int flite_rope_axes_bwd(void* stream, const flite_rope_axes_args* args) { return rope_axes_call(stream, args, true); }
+
+static NormTrainParams norm_train_params(const flite_norm_args& a) {
+  NormTrainParams p;
+  p.x = a.x;
+  p.ldx = a.ldx;
+  p.y = (bf16_t*)a.y;
+  p.ldy = a.ldy;
+  p.dy = (const bf16_t*)a.dy;
+  p.lddy = a.lddy;
+  p.dx = a.dx;
+  p.lddx = a.lddx;
+  p.w = (const bf16_t*)a.w;
+  p.b = (const bf16_t*)a.b;
+  p.shift = a.shift;
+  p.scale = a.scale;
+  p.mod_seg_stride = a.mod_seg_stride;
+  p.seg_rows = a.seg_rows;
+  p.rows = a.rows;
+  p.D = a.dim;
+  p.eps = a.eps;
+  p.dw = a.dw;
+  p.db = a.db;
+  p.dshift = a.dshift;
+  p.dscale = a.dscale;
+  return p;
+}
+
+int flite_layernorm_modulate(void* stream, const flite_norm_args* args) {
+  FLITE_REQUIRE(args, "flite_layernorm_modulate: null argument");
+  FLITE_REQUIRE(!args->rms, "flite_layernorm_modulate: rms is flite_rmsnorm_modulate's");
+  return layernorm_mod(norm_train_params(*args), args->x_is_bf16 != 0, (hipStream_t)stream);
+}
+
+long flite_norm_bwd_workspace_bytes(long rows, long seg_rows, int dim) {
+  return norm_bwd_workspace_bytes(rows, seg_rows, dim);
+}
+
+int flite_norm_modulate_bwd(void* stream, const flite_norm_args* args, void* workspace, long workspace_bytes) {
+  FLITE_REQUIRE(args, "flite_norm_modulate_bwd: null argument");
+  NormTrainParams p = norm_train_params(*args);
+  p.ws = (float*)workspace;
+  p.ws_bytes = workspace_bytes;
+  return norm_bwd(p, args->x_is_bf16 != 0, args->rms != 0, (hipStream_t)stream);
+}
+
 int flite_rope_tables(void* stream, float* cos_t, float* sin_t, int h, int w, int n_reg, float base,
                       int round_bf16) {
   float inv[64];

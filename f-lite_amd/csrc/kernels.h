@@ -113,6 +113,30 @@ int attn_q256_fwd(const AttnParams& p, hipStream_t stream);
 long attn_q256_workspace_bytes(int B, int H, int max_q, int max_k);
 int attn_q256_set(int mode);  // process-wide route policy: 0 never, 1 always, 2 by prediction (default)
 
+// attn_train.hip: attention that keeps its log-sum-exp, and its backward pass. Packed sequences, no mask; element
+// (row, head, i) of a tensor is at row * x_row + head * x_head + i.
+struct AttnTrainParams {
+  const bf16_t* q = nullptr;  // [total_q][H][dim]
+  const bf16_t* k = nullptr;  // [total_k][HK][dim], head h reads K/V head h / (H / HK)
+  const bf16_t* v = nullptr;
+  bf16_t* o = nullptr;        // written forward, read backward
+  float* lse = nullptr;       // [H][total_q], natural log; written forward, read backward
+  const bf16_t* dout = nullptr;
+  bf16_t* dq = nullptr;
+  bf16_t* dk = nullptr;
+  bf16_t* dv = nullptr;
+  long q_row = 0, q_head = 0, k_row = 0, k_head = 0, v_row = 0, v_head = 0, o_row = 0, o_head = 0;
+  long do_row = 0, do_head = 0, dq_row = 0, dq_head = 0, dk_row = 0, dk_head = 0, dv_row = 0, dv_head = 0;
+  const int* cu_q = nullptr;  // device int32 [B + 1]
+  const int* cu_k = nullptr;
+  int B = 0, H = 0, HK = 0, dim = 0, total_q = 0, total_k = 0;
+  float scale = 1.f;
+  int zero_outside = 0;  // 1: rows that no sequence covers become zeros (lse: -inf); 0: they stay as they were
+};
+int attn_train_fwd(const AttnTrainParams& p, hipStream_t s);
+long attn_train_workspace_bytes(const AttnTrainParams& p);  // -1: the sizes are refused
+int attn_train_bwd(const AttnTrainParams& p, void* ws, long ws_bytes, hipStream_t s);
+
 }  // namespace flite
 
 namespace flite {
@@ -164,6 +188,55 @@ struct RopeNormParams {
   float eps = 1e-6f;
 };
 int rope_qknorm(const RopeNormParams& p, hipStream_t s);
+
+// rope_axes.hip: rotary positions over several axes + optional per-head RMS norm, and the way back
+struct RopeAxesParams {
+  const void* x = nullptr;  // fp32 or bf16 heads: row r, head h at r * x_row + h * x_head (backward: the gradient dy)
+  long x_row = 0, x_head = 0;
+  void* out = nullptr;      // same type; may be x
+  long o_row = 0, o_head = 0;
+  const void* y = nullptr;  // backward with the norm: the forward pass's output
+  long y_row = 0, y_head = 0;
+  float* rstd = nullptr;    // with the norm: [rows][heads], written forward, read backward
+  const void* positions = nullptr;  // [tokens][axes] int32, or fp32 with pos_is_f32; row r is token r % tokens
+  int pos_is_f32 = 0, axes = 0;
+  long tokens = 0, rows = 0;
+  int heads = 0, rope_heads = 0;  // heads [0, rope_heads) are turned, all are normed
+  int dim = 0;
+  float eps = 1e-6f;
+};
+int rope_axes(const RopeAxesParams& p, const int* axis_pairs, const double* bases, bool x_bf16, bool interleaved,
+              bool norm, bool bwd, hipStream_t s);
+
+// norm_train.hip: layer norm + modulate, and the backward pass of layer / RMS norm + modulate
+struct NormTrainParams {
+  const void* x = nullptr;  // fp32 or bf16 rows
+  long ldx = 0;
+  bf16_t* y = nullptr;      // forward: bf16 rows
+  long ldy = 0;
+  const bf16_t* dy = nullptr;  // backward: bf16 rows
+  long lddy = 0;
+  void* dx = nullptr;          // backward: rows of x's type
+  long lddx = 0;
+  const bf16_t* w = nullptr;  // [D] or null
+  const bf16_t* b = nullptr;  // [D] or null (layer norm)
+  const float* shift = nullptr;  // modulation rows (fp32), one per segment of seg_rows rows (0: one segment), or null
+  const float* scale = nullptr;
+  long mod_seg_stride = 0;
+  long seg_rows = 0, rows = 0;
+  int D = 0;
+  float eps = 1e-6f;
+  // backward: fp32 gradients, each null where it is not wanted: [D], [D], [segments][D], [segments][D]
+  float* dw = nullptr;
+  float* db = nullptr;
+  float* dshift = nullptr;
+  float* dscale = nullptr;
+  float* ws = nullptr;  // norm_bwd_workspace_bytes; every byte that is read was written by the same call
+  long ws_bytes = 0;
+};
+int layernorm_mod(const NormTrainParams& p, bool x_bf16, hipStream_t s);
+int norm_bwd(const NormTrainParams& p, bool x_bf16, bool rms, hipStream_t s);
+long norm_bwd_workspace_bytes(long rows, long seg_rows, int D);
 
 int patchify(const void* lat, bool in_bf16, bf16_t* out, int Bi, int C, int H, int W, int P, int dup, hipStream_t s);
 int fill_registers(void* x, bool x16, const bf16_t* reg, int B, int T, int R, int D, hipStream_t s);

@@ -125,6 +125,102 @@ int flite_rope_qknorm(void* stream, void* x, long ldx, long rows, int heads, int
                       const float* sin_t, long tokens_per_seq, float eps);
 
 /* ---------------------------------------------------------------------------------------------
+ * Training operators of the DiT block: the backward pass of the operators above, and the forward passes that go with
+ * it. All are deterministic (no atomics), allocate nothing and can be captured in a graph; a workspace needs no
+ * initialisation and may be reused by the next launch on the same stream.
+ * ------------------------------------------------------------------------------------------- */
+
+/*
+ * Attention over packed sequences, no mask: out = softmax(scale q k^T) v per sequence and head. Element (row, head, i)
+ * of a tensor is at row * x_row + head * x_head + i (elements; strides multiples of 8, pointers 16-byte aligned, row
+ * strides head_dim .. 2^22). Query head h reads K/V head h / (heads / kv_heads). Sequence b holds rows
+ * cu_q[b] .. cu_q[b + 1] - 1 of q and cu_k[b] .. cu_k[b + 1] - 1 of k and v; either may be empty. A query whose
+ * sequence has no keys gives out = 0 and lse = -inf. head_dim is 64, 128 or 256.
+ */
+typedef struct flite_attn_train {
+  const void* q;        /* bf16 [total_q][heads][head_dim] */
+  const void* k;        /* bf16 [total_k][kv_heads][head_dim] */
+  const void* v;
+  void* out;            /* bf16, as q: written by flite_attn_lse_fwd, read by flite_attn_lse_bwd */
+  float* lse;           /* fp32 [heads][total_q], log sum exp of the scaled scores: written / read likewise */
+  const void* dout;     /* backward only, from here: bf16 gradient of out */
+  void* dq;             /* bf16 gradients; dk and dv are sums over the heads that share a K/V head */
+  void* dk;
+  void* dv;
+  long q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+  long dout_row, dout_head, dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
+  const int* cu_q;      /* device int32 [batch + 1] */
+  const int* cu_k;
+  int batch, heads, kv_heads, head_dim, total_q, total_k;
+  float scale;
+  int zero_outside;     /* rows outside all sequences: 1 = zeros in the outputs (lse: -inf), 0 = they stay as they are */
+} flite_attn_train;
+
+/* Writes out and lse. Training counterpart of
+ * flash_attn_varlen_func (reference f_lite/model.py:203-210). */
+int flite_attn_lse_fwd(void* stream, const flite_attn_train* args);
+/* Workspace of the backward pass for these sizes (256-byte aligned device memory); -1: the sizes are refused. */
+long flite_attn_lse_bwd_workspace_bytes(const flite_attn_train* args);
+/* dq, dk, dv of sum(out * dout), with the probabilities made again from q, k and lse. */
+int flite_attn_lse_bwd(void* stream, const flite_attn_train* args, void* workspace, long workspace_bytes);
+
+/*
+ * Rotary positions over 1 to 8 axes (time, height, width, ...), then (norm = 1) the per-head RMS norm of QKNorm
+ * (reference f_lite/model.py:115-126), on fp32 or bf16 heads of head_dim (a multiple of 16, at most 256). Axis a has
+ * axis_pairs[a] pairs; its pair i turns by -position[a] * bases[a]^(-i / axis_pairs[a]) (the sign of model.py:403-414;
+ * negative positions turn the other way). The pairs of all axes follow one another and add up to a multiple of 8; pair
+ * j is elements (j, j + pairs) or, interleaved, (2 j, 2 j + 1); elements past them are not turned. Row r takes the
+ * positions of token r % tokens. Heads [0, rope_heads) are turned, all are normed.
+ * Forward: out = (norm ? rstd : 1) * rot(x), rstd [rows][heads] fp32 written. Backward: x holds the gradient of out,
+ * y the forward pass's out, rstd as written (both with norm only); out becomes the gradient of x. out may be x.
+ */
+typedef struct flite_rope_axes_args {
+  const void* x;
+  void* out;               /* the type of x */
+  const void* y;           /* backward with norm */
+  float* rstd;             /* with norm */
+  const void* positions;   /* device [tokens][axes], int32 or (positions_f32) fp32 */
+  const int* axis_pairs;   /* host [axes] */
+  const double* bases;     /* host [axes] */
+  long x_row, x_head, out_row, out_head, y_row, y_head; /* elements, multiples of 8 */
+  long rows, tokens;
+  int axes, heads, rope_heads, head_dim;
+  int is_bf16, positions_f32, interleaved, norm;
+  float eps;
+} flite_rope_axes_args;
+int flite_rope_axes_fwd(void* stream, const flite_rope_axes_args* args);
+int flite_rope_axes_bwd(void* stream, const flite_rope_axes_args* args);
+
+/*
+ * Layer norm + modulate, y = ((x - mean) * rstd * w + b) * (1 + scale) + shift to bf16 rows, and the backward pass of
+ * it (rms = 0) and of flite_rmsnorm_modulate (rms = 1, no b). x is fp32 or bf16, dim a multiple of 8 up to 8192, every
+ * row 16-byte aligned (strides multiples of 8). w and b are bf16 [dim] or NULL. shift and scale are fp32 rows, one per
+ * segment of seg_rows rows (seg_rows = 0: one segment), or NULL. Backward: dx has the type of x; the fp32 gradients dw,
+ * db [dim], dshift, dscale [segments][dim] are written where they are not NULL (all rows' sums in 32 bits).
+ */
+typedef struct flite_norm_args {
+  const void* x;
+  void* y;              /* forward: bf16 */
+  const void* dy;       /* backward: bf16 */
+  void* dx;
+  const void* w;
+  const void* b;
+  const float* shift;   /* forward */
+  const float* scale;
+  float* dw;
+  float* db;
+  float* dshift;
+  float* dscale;
+  long ldx, ldy, lddy, lddx, mod_seg_stride, seg_rows, rows;
+  int dim, x_is_bf16, rms;
+  float eps;
+} flite_norm_args;
+int flite_layernorm_modulate(void* stream, const flite_norm_args* args);
+/* Workspace of flite_norm_modulate_bwd when any of dw, db, dshift, dscale is wanted (16-byte aligned). */
+long flite_norm_bwd_workspace_bytes(long rows, long seg_rows, int dim);
+int flite_norm_modulate_bwd(void* stream, const flite_norm_args* args, void* workspace, long workspace_bytes);
+
+/* ---------------------------------------------------------------------------------------------
  * MXFP8 (fp8 weights + activations). Elements OCP e4m3fn, one E8M0 scale per 32
  * consecutive K elements: e = ceil(log2(amax/448)), q = RNE(clamp(x * 2^-e, +-448)). Scale arrays are
  * "k-tile major": scales[K/128][rows_pad][4] bytes (rows_pad a multiple of 256, >= rows; pad rows are never
