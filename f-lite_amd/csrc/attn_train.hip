@@ -41,7 +41,8 @@ struct TrainDev {
   int tiles_q, tiles_k;    // upper bounds of the packed batch's 128-row tiles
   int split_q, split_k;    // ranges that a query / key workgroup's sweep is cut into
   int n_key_blocks;        // backward: the first blocks of the launch are key workgroups
-  float2* ld;              // [H][total_q] (lse * log2 e, delta)
+  float* lse2;             // [H][total_q] lse * log2 e
+  float* delta;            // [H][total_q]
   float* part_q;           // [split_q][total_q][H][D] fp32, with split_q > 1
   float* part_k;           // [split_k][total_k][HK][D]
   float* part_v;
@@ -304,162 +305,537 @@ __global__ __launch_bounds__(kThreads) void attn_delta_kernel(TrainDev d) {
     const long at = (long)h * p.total_q + row;
     const float lse = p.lse[at];
     // a row without keys (or with -inf scores alone) has P = 0: exp2(x - inf)
-    d.ld[at] = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e, s);
+    d.lse2[at] = lse == -INFINITY ? INFINITY : lse * kLog2e;
+    d.delta[at] = s;
   }
 }
 
-// A query workgroup: dq of 128 queries of head h
+// Two kinds of waves. A wave of 32 stationary rows would need every LDS byte for one MFMA each and sit on the LDS read
+// rate (128 B per clock and CU); 64 rows need twice the registers. So the waves of a pair share 64 stationary rows (two
+// blocks of 32) and split the products: each A fragment read from LDS feeds both blocks.
+//   key workgroup:   wave 0: S, P, dv    wave 1: dP, dS = P (dP - delta), dk      (P handed over in fp32)
+//   query workgroup: wave 0: S, dP, dS   wave 1: dq                               (dS handed over as two bf16, hi + lo)
+// All four have 64 MFMAs per 32 swept rows. dS enters dq as hi + lo (2^-17): its rows sum to 0, so where keys share a
+// direction, that direction cancels in dq and a single rounding's error would stay (dq 1.7 times as far from the exact
+// gradient as one final rounding to bf16 is, against 1.4 for dk and dv).
+
 template <int D>
-__device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem) {
-  const AttnTrainParams& p = d.p;
-  constexpr int TB = TR * D * 2;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int lq = lane & 31, hh = lane >> 5;
-  const int part = v % d.split_q;
-  v /= d.split_q;
-  const int h = v / d.tiles_q;
-  int b, row0;
-  if (!find_tile(p.cu_q, p.B, p.total_q, v % d.tiles_q, &b, &row0)) return;
-  int q_start, q_len, k_start, k_len;
-  seq_range(p.cu_q, b, p.total_q, &q_start, &q_len);
-  seq_range(p.cu_k, b, p.total_k, &k_start, &k_len);
-  const int hk = h / (p.H / p.HK);
-  const int row = row0 + wave * 32 + lq;
-  const bool live = row < q_len;
-  const int rc = q_start + min(row, q_len - 1);
-
-  bf16x8 qf[D / 16], df[D / 16];
-  load_frags<D>(p.q + (long)rc * p.q_row + (long)h * p.q_head, hh, qf);
-  load_frags<D>(p.dout + (long)rc * p.do_row + (long)h * p.do_head, hh, df);
-  const float2 ld = d.ld[(long)h * p.total_q + rc];
-  const LaneOff<D> off(lane);
-  const unsigned lds0 = lds_addr_of(smem);
-  const bf16_t* kp = p.k + (long)k_start * p.k_row + (long)hk * p.k_head;
-  const bf16_t* vp = p.v + (long)k_start * p.v_row + (long)hk * p.v_head;
-  auto fetch = [&](int t, int buf) {
-    const long r = (long)t * TR;
-    stage<D>(kp + r * p.k_row, p.k_row, k_len - r, lds0 + buf * 2 * TB, wave, lane);
-    stage<D>(vp + r * p.v_row, p.v_row, k_len - r, lds0 + buf * 2 * TB + TB, wave, lane);
-  };
-  const float sl2 = p.scale * kLog2e;
-  f32x16 acc[D / 32];
+struct Stage {
+  static constexpr int BYTES = 32 * D * 2;  // 32 swept rows
+  static constexpr int PIECES = D / 64;     // 1-KiB copies per wave
+  int voff[PIECES];                         // this lane's source bytes in the stage
+  __device__ __forceinline__ void init(long stride, int wave, int lane) {
+    constexpr int CPR = D / 8;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
-
-  const int all = (k_len + TR - 1) / TR, per = (all + d.split_q - 1) / d.split_q;
-  const int t0 = min(part * per, all), t1 = min(t0 + per, all);
-  if (t0 < t1) fetch(t0, 0);
-  TILE_SYNC();
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    if (t + 1 < t1) fetch(t + 1, buf ^ 1);
-    const char* kt = smem + buf * 2 * TB;
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      f32x16 s = row_product<D>(kt + hf * 32 * D * 2, off, qf);
-      const f32x16 dp = row_product<D>(kt + TB + hf * 32 * D * 2, off, df);
-      // keys past the end are zero rows: they add nothing to dq, but exp2(-lse) could overflow (inf * 0)
-      const int k_left = k_len - t * TR - hf * 32 - 4 * hh;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sl2, -ld.x)) * (dp[r] - ld.y);
-        s[r] = 8 * (r >> 2) + (r & 3) < k_left ? e : 0.f;
-      }
-      tr_product<D>(kt + hf * 32 * D * 2, off, s, acc);
+    for (int i = 0; i < PIECES; ++i) {
+      const int pos = (wave * PIECES + i) * 64 + lane;
+      const int row = pos / CPR, ch = (pos % CPR) ^ swz<D>(row);
+      voff[i] = (int)(row * stride * 2) + ch * 16;
     }
-    TILE_SYNC();
   }
-  if (d.split_q > 1)
-    store_part<D>(d.part_q + (((long)part * p.total_q + rc) * p.H + h) * D, acc, p.scale, hh, live);
-  else
-    store_row<D>(p.dq + (long)rc * p.dq_row + (long)h * p.dq_head, acc, p.scale, hh, live);
+};
+
+// Buffer range of the rows left in a sequence (0: the stage becomes zeros)
+__device__ __forceinline__ unsigned rows_bytes(int rows_left, long stride) {
+  return (unsigned)min((long)max(rows_left, 0) * stride * 2, 0x7fffffffL);
 }
 
-// A key workgroup: dk and dv of 128 keys of K/V head hk
+// 4-B-per-lane LDS copy of 32 floats (lanes 32.. read past the range: zeros behind them)
+__device__ __forceinline__ void blds4(const i32x4& rsrc, unsigned voff, unsigned lds_addr) {
+  unsigned keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %3\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dword %1, %2, 0 offen lds\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(voff), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(lds_addr))
+      : "memory");
+}
+
+// The step barrier: own LDS writes and copies done, then everyone's
+__device__ __forceinline__ void step_sync() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// LDS offsets of a lane's reads in a stage; k-steps s >= 8 and column tiles dt >= 4 are 256 B further (the XOR stays
+// within 16 chunks)
+template <int D>
+struct ReadOff {
+  static constexpr int NR = D / 16 < 8 ? D / 16 : 8, NT = D / 32 < 4 ? D / 32 : 4;
+  int row[NR];
+  int tr[2][NT];
+  __device__ __forceinline__ void init(int lane) {
+    const int lq = lane & 31, hh = lane >> 5;
+#pragma unroll
+    for (int s = 0; s < NR; ++s) row[s] = lq * D * 2 + (((2 * s + hh) ^ swz<D>(lq)) << 4);
+    const int G = lane >> 4, vq = (lane & 15) >> 2, vp = lane & 3;
+    const int r0 = 4 * (G >> 1) + vq;
+#pragma unroll
+    for (int o = 0; o < 2; ++o)
+#pragma unroll
+      for (int dt = 0; dt < NT; ++dt)
+        tr[o][dt] = (r0 + 8 * o) * D * 2 + (((4 * dt + 2 * (G & 1) + (vp >> 1)) ^ swz<D>(r0 + 8 * o)) << 4) + (vp & 1) * 8;
+  }
+  __device__ __forceinline__ bf16x8 read_row(const char* st, int s) const {
+    return *(const bf16x8*)(st + row[s % NR] + 256 * (s / NR));
+  }
+  __device__ __forceinline__ bf16x8 read_tr(const char* st, int ks, int dt) const {
+    const char* b = st + ks * 16 * D * 2 + 256 * (dt / NT);
+    const s16x4 lo = ds_tr16(b + tr[0][dt % NT]);
+    const s16x4 hi = ds_tr16(b + tr[1][dt % NT]);
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+
+#define FENCE() __builtin_amdgcn_sched_barrier(0)
+
+// acc[n] (VGPRs) = stage rows . stationary block n; hook(s) after each k-step
+template <int D, typename Hook>
+__device__ __forceinline__ void row_phase(const char* st, const ReadOff<D>& o, const bf16x8 (&f)[2][D / 16],
+                                          f32x16 (&acc)[2], Hook hook) {
+  constexpr int NS = D / 16, AHEAD = 3;
+  bf16x8 a[NS];
+#pragma unroll
+  for (int s = 0; s < AHEAD; ++s) a[s] = o.read_row(st, s);
+  FENCE();
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    if (s + AHEAD < NS) a[s + AHEAD] = o.read_row(st, s + AHEAD);
+    FENCE();
+    if (s == 0) {
+      mfma_sv_first(acc[0], a[0], f[0][0]);
+      mfma_sv_first(acc[1], a[0], f[1][0]);
+    } else {
+      mfma_sv(acc[0], a[s], f[0][s]);
+      mfma_sv(acc[1], a[s], f[1][s]);
+    }
+    FENCE();
+    hook(s);
+    FENCE();
+  }
+  mfma_read_fence(acc[0], acc[1]);
+}
+
+// acc[n][dt] (AGPRs) += (stage columns)^T . b[n]; hook(m) after each of the 2 D / 32 column reads
+template <int D, typename Hook>
+__device__ __forceinline__ void tr_phase(const char* st, const ReadOff<D>& o, bf16x8 (&b)[2][2],
+                                         f32x16 (&acc)[2][D / 32], Hook hook) {
+  constexpr int ND = D / 32, AHEAD = 2;
+  bf16x8 a[2 * ND];
+#pragma unroll
+  for (int m = 0; m < AHEAD; ++m) a[m] = o.read_tr(st, m / ND, m % ND);
+  FENCE();
+#pragma unroll
+  for (int m = 0; m < 2 * ND; ++m) {
+    if (m + AHEAD < 2 * ND) a[m + AHEAD] = o.read_tr(st, (m + AHEAD) / ND, (m + AHEAD) % ND);
+    FENCE();
+    mfma_o<false>(acc[0][m % ND], a[m], b[0][m / ND]);
+    mfma_o<false>(acc[1][m % ND], a[m], b[1][m / ND]);
+    FENCE();
+    hook(m);
+    FENCE();
+  }
+}
+
+template <int ND>
+__device__ __forceinline__ void acc_zero(f32x16 (&acc)[2][ND]) {
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[n][i][r] = 0.f;
+}
+
+// MFMA writes of the accumulators -> their readers
+template <int ND>
+__device__ __forceinline__ void acc_fence(f32x16 (&acc)[2][ND]) {
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" ::: "memory");
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int i = 0; i < ND; ++i) asm volatile("" : "+a"(acc[n][i]));
+}
+
+__device__ __forceinline__ unsigned pack_bf(float lo, float hi) {
+  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+  const bf16x2 v = {(__bf16)lo, (__bf16)hi};
+  return __builtin_bit_cast(unsigned, v);
+}
+
+// LDS of a key workgroup: q ring of 4 stages, dout ring of 2, P double-buffered, lse ring of 4, delta ring of 2; of a
+// query workgroup: k ring of 4, v ring of 2, dS double-buffered
+template <int D>
+struct Lds {
+  static constexpr int A = 0, B = 4 * Stage<D>::BYTES, X = B + 2 * Stage<D>::BYTES, XBYTES = 16384;
+  static constexpr int LSE = X + 2 * XBYTES, DELTA = LSE + 4 * 256, TOTAL = DELTA + 2 * 256;
+};
+
+// A key workgroup: dk and dv of 128 keys of K/V head hk. Step i: wave 0 makes S(i + 1), then dv += dout(i)^T P(i) while
+// it makes P(i + 1); wave 1 makes dP(i), then dk += q(i - 1)^T dS(i - 1) while it makes dS(i) from P(i).
 template <int D>
 __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) {
   const AttnTrainParams& p = d.p;
-  constexpr int TB = TR * D * 2;
-  constexpr int LDB = TR * 8;  // (lse, delta) of a tile
+  using L = Lds<D>;
+  constexpr int ND = D / 32, SB = Stage<D>::BYTES, EPH = 32 / (2 * ND);  // scores per hook
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int lq = lane & 31, hh = lane >> 5;
+  const int lq = lane & 31, hh = lane >> 5, pair = wave >> 1;
   const int part = v % d.split_k;
   v /= d.split_k;
   const int hk = v / d.tiles_k;
   int b, row0;
   if (!find_tile(p.cu_k, p.B, p.total_k, v % d.tiles_k, &b, &row0)) return;
+  b = __builtin_amdgcn_readfirstlane(b);
+  row0 = __builtin_amdgcn_readfirstlane(row0);
   int q_start, q_len, k_start, k_len;
   seq_range(p.cu_q, b, p.total_q, &q_start, &q_len);
   seq_range(p.cu_k, b, p.total_k, &k_start, &k_len);
   const int group = p.H / p.HK;
-  const int row = row0 + wave * 32 + lq;
-  const bool live = row < k_len;
-  const int rc = k_start + min(row, k_len - 1);
+  const int tiles = (q_len + 31) / 32;  // stages of one head
+  const int all = tiles * group, per = (all + d.split_k - 1) / d.split_k;
+  const int t0 = min(part * per, all), n = min(per, all - t0);
 
-  bf16x8 kf[D / 16], vf[D / 16];
-  load_frags<D>(p.k + (long)rc * p.k_row + (long)hk * p.k_head, hh, kf);
-  load_frags<D>(p.v + (long)rc * p.v_row + (long)hk * p.v_head, hh, vf);
-  const LaneOff<D> off(lane);
-  const unsigned lds0 = lds_addr_of(smem);
-  const int tiles = (q_len + TR - 1) / TR;  // tiles of one head
-  char* const ld_s = smem + 4 * TB;
-  // tile i of the sweep over the group's heads and their query tiles. Rows past the sequence end are zeros, (lse,
-  // delta) included: P = exp2(0 - 0) = 1 meets zero rows of q and dout and adds nothing
-  auto fetch = [&](int i, int buf) {
-    const int h = hk * group + i / tiles;
-    const long r = (long)(i % tiles) * TR;
-    const long at = q_start + r;
-    stage<D>(p.q + at * p.q_row + (long)h * p.q_head, p.q_row, q_len - r, lds0 + buf * 2 * TB, wave, lane);
-    stage<D>(p.dout + at * p.do_row + (long)h * p.do_head, p.do_row, q_len - r, lds0 + buf * 2 * TB + TB, wave, lane);
-    if (threadIdx.x < TR) {
-      float2 x = make_float2(0.f, 0.f);
-      if (r + (int)threadIdx.x < q_len) x = d.ld[(long)h * p.total_q + at + threadIdx.x];
-      *(float2*)(ld_s + buf * LDB + threadIdx.x * 8) = x;
+  ReadOff<D> off;
+  off.init(lane);
+  Stage<D> sq, sd;
+  sq.init(p.q_row, wave, lane);
+  sd.init(p.do_row, wave, lane);
+  const unsigned lds0 = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_addr_of(smem));
+  const unsigned wlds = lds0 + wave * Stage<D>::PIECES * 1024;
+  const unsigned ld_off = lane < 32 ? lane * 4 : 0x7ffffff0u;
+  // stage j of this range: rows (t0 + j) % tiles * 32 .. of head hk * group + (t0 + j) / tiles. Rows past the sequence
+  // end and stages outside 0 .. n - 1 are zeros, lse and delta included: P = exp2(0 - 0) = 1 meets zero rows
+  auto at = [&](int j, int* h, int* r) {
+    const int t = t0 + j;
+    const bool live = j >= 0 && j < n;
+    *h = live ? hk * group + t / tiles : 0;
+    *r = live ? t % tiles * 32 : 0;
+    return live ? q_len - *r : 0;  // rows left
+  };
+  auto copy_q = [&](int j) {  // and lse
+    int h, r;
+    const int left = at(j, &h, &r);
+    const i32x4 rs = make_rsrc(p.q + (long)(q_start + r) * p.q_row + (long)h * p.q_head, rows_bytes(left, p.q_row));
+#pragma unroll
+    for (int i = 0; i < Stage<D>::PIECES; ++i) blds16(rs, sq.voff[i], wlds + L::A + (j & 3) * SB + i * 1024);
+    if (wave == 0)
+      blds4(make_rsrc(d.lse2 + (long)h * p.total_q + q_start + r, (unsigned)max(min(left, 32), 0) * 4), ld_off,
+            lds0 + L::LSE + (j & 3) * 256);
+  };
+  auto copy_do = [&](int j) {  // and delta
+    int h, r;
+    const int left = at(j, &h, &r);
+    const i32x4 rs =
+        make_rsrc(p.dout + (long)(q_start + r) * p.do_row + (long)h * p.do_head, rows_bytes(left, p.do_row));
+#pragma unroll
+    for (int i = 0; i < Stage<D>::PIECES; ++i) blds16(rs, sd.voff[i], wlds + L::B + (j & 1) * SB + i * 1024);
+    if (wave == 1)
+      blds4(make_rsrc(d.delta + (long)h * p.total_q + q_start + r, (unsigned)max(min(left, 32), 0) * 4), ld_off,
+            lds0 + L::DELTA + (j & 1) * 256);
+  };
+
+  f32x16 acc[2][ND];
+  acc_zero<ND>(acc);
+  if (n > 0) {
+    copy_q(-1);
+    copy_q(0);
+    copy_do(0);
+    copy_q(1);
+    // stationary rows: k for wave 0, v for wave 1
+    bf16x8 f[2][D / 16];
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+      const long rc = k_start + min(row0 + pair * 64 + nb * 32 + lq, k_len - 1);
+      load_frags<D>(wave & 1 ? p.v + rc * p.v_row + (long)hk * p.v_head : p.k + rc * p.k_row + (long)hk * p.k_head, hh,
+                    f[nb]);
+    }
+    bf16x8 bc[2][2];  // P (wave 0) or dS (wave 1) of the stage that the tr phase takes, B operands
+    u32x4 bn[2][2];   // of the next
+    f32x16 s[2];
+    const float sl2 = p.scale * kLog2e;
+    char* const xch = smem + L::X + pair * 8192 + lane * 16;  // [buffer][pair][block][r4][lane] f32x4
+    auto none = [](int) {};
+    step_sync();
+    if ((wave & 1) == 0) {
+      // score e of stage j: group r4 = e >> 3 (rows 8 r4 + 4 hh + 0..3), block (e >> 2) & 1
+      f32x4 lse;
+      auto prob = [&](int j, int e) {
+        const int r4 = e >> 3, nb = (e >> 2) & 1, i = e & 3, r = 4 * r4 + i;
+        if ((e & 7) == 0) lse = *(const f32x4*)(smem + L::LSE + (j & 3) * 256 + (8 * r4 + 4 * hh) * 4);
+        s[nb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][r], sl2, -lse[i]));
+        if (i & 1) bn[nb][r >> 3][(r & 7) >> 1] = pack_bf(s[nb][r - 1], s[nb][r]);
+        if (i == 3)
+          *(f32x4*)(xch + (j & 1) * L::XBYTES + (nb * 4 + r4) * 1024) = f32x4{s[nb][r - 3], s[nb][r - 2], s[nb][r - 1], s[nb][r]};
+      };
+      auto next = [&]() {
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) bc[nb][ks] = __builtin_bit_cast(bf16x8, bn[nb][ks]);
+      };
+      row_phase<D>(smem + L::A, off, f, s, none);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) prob(0, e);
+      next();
+      step_sync();
+      for (int i = 0; i < n; ++i) {
+        copy_q(i + 2);
+        copy_do(i + 1);
+        row_phase<D>(smem + L::A + ((i + 1) & 3) * SB, off, f, s, none);
+        tr_phase<D>(smem + L::B + (i & 1) * SB, off, bc, acc, [&](int m) {
+#pragma unroll
+          for (int e = 0; e < EPH; ++e) prob(i + 1, m * EPH + e);
+        });
+        next();
+        step_sync();
+      }
+      step_sync();
+    } else {
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) bc[nb][ks] = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
+      step_sync();
+      f32x4 del, pr;
+      for (int i = 0; i <= n; ++i) {
+        if (i < n) {
+          copy_q(i + 2);
+          copy_do(i + 1);
+        }
+        row_phase<D>(smem + L::B + (i & 1) * SB, off, f, s, none);
+        tr_phase<D>(smem + L::A + ((i - 1) & 3) * SB, off, bc, acc, [&](int m) {
+#pragma unroll
+          for (int e0 = 0; e0 < EPH; ++e0) {
+            const int e = m * EPH + e0;
+            const int r4 = e >> 3, nb = (e >> 2) & 1, k = e & 3, r = 4 * r4 + k;
+            if ((e & 7) == 0) del = *(const f32x4*)(smem + L::DELTA + (i & 1) * 256 + (8 * r4 + 4 * hh) * 4);
+            if (k == 0) pr = *(const f32x4*)(xch + (i & 1) * L::XBYTES + (nb * 4 + r4) * 1024);
+            s[nb][r] = pr[k] * (s[nb][r] - del[k]);
+            if (k & 1) bn[nb][r >> 3][(r & 7) >> 1] = pack_bf(s[nb][r - 1], s[nb][r]);
+          }
+        });
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) bc[nb][ks] = __builtin_bit_cast(bf16x8, bn[nb][ks]);
+        step_sync();
+      }
+    }
+  }
+  acc_fence<ND>(acc);
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb) {
+    const int row = row0 + pair * 64 + nb * 32 + lq;
+    const bool live = row < k_len;
+    const long rc = k_start + min(row, k_len - 1);
+    if (d.split_k > 1) {
+      const long to = (((long)part * p.total_k + rc) * p.HK + hk) * D;
+      store_part<D>((wave & 1 ? d.part_k : d.part_v) + to, acc[nb], wave & 1 ? p.scale : 1.f, hh, live);
+    } else if (wave & 1) {
+      store_row<D>(p.dk + rc * p.dk_row + (long)hk * p.dk_head, acc[nb], p.scale, hh, live);
+    } else {
+      store_row<D>(p.dv + rc * p.dv_row + (long)hk * p.dv_head, acc[nb], 1.f, hh, live);
+    }
+  }
+}
+
+// A query workgroup: dq of 128 queries of head h. Step i: wave 0 makes S and dP of stage i + 1 while it makes dS(i);
+// wave 1 adds k(i - 1)^T dS(i - 1) to dq.
+template <int D>
+__device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem) {
+  const AttnTrainParams& p = d.p;
+  using L = Lds<D>;
+  constexpr int ND = D / 32, NS = D / 16, SB = Stage<D>::BYTES;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int lq = lane & 31, hh = lane >> 5, pair = wave >> 1;
+  const int part = v % d.split_q;
+  v /= d.split_q;
+  const int h = v / d.tiles_q;
+  int b, row0;
+  if (!find_tile(p.cu_q, p.B, p.total_q, v % d.tiles_q, &b, &row0)) return;
+  b = __builtin_amdgcn_readfirstlane(b);
+  row0 = __builtin_amdgcn_readfirstlane(row0);
+  int q_start, q_len, k_start, k_len;
+  seq_range(p.cu_q, b, p.total_q, &q_start, &q_len);
+  seq_range(p.cu_k, b, p.total_k, &k_start, &k_len);
+  const int hk = h / (p.H / p.HK);
+  const int all = (k_len + 31) / 32, per = (all + d.split_q - 1) / d.split_q;
+  const int t0 = min(part * per, all), n = min(per, all - t0);
+
+  ReadOff<D> off;
+  off.init(lane);
+  Stage<D> sk, sv;
+  sk.init(p.k_row, wave, lane);
+  sv.init(p.v_row, wave, lane);
+  const unsigned lds0 = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_addr_of(smem));
+  const unsigned wlds = lds0 + wave * Stage<D>::PIECES * 1024;
+  const bf16_t* kp = p.k + (long)k_start * p.k_row + (long)hk * p.k_head;
+  const bf16_t* vp = p.v + (long)k_start * p.v_row + (long)hk * p.v_head;
+  auto copy = [&](int j) {  // k and v rows of stage j of this range; zeros past its end
+    const int r = (t0 + j) * 32, left = j < n ? k_len - r : 0;
+    const i32x4 krs = make_rsrc(kp + (long)r * p.k_row, rows_bytes(left, p.k_row));
+    const i32x4 vrs = make_rsrc(vp + (long)r * p.v_row, rows_bytes(left, p.v_row));
+#pragma unroll
+    for (int i = 0; i < Stage<D>::PIECES; ++i) {
+      blds16(krs, sk.voff[i], wlds + L::A + (j & 3) * SB + i * 1024);
+      blds16(vrs, sv.voff[i], wlds + L::B + (j & 1) * SB + i * 1024);
     }
   };
-  const float sl2 = p.scale * kLog2e;
-  f32x16 dk[D / 32], dv[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
 
-  const int all = tiles * group, per = (all + d.split_k - 1) / d.split_k;
-  const int t0 = min(part * per, all), t1 = min(t0 + per, all);
-  if (t0 < t1) fetch(t0, 0);
-  TILE_SYNC();
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    if (t + 1 < t1) fetch(t + 1, buf ^ 1);
-    const char* qt = smem + buf * 2 * TB;
+  char* const xch = smem + L::X + pair * 8192 + lane * 16;  // [buffer][pair][block][hi 2, lo 2][lane] 16 B
+  if ((wave & 1) == 0) {
+    if (n <= 0) return;  // wave 1 stores the zeros
+    copy(0);
+    copy(1);
+    bf16x8 qf[2][NS], df[2][NS];
+    float lse[2], del[2];
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const char* qh = qt + hf * 32 * D * 2;
-      f32x16 s = row_product<D>(qh, off, kf);
-      f32x16 dp = row_product<D>(qh + TB, off, vf);
-      const f32x4* ld = (const f32x4*)(ld_s + buf * LDB + (hf * 32 + 4 * hh) * 8);
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {  // rows 8 (r >> 2) + 4 hh + (r & 3): two per 16 B
-        const f32x4 x = ld[4 * (r >> 2) + ((r & 3) >> 1)];
-        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sl2, -x[0]));
-        s[r + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + 1], sl2, -x[2]));
-        dp[r] = s[r] * (dp[r] - x[1]);
-        dp[r + 1] = s[r + 1] * (dp[r + 1] - x[3]);
-      }
-      tr_product<D>(qh + TB, off, s, dv);
-      tr_product<D>(qh, off, dp, dk);
+    for (int nb = 0; nb < 2; ++nb) {
+      const long rc = q_start + min(row0 + pair * 64 + nb * 32 + lq, q_len - 1);
+      load_frags<D>(p.q + rc * p.q_row + (long)h * p.q_head, hh, qf[nb]);
+      load_frags<D>(p.dout + rc * p.do_row + (long)h * p.do_head, hh, df[nb]);
+      lse[nb] = d.lse2[(long)h * p.total_q + rc];
+      del[nb] = d.delta[(long)h * p.total_q + rc];
     }
-    TILE_SYNC();
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        asm volatile("" : "+a"(qf[nb][s]));
+        asm volatile("" : "+a"(df[nb][s]));
+      }
+    asm volatile("s_nop 4" ::: "memory");
+    const float sl2 = p.scale * kLog2e;
+    f32x16 sa[2], da[2], sb[2], db[2];
+    u32x4 hi, lo;
+    // element e (block e >> 4, score e & 15) of stage j's dS, from its S and dP
+    auto ds_elem = [&](int j, f32x16 (&s)[2], f32x16 (&dp)[2], int e) {
+      const int nb = e >> 4, r = e & 15;
+      s[nb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][r], sl2, -lse[nb])) * (dp[nb][r] - del[nb]);
+      if (r & 1) {
+        const int w = (r & 7) >> 1;
+        const float x = s[nb][r - 1], y = s[nb][r];
+        const unsigned h2 = pack_bf(x, y);
+        hi[w] = h2;
+        lo[w] = pack_bf(x - __uint_as_float(h2 << 16), y - __uint_as_float(h2 & 0xffff0000u));
+        if (w == 3) {
+          char* to = xch + (j & 1) * L::XBYTES + nb * 4096 + (r >> 3) * 1024;
+          *(u32x4*)to = hi;
+          *(u32x4*)(to + 2048) = lo;
+        }
+      }
+    };
+    // S and dP of stage j into (s, dp); hook(m) after each of the 2 NS fragment reads
+    auto products = [&](int j, f32x16 (&s)[2], f32x16 (&dp)[2], auto hook) {
+      const char* ks = smem + L::A + (j & 3) * SB;
+      const char* vs = smem + L::B + (j & 1) * SB;
+      constexpr int AHEAD = 4;
+      bf16x8 a[2 * NS];
+      auto rd = [&](int m) { a[m] = off.read_row(m & 1 ? vs : ks, m >> 1); };
+#pragma unroll
+      for (int m = 0; m < AHEAD; ++m) rd(m);
+      FENCE();
+#pragma unroll
+      for (int m = 0; m < 2 * NS; ++m) {
+        if (m + AHEAD < 2 * NS) rd(m + AHEAD);
+        FENCE();
+        f32x16(&x)[2] = m & 1 ? dp : s;
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) {
+          const bf16x8& f = m & 1 ? df[nb][m >> 1] : qf[nb][m >> 1];
+          if (m < 2)
+            mfma_s_first(x[nb], a[m], f);
+          else
+            mfma_s(x[nb], a[m], f);
+        }
+        FENCE();
+        hook(m);
+        FENCE();
+      }
+      mfma_read_fence(s[0], s[1]);
+      mfma_read_fence(dp[0], dp[1]);
+    };
+    auto mask = [&](int j, f32x16 (&s)[2]) {  // keys past the end: P = 0 (their exp2(-lse) may overflow)
+      const int left = k_len - (t0 + j) * 32;
+      if (left >= 32) return;
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[nb][r] = 8 * (r >> 2) + 4 * hh + (r & 3) < left ? s[nb][r] : -INFINITY;
+    };
+    auto step = [&](int i, f32x16 (&s)[2], f32x16 (&dp)[2], f32x16 (&s2)[2], f32x16 (&dp2)[2]) {
+      copy(i + 2);
+      mask(i, s);
+      constexpr int EPH = 32 / (2 * NS) > 0 ? 32 / (2 * NS) : 1;
+      products(i + 1, s2, dp2, [&](int m) {
+#pragma unroll
+        for (int e = 0; e < EPH; ++e) ds_elem(i, s, dp, m * EPH + e);
+      });
+      step_sync();
+    };
+    step_sync();
+    products(0, sa, da, [](int) {});
+    step_sync();
+    int i = 0;
+    for (; i + 1 < n; i += 2) {
+      step(i, sa, da, sb, db);
+      step(i + 1, sb, db, sa, da);
+    }
+    if (i < n) step(i, sa, da, sb, db);
+    return;
   }
-  if (d.split_k > 1) {
-    const long at = (((long)part * p.total_k + rc) * p.HK + hk) * D;
-    store_part<D>(d.part_k + at, dk, p.scale, hh, live);
-    store_part<D>(d.part_v + at, dv, 1.f, hh, live);
-  } else {
-    store_row<D>(p.dk + (long)rc * p.dk_row + (long)hk * p.dk_head, dk, p.scale, hh, live);
-    store_row<D>(p.dv + (long)rc * p.dv_row + (long)hk * p.dv_head, dv, 1.f, hh, live);
+  f32x16 acc[2][ND];
+  acc_zero<ND>(acc);
+  if (n > 0) {
+    copy(0);
+    copy(1);
+    step_sync();
+    step_sync();
+    for (int i = 0; i <= n; ++i) {
+      if (i < n) copy(i + 2);
+      if (i > 0) {
+        const char* ks = smem + L::A + ((i - 1) & 3) * SB;
+        const char* x = xch + ((i - 1) & 1) * L::XBYTES;
+        bf16x8 hi[2][2], lo[2][2];
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            hi[nb][s] = *(const bf16x8*)(x + nb * 4096 + s * 1024);
+            lo[nb][s] = *(const bf16x8*)(x + nb * 4096 + 2048 + s * 1024);
+          }
+        constexpr int AHEAD = 2;
+        bf16x8 a[2 * ND];
+#pragma unroll
+        for (int m = 0; m < AHEAD; ++m) a[m] = off.read_tr(ks, m / ND, m % ND);
+        FENCE();
+#pragma unroll
+        for (int m = 0; m < 2 * ND; ++m) {
+          if (m + AHEAD < 2 * ND) a[m + AHEAD] = off.read_tr(ks, (m + AHEAD) / ND, (m + AHEAD) % ND);
+          FENCE();
+#pragma unroll
+          for (int nb = 0; nb < 2; ++nb) {
+            mfma_o<false>(acc[nb][m % ND], a[m], hi[nb][m / ND]);
+            mfma_o<false>(acc[nb][m % ND], a[m], lo[nb][m / ND]);
+          }
+          FENCE();
+        }
+      }
+      if (i < n) step_sync();
+    }
+  }
+  acc_fence<ND>(acc);
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb) {
+    const int row = row0 + pair * 64 + nb * 32 + lq;
+    const bool live = row < q_len;
+    const long rc = q_start + min(row, q_len - 1);
+    if (d.split_q > 1)
+      store_part<D>(d.part_q + (((long)part * p.total_q + rc) * p.H + h) * D, acc[nb], p.scale, hh, live);
+    else
+      store_row<D>(p.dq + rc * p.dq_row + (long)h * p.dq_head, acc[nb], p.scale, hh, live);
   }
 }
 
@@ -585,7 +961,7 @@ int launch_fwd(const TrainDev& d, hipStream_t s) {
 template <int D>
 int launch_bwd(const TrainDev& d, hipStream_t s) {
   const AttnTrainParams& p = d.p;
-  constexpr int lds = 4 * TR * D * 2 + 2 * TR * 8;
+  constexpr int lds = Lds<D>::TOTAL;
   static std::atomic<unsigned long long> done{0};
   if (lds_limit(attn_bwd_kernel<D>, lds, done)) return 1;
   auto blocks = [](long rows_heads) { return dim3((unsigned)((rows_heads * (D / 8) + kThreads - 1) / kThreads)); };
@@ -663,7 +1039,8 @@ int attn_train_bwd(const AttnTrainParams& p, void* ws, long ws_bytes, hipStream_
   d.split_q = x.split_q;
   d.split_k = x.split_k;
   d.n_key_blocks = any_k ? x.tiles_k * p.HK * x.split_k : 0;
-  d.ld = (float2*)ws;
+  d.lse2 = (float*)ws;
+  d.delta = d.lse2 + (long)p.H * p.total_q;
   d.part_q = (float*)((char*)ws + x.ld_bytes);
   d.part_k = (float*)((char*)ws + x.ld_bytes + x.part_q_bytes);
   d.part_v = (float*)((char*)ws + x.ld_bytes + x.part_q_bytes + x.part_k_bytes);
