@@ -340,19 +340,54 @@ __device__ __forceinline__ unsigned rows_bytes(int rows_left, long stride) {
   return (unsigned)min((long)max(rows_left, 0) * stride * 2, 0x7fffffffL);
 }
 
-// 4-B-per-lane LDS copy of 32 floats (lanes 32.. read past the range: zeros behind them)
-__device__ __forceinline__ void blds4(const i32x4& rsrc, unsigned voff, unsigned lds_addr) {
-  unsigned keep;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %3\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dword %1, %2, 0 offen lds\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(keep)
-      : "v"(voff), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(lds_addr))
-      : "memory");
+// LDS copies, 16 B or 4 B per lane (0 where voff is past the range). Inline asm for the reason given at blds16
+// (attn_common.h): the compiler would wait for a builtin copy before every later LDS read. m0 is named as clobbered
+// instead of kept: two scalar instructions fewer per copy.
+__device__ __forceinline__ void copy16(const i32x4& rsrc, unsigned voff, unsigned lds_addr) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+               :
+               : "v"(voff), "s"(rsrc), "s"(lds_addr)
+               : "memory", "m0");
 }
+__device__ __forceinline__ void copy4(const i32x4& rsrc, unsigned voff, unsigned lds_addr) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
+               :
+               : "v"(voff), "s"(rsrc), "s"(lds_addr)
+               : "memory", "m0");
+}
+
+// A stream of 32-row stages over a tensor: descriptor of the next one, zeros after the last. One head's rows [0, len)
+// follow those of the head before; all in scalar registers.
+struct Stream {
+  const char* ptr;   // first byte of the next stage
+  int left;          // rows from there to the sequence end
+  int stages;        // stages that are still to come
+  int len, row_b;    // rows of a sequence, bytes of a row
+  long step, wrap;   // bytes to the next stage, and what moves past a head's last stage to the next head's first
+  // len > 0; the first stage is number t of the sweep, `stages` follow
+  __device__ __forceinline__ void init(const void* base, int t, int tiles, int len_, int stages_, long row_bytes,
+                                       long head_bytes) {
+    const int h = t / tiles, r = (t - h * tiles) * 32;
+    len = len_;
+    row_b = (int)row_bytes;
+    left = len - r;
+    stages = stages_;
+    step = 32 * row_bytes;
+    wrap = head_bytes - (long)(tiles - 1) * step;
+    ptr = (const char*)base + (long)h * head_bytes + (long)r * row_bytes;
+  }
+  // rows_of: bytes per row that the range counts (the whole stride: offsets are row * stride + column)
+  __device__ __forceinline__ i32x4 next() {
+    const int live = stages > 0 ? min(left, 32) : 0;
+    const i32x4 rs = make_rsrc(ptr, (unsigned)(live * row_b));
+    --stages;
+    left -= 32;
+    const bool w = left <= 0;
+    ptr += stages > 0 ? (w ? wrap : step) : 0;
+    left = w ? len : left;
+    return rs;
+  }
+};
 
 // The step barrier: own LDS writes and copies done, then everyone's
 __device__ __forceinline__ void step_sync() {
@@ -505,44 +540,50 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
   const unsigned lds0 = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_addr_of(smem));
   const unsigned wlds = lds0 + wave * Stage<D>::PIECES * 1024;
   const unsigned ld_off = lane < 32 ? lane * 4 : 0x7ffffff0u;
-  // stage j of this range: rows (t0 + j) % tiles * 32 .. of head hk * group + (t0 + j) / tiles. Rows past the sequence
-  // end and stages outside 0 .. n - 1 are zeros, lse and delta included: P = exp2(0 - 0) = 1 meets zero rows
-  auto at = [&](int j, int* h, int* r) {
-    const int t = t0 + j;
-    const bool live = j >= 0 && j < n;
-    *h = live ? hk * group + t / tiles : 0;
-    *r = live ? t % tiles * 32 : 0;
-    return live ? q_len - *r : 0;  // rows left
+  // Stages: rows of the group's heads in turn. Rows past the sequence end and stages past the last are zeros, lse and
+  // delta included: P = exp2(0 - 0) = 1 meets zero rows
+  Stream st_q, st_d, st_x;  // st_x: lse for wave 0, delta for the others (wave 1 copies it)
+  if (n > 0) {
+    const long h0 = (long)hk * group;
+    st_q.init(p.q + (long)q_start * p.q_row + h0 * p.q_head, t0, tiles, q_len, n, p.q_row * 2, p.q_head * 2);
+    st_d.init(p.dout + (long)q_start * p.do_row + h0 * p.do_head, t0, tiles, q_len, n, p.do_row * 2, p.do_head * 2);
+    st_x.init((wave == 0 ? d.lse2 : d.delta) + h0 * p.total_q + q_start, t0, tiles, q_len, n, 4, (long)p.total_q * 4);
+  }
+  i32x4 rq, rd, rx;
+  // the copies of q stage j and dout stage j - 1, in 2 PIECES + 1 pieces
+  auto open = [&]() {
+    rq = st_q.next();
+    rd = st_d.next();
+    rx = st_x.next();
   };
-  auto copy_q = [&](int j) {  // and lse
-    int h, r;
-    const int left = at(j, &h, &r);
-    const i32x4 rs = make_rsrc(p.q + (long)(q_start + r) * p.q_row + (long)h * p.q_head, rows_bytes(left, p.q_row));
-#pragma unroll
-    for (int i = 0; i < Stage<D>::PIECES; ++i) blds16(rs, sq.voff[i], wlds + L::A + (j & 3) * SB + i * 1024);
-    if (wave == 0)
-      blds4(make_rsrc(d.lse2 + (long)h * p.total_q + q_start + r, (unsigned)max(min(left, 32), 0) * 4), ld_off,
-            lds0 + L::LSE + (j & 3) * 256);
-  };
-  auto copy_do = [&](int j) {  // and delta
-    int h, r;
-    const int left = at(j, &h, &r);
-    const i32x4 rs =
-        make_rsrc(p.dout + (long)(q_start + r) * p.do_row + (long)h * p.do_head, rows_bytes(left, p.do_row));
-#pragma unroll
-    for (int i = 0; i < Stage<D>::PIECES; ++i) blds16(rs, sd.voff[i], wlds + L::B + (j & 1) * SB + i * 1024);
-    if (wave == 1)
-      blds4(make_rsrc(d.delta + (long)h * p.total_q + q_start + r, (unsigned)max(min(left, 32), 0) * 4), ld_off,
-            lds0 + L::DELTA + (j & 1) * 256);
+  auto copy = [&](int j, int i) {
+    constexpr int P = Stage<D>::PIECES;
+    if (i < P)
+      copy16(rq, sq.voff[i], wlds + L::A + (j & 3) * SB + i * 1024);
+    else if (i < 2 * P)
+      copy16(rd, sd.voff[i - P], wlds + L::B + ((j - 1) & 1) * SB + (i - P) * 1024);
+    else if (i == 2 * P) {
+      if (wave < 2) copy4(rx, ld_off, lds0 + (wave == 0 ? L::LSE + (j & 3) * 256 : L::DELTA + ((j - 1) & 1) * 256));
+    }
   };
 
   f32x16 acc[2][ND];
   acc_zero<ND>(acc);
   if (n > 0) {
-    copy_q(-1);
-    copy_q(0);
-    copy_do(0);
-    copy_q(1);
+    // q stages -1 (zeros: dk(-1) adds nothing), 0 and 1, dout stage 0
+    {
+      constexpr int P = Stage<D>::PIECES;
+      const i32x4 zero = make_rsrc(p.q, 0);
+#pragma unroll
+      for (int i = 0; i < P; ++i) copy16(zero, sq.voff[i], wlds + L::A + 3 * SB + i * 1024);
+      rq = st_q.next();
+#pragma unroll
+      for (int i = 0; i < P; ++i) copy16(rq, sq.voff[i], wlds + L::A + i * 1024);
+      if (wave == 0) copy4(st_x.next(), ld_off, lds0 + L::LSE);
+      open();
+#pragma unroll
+      for (int i = 0; i <= 2 * P; ++i) copy(1, i);
+    }
     // stationary rows: k for wave 0, v for wave 1
     bf16x8 f[2][D / 16];
 #pragma unroll
@@ -581,9 +622,8 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
       next();
       step_sync();
       for (int i = 0; i < n; ++i) {
-        copy_q(i + 2);
-        copy_do(i + 1);
-        row_phase<D>(smem + L::A + ((i + 1) & 3) * SB, off, f, s, none);
+        open();
+        row_phase<D>(smem + L::A + ((i + 1) & 3) * SB, off, f, s, [&](int k) { copy(i + 2, k); });
         tr_phase<D>(smem + L::B + (i & 1) * SB, off, bc, acc, [&](int m) {
 #pragma unroll
           for (int e = 0; e < EPH; ++e) prob(i + 1, m * EPH + e);
@@ -600,11 +640,8 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
       step_sync();
       f32x4 del, pr;
       for (int i = 0; i <= n; ++i) {
-        if (i < n) {
-          copy_q(i + 2);
-          copy_do(i + 1);
-        }
-        row_phase<D>(smem + L::B + (i & 1) * SB, off, f, s, none);
+        open();  // after the last stage: zeros
+        row_phase<D>(smem + L::B + (i & 1) * SB, off, f, s, [&](int k) { copy(i + 2, k); });
         tr_phase<D>(smem + L::A + ((i - 1) & 3) * SB, off, bc, acc, [&](int m) {
 #pragma unroll
           for (int e0 = 0; e0 < EPH; ++e0) {
@@ -671,24 +708,34 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
   sv.init(p.v_row, wave, lane);
   const unsigned lds0 = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_addr_of(smem));
   const unsigned wlds = lds0 + wave * Stage<D>::PIECES * 1024;
-  const bf16_t* kp = p.k + (long)k_start * p.k_row + (long)hk * p.k_head;
-  const bf16_t* vp = p.v + (long)k_start * p.v_row + (long)hk * p.v_head;
-  auto copy = [&](int j) {  // k and v rows of stage j of this range; zeros past its end
-    const int r = (t0 + j) * 32, left = j < n ? k_len - r : 0;
-    const i32x4 krs = make_rsrc(kp + (long)r * p.k_row, rows_bytes(left, p.k_row));
-    const i32x4 vrs = make_rsrc(vp + (long)r * p.v_row, rows_bytes(left, p.v_row));
+  Stream st_k, st_v;
+  if (n > 0) {
+    st_k.init(p.k + (long)k_start * p.k_row + (long)hk * p.k_head, t0, all, k_len, n, p.k_row * 2, 0);
+    st_v.init(p.v + (long)k_start * p.v_row + (long)hk * p.v_head, t0, all, k_len, n, p.v_row * 2, 0);
+  }
+  i32x4 rk, rv;
+  auto open = [&]() {
+    rk = st_k.next();
+    rv = st_v.next();
+  };
+  auto copy = [&](int j, int i) {  // piece i of k and v stage j
+    constexpr int P = Stage<D>::PIECES;
+    if (i < P)
+      copy16(rk, sk.voff[i], wlds + L::A + (j & 3) * SB + i * 1024);
+    else if (i < 2 * P)
+      copy16(rv, sv.voff[i - P], wlds + L::B + (j & 1) * SB + (i - P) * 1024);
+  };
+  auto copy_all = [&](int j) {
+    open();
 #pragma unroll
-    for (int i = 0; i < Stage<D>::PIECES; ++i) {
-      blds16(krs, sk.voff[i], wlds + L::A + (j & 3) * SB + i * 1024);
-      blds16(vrs, sv.voff[i], wlds + L::B + (j & 1) * SB + i * 1024);
-    }
+    for (int i = 0; i < 2 * Stage<D>::PIECES; ++i) copy(j, i);
   };
 
   char* const xch = smem + L::X + pair * 8192 + lane * 16;  // [buffer][pair][block][hi 2, lo 2][lane] 16 B
   if ((wave & 1) == 0) {
     if (n <= 0) return;  // wave 1 stores the zeros
-    copy(0);
-    copy(1);
+    copy_all(0);
+    copy_all(1);
     bf16x8 qf[2][NS], df[2][NS];
     float lse[2], del[2];
 #pragma unroll
@@ -766,10 +813,11 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
         for (int r = 0; r < 16; ++r) s[nb][r] = 8 * (r >> 2) + 4 * hh + (r & 3) < left ? s[nb][r] : -INFINITY;
     };
     auto step = [&](int i, f32x16 (&s)[2], f32x16 (&dp)[2], f32x16 (&s2)[2], f32x16 (&dp2)[2]) {
-      copy(i + 2);
+      open();
       mask(i, s);
       constexpr int EPH = 32 / (2 * NS) > 0 ? 32 / (2 * NS) : 1;
       products(i + 1, s2, dp2, [&](int m) {
+        copy(i + 2, m);
 #pragma unroll
         for (int e = 0; e < EPH; ++e) ds_elem(i, s, dp, m * EPH + e);
       });
@@ -789,13 +837,15 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
   f32x16 acc[2][ND];
   acc_zero<ND>(acc);
   if (n > 0) {
-    copy(0);
-    copy(1);
+    copy_all(0);
+    copy_all(1);
     step_sync();
     step_sync();
-    for (int i = 0; i <= n; ++i) {
-      if (i < n) copy(i + 2);
-      if (i > 0) {
+    copy_all(2);
+    step_sync();
+    for (int i = 1; i <= n; ++i) {
+      open();  // after the last stage: zeros
+      {
         const char* ks = smem + L::A + ((i - 1) & 3) * SB;
         const char* x = xch + ((i - 1) & 1) * L::XBYTES;
         bf16x8 hi[2][2], lo[2][2];
@@ -821,10 +871,13 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
             mfma_o<false>(acc[nb][m % ND], a[m], lo[nb][m / ND]);
           }
           FENCE();
+          copy(i + 2, m);
+          FENCE();
         }
       }
       if (i < n) step_sync();
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may outlive the workgroup
   }
   acc_fence<ND>(acc);
 #pragma unroll
