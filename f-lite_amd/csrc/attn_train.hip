@@ -426,26 +426,33 @@ struct ReadOff {
 
 #define FENCE() __builtin_amdgcn_sched_barrier(0)
 
+// The phases below fix the instruction order by hand. Waves issue in order and a 32x32x16 MFMA holds its pipe for 32
+// cycles, so a second MFMA right behind the first blocks the wave until the first is done: other work overlaps only
+// where it stands BETWEEN MFMAs, at most 28 cycles of it (7 VALU instructions, or a v_exp and 3) per MFMA. With the VALU
+// work behind pairs of MFMAs a step took the sum of both, 4400 cycles instead of 2700.
+
 // acc[n] (VGPRs) = stage rows . stationary block n; hook(s) after each k-step
 template <int D, typename Hook>
 __device__ __forceinline__ void row_phase(const char* st, const ReadOff<D>& o, const bf16x8 (&f)[2][D / 16],
                                           f32x16 (&acc)[2], Hook hook) {
-  constexpr int NS = D / 16, AHEAD = 3;
+  constexpr int NS = D / 16, AHEAD = NS < 5 ? NS : 5;
   bf16x8 a[NS];
 #pragma unroll
   for (int s = 0; s < AHEAD; ++s) a[s] = o.read_row(st, s);
   FENCE();
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
+    if (s == 0)
+      mfma_sv_first(acc[0], a[0], f[0][0]);
+    else
+      mfma_sv(acc[0], a[s], f[0][s]);
+    FENCE();
     if (s + AHEAD < NS) a[s + AHEAD] = o.read_row(st, s + AHEAD);
     FENCE();
-    if (s == 0) {
-      mfma_sv_first(acc[0], a[0], f[0][0]);
+    if (s == 0)
       mfma_sv_first(acc[1], a[0], f[1][0]);
-    } else {
-      mfma_sv(acc[0], a[s], f[0][s]);
+    else
       mfma_sv(acc[1], a[s], f[1][s]);
-    }
     FENCE();
     hook(s);
     FENCE();
@@ -453,23 +460,25 @@ __device__ __forceinline__ void row_phase(const char* st, const ReadOff<D>& o, c
   mfma_read_fence(acc[0], acc[1]);
 }
 
-// acc[n][dt] (AGPRs) += (stage columns)^T . b[n]; hook(m) after each of the 2 D / 32 column reads
+// acc[n][dt] (AGPRs) += (stage columns)^T . b[n]; hook(m) after each of the 4 D / 32 MFMAs
 template <int D, typename Hook>
 __device__ __forceinline__ void tr_phase(const char* st, const ReadOff<D>& o, bf16x8 (&b)[2][2],
                                          f32x16 (&acc)[2][D / 32], Hook hook) {
-  constexpr int ND = D / 32, AHEAD = 2;
+  constexpr int ND = D / 32, AHEAD = 3;
   bf16x8 a[2 * ND];
 #pragma unroll
   for (int m = 0; m < AHEAD; ++m) a[m] = o.read_tr(st, m / ND, m % ND);
   FENCE();
 #pragma unroll
   for (int m = 0; m < 2 * ND; ++m) {
-    if (m + AHEAD < 2 * ND) a[m + AHEAD] = o.read_tr(st, (m + AHEAD) / ND, (m + AHEAD) % ND);
-    FENCE();
     mfma_o<false>(acc[0][m % ND], a[m], b[0][m / ND]);
+    FENCE();
+    if (m + AHEAD < 2 * ND) a[m + AHEAD] = o.read_tr(st, (m + AHEAD) / ND, (m + AHEAD) % ND);
+    hook(2 * m);
+    FENCE();
     mfma_o<false>(acc[1][m % ND], a[m], b[1][m / ND]);
     FENCE();
-    hook(m);
+    hook(2 * m + 1);
     FENCE();
   }
 }
@@ -514,7 +523,7 @@ template <int D>
 __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) {
   const AttnTrainParams& p = d.p;
   using L = Lds<D>;
-  constexpr int ND = D / 32, SB = Stage<D>::BYTES, EPH = 32 / (2 * ND);  // scores per hook
+  constexpr int ND = D / 32, SB = Stage<D>::BYTES, EPH = 32 / (4 * ND);  // scores per hook
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lq = lane & 31, hh = lane >> 5, pair = wave >> 1;
   const int part = v % d.split_k;
@@ -600,15 +609,30 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
     auto none = [](int) {};
     step_sync();
     if ((wave & 1) == 0) {
-      // score e of stage j: group r4 = e >> 3 (rows 8 r4 + 4 hh + 0..3), block (e >> 2) & 1
-      f32x4 lse;
-      auto prob = [&](int j, int e) {
+      // score e of stage j: group r4 = e >> 3 (rows 8 r4 + 4 hh + 0..3), block (e >> 2) & 1. Each call does the exp2 of
+      // its score, the argument of the next and the stores of the ones before, so that nothing waits on the exp2
+      f32x4 lse, lse_n;
+      float x;
+      auto arg = [&](int j, int e) {
+        const int r4 = e >> 3, nb = (e >> 2) & 1, i = e & 3;
+        if ((e & 7) == 0) lse = lse_n;
+        x = __builtin_fmaf(s[nb][4 * r4 + i], sl2, -lse[i]);
+        if ((e & 7) == 0 && r4 < 3)
+          lse_n = *(const f32x4*)(smem + L::LSE + (j & 3) * 256 + (8 * (r4 + 1) + 4 * hh) * 4);
+      };
+      auto store = [&](int j, int e) {  // P of score e is there
         const int r4 = e >> 3, nb = (e >> 2) & 1, i = e & 3, r = 4 * r4 + i;
-        if ((e & 7) == 0) lse = *(const f32x4*)(smem + L::LSE + (j & 3) * 256 + (8 * r4 + 4 * hh) * 4);
-        s[nb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][r], sl2, -lse[i]));
         if (i & 1) bn[nb][r >> 3][(r & 7) >> 1] = pack_bf(s[nb][r - 1], s[nb][r]);
         if (i == 3)
           *(f32x4*)(xch + (j & 1) * L::XBYTES + (nb * 4 + r4) * 1024) = f32x4{s[nb][r - 3], s[nb][r - 2], s[nb][r - 1], s[nb][r]};
+      };
+      auto begin = [&](int j) { lse_n = *(const f32x4*)(smem + L::LSE + (j & 3) * 256 + 4 * hh * 4); };
+      auto prob = [&](int j, int e) {
+        if (e == 0) arg(j, 0);
+        s[(e >> 2) & 1][4 * (e >> 3) + (e & 3)] = __builtin_amdgcn_exp2f(x);
+        if (e < 31) arg(j, e + 1);
+        if (e > 0) store(j, e - 1);
+        if (e == 31) store(j, 31);
       };
       auto next = [&]() {
 #pragma unroll
@@ -616,6 +640,7 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
 #pragma unroll
           for (int ks = 0; ks < 2; ++ks) bc[nb][ks] = __builtin_bit_cast(bf16x8, bn[nb][ks]);
       };
+      begin(0);
       row_phase<D>(smem + L::A, off, f, s, none);
 #pragma unroll
       for (int e = 0; e < 32; ++e) prob(0, e);
@@ -623,6 +648,7 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
       step_sync();
       for (int i = 0; i < n; ++i) {
         open();
+        begin(i + 1);
         row_phase<D>(smem + L::A + ((i + 1) & 3) * SB, off, f, s, [&](int k) { copy(i + 2, k); });
         tr_phase<D>(smem + L::B + (i & 1) * SB, off, bc, acc, [&](int m) {
 #pragma unroll
@@ -638,17 +664,26 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) bc[nb][ks] = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
       step_sync();
-      f32x4 del, pr;
+      f32x4 del, pr, del_n, pr_n;
       for (int i = 0; i <= n; ++i) {
         open();  // after the last stage: zeros
         row_phase<D>(smem + L::B + (i & 1) * SB, off, f, s, [&](int k) { copy(i + 2, k); });
+        auto rd = [&](int e) {  // delta and P of the 4 scores from e on
+          const int r4 = e >> 3, nb = (e >> 2) & 1;
+          if (nb == 0) del_n = *(const f32x4*)(smem + L::DELTA + (i & 1) * 256 + (8 * r4 + 4 * hh) * 4);
+          pr_n = *(const f32x4*)(xch + (i & 1) * L::XBYTES + (nb * 4 + r4) * 1024);
+        };
+        rd(0);
         tr_phase<D>(smem + L::A + ((i - 1) & 3) * SB, off, bc, acc, [&](int m) {
 #pragma unroll
           for (int e0 = 0; e0 < EPH; ++e0) {
             const int e = m * EPH + e0;
-            const int r4 = e >> 3, nb = (e >> 2) & 1, k = e & 3, r = 4 * r4 + k;
-            if ((e & 7) == 0) del = *(const f32x4*)(smem + L::DELTA + (i & 1) * 256 + (8 * r4 + 4 * hh) * 4);
-            if (k == 0) pr = *(const f32x4*)(xch + (i & 1) * L::XBYTES + (nb * 4 + r4) * 1024);
+            const int nb = (e >> 2) & 1, k = e & 3, r = 4 * (e >> 3) + k;
+            if (k == 0) {
+              pr = pr_n;
+              if (nb == 0) del = del_n;
+              if (e + 4 < 32) rd(e + 4);
+            }
             s[nb][r] = pr[k] * (s[nb][r] - del[k]);
             if (k & 1) bn[nb][r >> 3][(r & 7) >> 1] = pack_bf(s[nb][r - 1], s[nb][r]);
           }
@@ -757,28 +792,39 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
     const float sl2 = p.scale * kLog2e;
     f32x16 sa[2], da[2], sb[2], db[2];
     u32x4 hi, lo;
-    // element e (block e >> 4, score e & 15) of stage j's dS, from its S and dP
-    auto ds_elem = [&](int j, f32x16 (&s)[2], f32x16 (&dp)[2], int e) {
-      const int nb = e >> 4, r = e & 15;
-      s[nb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][r], sl2, -lse[nb])) * (dp[nb][r] - del[nb]);
-      if (r & 1) {
-        const int w = (r & 7) >> 1;
-        const float x = s[nb][r - 1], y = s[nb][r];
-        const unsigned h2 = pack_bf(x, y);
-        hi[w] = h2;
-        lo[w] = pack_bf(x - __uint_as_float(h2 << 16), y - __uint_as_float(h2 & 0xffff0000u));
-        if (w == 3) {
-          char* to = xch + (j & 1) * L::XBYTES + nb * 4096 + (r >> 3) * 1024;
-          *(u32x4*)to = hi;
-          *(u32x4*)(to + 2048) = lo;
-        }
+    // Half u of the 64 that make stage j's dS from its S and dP: element e = u >> 1 (block e >> 4, score e & 15); even
+    // halves do an exp2 and the next one's argument, odd ones the products and the split of the pair before
+    float x, pe;
+    auto split = [&](int j, f32x16 (&s)[2], int e) {  // e odd: dS of e - 1 and e -> hi, lo
+      const int nb = e >> 4, r = e & 15, w = (r & 7) >> 1;
+      const unsigned h2 = hi[w];
+      lo[w] = pack_bf(s[nb][r - 1] - __uint_as_float(h2 << 16), s[nb][r] - __uint_as_float(h2 & 0xffff0000u));
+      if (w == 3) {
+        char* to = xch + (j & 1) * L::XBYTES + nb * 4096 + (r >> 3) * 1024;
+        *(u32x4*)to = hi;
+        *(u32x4*)(to + 2048) = lo;
       }
     };
-    // S and dP of stage j into (s, dp); hook(m) after each of the 2 NS fragment reads
+    auto ds_half = [&](int j, f32x16 (&s)[2], f32x16 (&dp)[2], int u) {
+      const int e = u >> 1, nb = e >> 4, r = e & 15;
+      if ((u & 1) == 0) {
+        if (e == 0) x = __builtin_fmaf(s[0][0], sl2, -lse[0]);
+        pe = __builtin_amdgcn_exp2f(x);
+        if (e < 31) x = __builtin_fmaf(s[(e + 1) >> 4][(e + 1) & 15], sl2, -lse[(e + 1) >> 4]);
+      } else {
+        s[nb][r] = pe * (dp[nb][r] - del[nb]);
+        if (e & 1)
+          hi[(r & 7) >> 1] = pack_bf(s[nb][r - 1], s[nb][r]);
+        else if (e > 0)
+          split(j, s, e - 1);
+        if (e == 31) split(j, s, 31);
+      }
+    };
+    // S and dP of stage j into (s, dp); hook(u) after each of the 4 NS MFMAs
     auto products = [&](int j, f32x16 (&s)[2], f32x16 (&dp)[2], auto hook) {
       const char* ks = smem + L::A + (j & 3) * SB;
       const char* vs = smem + L::B + (j & 1) * SB;
-      constexpr int AHEAD = 4;
+      constexpr int AHEAD = 5;
       bf16x8 a[2 * NS];
       auto rd = [&](int m) { a[m] = off.read_row(m & 1 ? vs : ks, m >> 1); };
 #pragma unroll
@@ -786,20 +832,19 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
       FENCE();
 #pragma unroll
       for (int m = 0; m < 2 * NS; ++m) {
-        if (m + AHEAD < 2 * NS) rd(m + AHEAD);
-        FENCE();
-        f32x16(&x)[2] = m & 1 ? dp : s;
+        f32x16(&acc)[2] = m & 1 ? dp : s;
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb) {
           const bf16x8& f = m & 1 ? df[nb][m >> 1] : qf[nb][m >> 1];
           if (m < 2)
-            mfma_s_first(x[nb], a[m], f);
+            mfma_s_first(acc[nb], a[m], f);
           else
-            mfma_s(x[nb], a[m], f);
+            mfma_s(acc[nb], a[m], f);
+          FENCE();
+          if (nb == 0 && m + AHEAD < 2 * NS) rd(m + AHEAD);
+          hook(2 * m + nb);
+          FENCE();
         }
-        FENCE();
-        hook(m);
-        FENCE();
       }
       mfma_read_fence(s[0], s[1]);
       mfma_read_fence(dp[0], dp[1]);
@@ -815,11 +860,11 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
     auto step = [&](int i, f32x16 (&s)[2], f32x16 (&dp)[2], f32x16 (&s2)[2], f32x16 (&dp2)[2]) {
       open();
       mask(i, s);
-      constexpr int EPH = 32 / (2 * NS) > 0 ? 32 / (2 * NS) : 1;
+      constexpr int UPH = 64 / (4 * NS);
       products(i + 1, s2, dp2, [&](int m) {
-        copy(i + 2, m);
 #pragma unroll
-        for (int e = 0; e < EPH; ++e) ds_elem(i, s, dp, m * EPH + e);
+        for (int u = 0; u < UPH; ++u) ds_half(i, s, dp, m * UPH + u);
+        if (m & 1) copy(i + 2, m >> 1);
       });
       step_sync();
     };
@@ -863,15 +908,16 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
         FENCE();
 #pragma unroll
         for (int m = 0; m < 2 * ND; ++m) {
+          mfma_o<false>(acc[0][m % ND], a[m], hi[0][m / ND]);
+          FENCE();
           if (m + AHEAD < 2 * ND) a[m + AHEAD] = off.read_tr(ks, (m + AHEAD) / ND, (m + AHEAD) % ND);
           FENCE();
-#pragma unroll
-          for (int nb = 0; nb < 2; ++nb) {
-            mfma_o<false>(acc[nb][m % ND], a[m], hi[nb][m / ND]);
-            mfma_o<false>(acc[nb][m % ND], a[m], lo[nb][m / ND]);
-          }
+          mfma_o<false>(acc[1][m % ND], a[m], hi[1][m / ND]);
           FENCE();
           copy(i + 2, m);
+          FENCE();
+          mfma_o<false>(acc[0][m % ND], a[m], lo[0][m / ND]);
+          mfma_o<false>(acc[1][m % ND], a[m], lo[1][m / ND]);
           FENCE();
         }
       }
