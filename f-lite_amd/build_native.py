@@ -42,8 +42,11 @@ CFLAGS = [
 # epilogue (packed f32 beside MFMAs is an anti-lever anyway: MI355X guide, per-instruction costs).
 # attention_q256.hip: the same, for the softmax row sums of its two query blocks, which SLP paired into one
 # v_pk_add_f32 chain inside the PV phase (16 per key tile, each ~13 cycles dearer than a v_add_f32 there).
+# attn_train.hip: MFMAs that the compiler places keep their accumulators in VGPRs, where the softmax reads them (the
+# AGPRs are taken by the gradients' accumulators).
 FILE_FLAGS = {"gemm.hip": ["-fno-slp-vectorize"], "gemm_fp8.hip": ["-fno-slp-vectorize"],
-              "attention_q256.hip": ["-fno-slp-vectorize"]}
+              "attention_q256.hip": ["-fno-slp-vectorize"],
+              "attn_train.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _sources():

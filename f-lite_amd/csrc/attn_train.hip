@@ -30,6 +30,10 @@ namespace flite {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+// The backward pass works with 2^15 P (and 2^15 dS), taken back when the gradients are stored: P goes from wave to wave
+// in fp16 (2^-12, against the 2^-9 of the rounding that follows), where 2^15 P <= 2^15 fits and stays normal down to
+// P = 2^-29.
+constexpr float kShift = 15.f, kUnshift = 1.f / 32768.f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int WROWS = 128;  // stationary rows of a workgroup
 constexpr int TR = 64;      // swept rows of an LDS tile
@@ -41,7 +45,7 @@ struct TrainDev {
   int tiles_q, tiles_k;    // upper bounds of the packed batch's 128-row tiles
   int split_q, split_k;    // ranges that a query / key workgroup's sweep is cut into
   int n_key_blocks;        // backward: the first blocks of the launch are key workgroups
-  float* lse2;             // [H][total_q] lse * log2 e
+  float* lse2;             // [H][total_q] lse * log2 e - kShift
   float* delta;            // [H][total_q]
   float* part_q;           // [split_q][total_q][H][D] fp32, with split_q > 1
   float* part_k;           // [split_k][total_k][HK][D]
@@ -305,34 +309,42 @@ __global__ __launch_bounds__(kThreads) void attn_delta_kernel(TrainDev d) {
     const long at = (long)h * p.total_q + row;
     const float lse = p.lse[at];
     // a row without keys (or with -inf scores alone) has P = 0: exp2(x - inf)
-    d.lse2[at] = lse == -INFINITY ? INFINITY : lse * kLog2e;
+    d.lse2[at] = lse == -INFINITY ? INFINITY : lse * kLog2e - kShift;
     d.delta[at] = s;
   }
 }
 
-// Two kinds of waves. A wave of 32 stationary rows would need every LDS byte for one MFMA each and sit on the LDS read
-// rate (128 B per clock and CU); 64 rows need twice the registers. So the waves of a pair share 64 stationary rows (two
-// blocks of 32) and split the products: each A fragment read from LDS feeds both blocks.
-//   key workgroup:   wave 0: S, P, dv    wave 1: dP, dS = P (dP - delta), dk      (P handed over in fp32)
-//   query workgroup: wave 0: S, dP, dS   wave 1: dq                               (dS handed over as two bf16, hi + lo)
-// All four have 64 MFMAs per 32 swept rows. dS enters dq as hi + lo (2^-17): its rows sum to 0, so where keys share a
-// direction, that direction cancels in dq and a single rounding's error would stay (dq 1.7 times as far from the exact
-// gradient as one final rounding to bf16 is, against 1.4 for dk and dv).
+// Two kinds of waves. A wave with 32 stationary rows would read every LDS byte for one MFMA; with 64 rows the gradients
+// take twice the registers. So the waves of a pair share 64 stationary rows (two blocks of 32) and split the products:
+// each A fragment read from LDS feeds both blocks.
+//   key workgroup:   wave 0: S, P, dv    wave 1: dP, dS = P (dP - delta), dk      (P handed over)
+//   query workgroup: wave 0: S, dP, dS   wave 1: dq                               (dS handed over)
+// All four have 64 MFMAs per 32 swept rows. dS enters dq as a bf16 pair hi + lo (2^-17): its rows sum to 0, so where
+// keys share a direction, that direction cancels in dq and a single rounding's error would stay (dq 1.7 times as far
+// from the exact gradient as one final rounding to bf16 is, against 1.4 for dk and dv).
+//
+// Everything is made a step (32 swept rows) or more ahead, so that between two barriers no wave waits: a step's tiles
+// have been in LDS for a whole step, the first fragments of a step are read before its barrier, scores are turned into
+// P or dS in the step after their products. What a step costs beyond its 2048 MFMA cycles is the barrier.
 
 template <int D>
 struct Stage {
-  static constexpr int BYTES = 32 * D * 2;  // 32 swept rows
-  static constexpr int PIECES = D / 64;     // 1-KiB copies per wave
-  int voff[PIECES];                         // this lane's source bytes in the stage
+  static constexpr int BYTES = 32 * D * 2;      // 32 swept rows
+  static constexpr int PIECES = D / 64;         // 1-KiB copies per wave: pieces wave, wave + 4, ...
+  static constexpr int ROWS = 1024 / (D * 2);   // rows of a piece
+  int voff[PIECES > 1 ? 2 : 1];                 // this lane's source bytes, even and odd pieces (less the rows before)
+  int step;                                     // bytes of 4 pieces' rows
   __device__ __forceinline__ void init(long stride, int wave, int lane) {
     constexpr int CPR = D / 8;
+    step = (int)(4 * ROWS * stride * 2);
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const int pos = (wave * PIECES + i) * 64 + lane;
-      const int row = pos / CPR, ch = (pos % CPR) ^ swz<D>(row);
-      voff[i] = (int)(row * stride * 2) + ch * 16;
+    for (int i = 0; i < (PIECES > 1 ? 2 : 1); ++i) {
+      const int row = wave * ROWS + lane / CPR;  // 4 pieces further: the same XOR but for bit 3 of the row
+      voff[i] = (int)(row * stride * 2) + (((lane % CPR) ^ swz<D>(row + 4 * ROWS * i)) << 4);
     }
   }
+  __device__ __forceinline__ unsigned src(int i) const { return (unsigned)(voff[PIECES > 1 ? i & 1 : 0] + i * step); }
+  static __device__ __forceinline__ unsigned dst(int i) { return i * 4096; }
 };
 
 // Buffer range of the rows left in a sequence (0: the stage becomes zeros)
@@ -394,32 +406,49 @@ __device__ __forceinline__ void step_sync() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// LDS offsets of a lane's reads in a stage; k-steps s >= 8 and column tiles dt >= 4 are 256 B further (the XOR stays
-// within 16 chunks)
+// LDS addresses of a lane's reads in a stage, moved along from stage to stage in place (no registers for sums); k-steps
+// s >= 8 and column tiles dt >= 4 are 256 B further (the XOR stays within 16 chunks)
 template <int D>
-struct ReadOff {
-  static constexpr int NR = D / 16 < 8 ? D / 16 : 8, NT = D / 32 < 4 ? D / 32 : 4;
-  int row[NR];
-  int tr[2][NT];
-  __device__ __forceinline__ void init(int lane) {
+struct RowReader {
+  static constexpr int NR = D / 16 < 8 ? D / 16 : 8;
+  unsigned at[NR];
+  __device__ __forceinline__ void init(int lane, unsigned st) {
     const int lq = lane & 31, hh = lane >> 5;
 #pragma unroll
-    for (int s = 0; s < NR; ++s) row[s] = lq * D * 2 + (((2 * s + hh) ^ swz<D>(lq)) << 4);
+    for (int s = 0; s < NR; ++s) at[s] = st + lq * D * 2 + (((2 * s + hh) ^ swz<D>(lq)) << 4);
+  }
+  __device__ __forceinline__ void move(int by) {
+#pragma unroll
+    for (int s = 0; s < NR; ++s) at[s] += by;
+  }
+  __device__ __forceinline__ bf16x8 read(int s) const {
+    return *(const LDS_AS bf16x8*)(unsigned long)(at[s % NR] + 256 * (s / NR));
+  }
+};
+template <int D>
+struct TrReader {
+  static constexpr int NT = D / 32 < 4 ? D / 32 : 4;
+  unsigned at[2][NT];
+  __device__ __forceinline__ void init(int lane, unsigned st) {
     const int G = lane >> 4, vq = (lane & 15) >> 2, vp = lane & 3;
     const int r0 = 4 * (G >> 1) + vq;
 #pragma unroll
     for (int o = 0; o < 2; ++o)
 #pragma unroll
       for (int dt = 0; dt < NT; ++dt)
-        tr[o][dt] = (r0 + 8 * o) * D * 2 + (((4 * dt + 2 * (G & 1) + (vp >> 1)) ^ swz<D>(r0 + 8 * o)) << 4) + (vp & 1) * 8;
+        at[o][dt] = st + (r0 + 8 * o) * D * 2 +
+                    (((4 * dt + 2 * (G & 1) + (vp >> 1)) ^ swz<D>(r0 + 8 * o)) << 4) + (vp & 1) * 8;
   }
-  __device__ __forceinline__ bf16x8 read_row(const char* st, int s) const {
-    return *(const bf16x8*)(st + row[s % NR] + 256 * (s / NR));
+  __device__ __forceinline__ void move(int by) {
+#pragma unroll
+    for (int o = 0; o < 2; ++o)
+#pragma unroll
+      for (int dt = 0; dt < NT; ++dt) at[o][dt] += by;
   }
-  __device__ __forceinline__ bf16x8 read_tr(const char* st, int ks, int dt) const {
-    const char* b = st + ks * 16 * D * 2 + 256 * (dt / NT);
-    const s16x4 lo = ds_tr16(b + tr[0][dt % NT]);
-    const s16x4 hi = ds_tr16(b + tr[1][dt % NT]);
+  __device__ __forceinline__ bf16x8 read(int ks, int dt) const {
+    const int by = ks * 16 * D * 2 + 256 * (dt / NT);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)(unsigned long)(at[0][dt % NT] + by));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS s16x4*)(unsigned long)(at[1][dt % NT] + by));
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 };
@@ -429,51 +458,81 @@ struct ReadOff {
 // The phases below fix the instruction order by hand. Waves issue in order and a 32x32x16 MFMA holds its pipe for 32
 // cycles, so a second MFMA right behind the first blocks the wave until the first is done: other work overlaps only
 // where it stands BETWEEN MFMAs, at most 28 cycles of it (7 VALU instructions, or a v_exp and 3) per MFMA. With the VALU
-// work behind pairs of MFMAs a step took the sum of both, 4400 cycles instead of 2700.
+// work behind pairs of MFMAs a step took the sum of both. Score products are builtins, so that the compiler keeps the
+// wait states before the VALU reads them (built with -amdgpu-mfma-vgpr-form: scores stay in VGPRs); the gradients' are
+// asm with the accumulators pinned to AGPRs (attn_common.h, mfma_o).
 
-// acc[n] (VGPRs) = stage rows . stationary block n; hook(s) after each k-step
-template <int D, typename Hook>
-__device__ __forceinline__ void row_phase(const char* st, const ReadOff<D>& o, const bf16x8 (&f)[2][D / 16],
-                                          f32x16 (&acc)[2], Hook hook) {
-  constexpr int NS = D / 16, AHEAD = NS < 5 ? NS : 5;
+// MFMAs of the next phase that are issued before the VALU reads a phase's scores: an 8-pass MFMA's result may be read 72
+// cycles after its start, and the third MFMA behind it starts after 96
+constexpr int SKIP = 2;
+
+__device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.f;
+  return z;
+}
+
+// The first reads of a phase, made before it starts
+template <int D>
+struct RowAhead {
+  static constexpr int N = 4;
+  bf16x8 a[N];
+  __device__ __forceinline__ void read(const RowReader<D>& o) {
+#pragma unroll
+    for (int s = 0; s < N; ++s) a[s] = o.read(s);
+  }
+};
+template <int D>
+struct TrAhead {
+  static constexpr int N = 3;
+  bf16x8 a[N];
+  __device__ __forceinline__ void read(const TrReader<D>& o) {
+#pragma unroll
+    for (int m = 0; m < N; ++m) a[m] = o.read(m / (D / 32), m % (D / 32));
+  }
+};
+
+// acc[n] (VGPRs) = stage rows . stationary block n. hook(s) after k-step s; last(): reads of the next phase
+template <int D, typename Hook, typename Last>
+__device__ __forceinline__ void row_phase(const RowReader<D>& o, const RowAhead<D>& first,
+                                          const bf16x8 (&f)[2][D / 16], f32x16 (&acc)[2], Hook hook, Last last) {
+  constexpr int NS = D / 16, AHEAD = RowAhead<D>::N;
   bf16x8 a[NS];
 #pragma unroll
-  for (int s = 0; s < AHEAD; ++s) a[s] = o.read_row(st, s);
-  FENCE();
+  for (int s = 0; s < AHEAD; ++s) a[s] = first.a[s];
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
-    if (s == 0)
-      mfma_sv_first(acc[0], a[0], f[0][0]);
-    else
-      mfma_sv(acc[0], a[s], f[0][s]);
+    acc[0] = mfma(a[s], f[0][s], s == 0 ? zero16() : acc[0]);
     FENCE();
-    if (s + AHEAD < NS) a[s + AHEAD] = o.read_row(st, s + AHEAD);
+    if (s + AHEAD < NS) a[s + AHEAD] = o.read(s + AHEAD);
+    if (s + AHEAD == NS) last();
     FENCE();
-    if (s == 0)
-      mfma_sv_first(acc[1], a[0], f[1][0]);
-    else
-      mfma_sv(acc[1], a[s], f[1][s]);
+    acc[1] = mfma(a[s], f[1][s], s == 0 ? zero16() : acc[1]);
     FENCE();
     hook(s);
     FENCE();
   }
-  mfma_read_fence(acc[0], acc[1]);
 }
 
-// acc[n][dt] (AGPRs) += (stage columns)^T . b[n]; hook(m) after each of the 4 D / 32 MFMAs
-template <int D, typename Hook>
-__device__ __forceinline__ void tr_phase(const char* st, const ReadOff<D>& o, bf16x8 (&b)[2][2],
-                                         f32x16 (&acc)[2][D / 32], Hook hook) {
-  constexpr int ND = D / 32, AHEAD = 3;
+// acc[n][dt] (AGPRs) += (stage columns)^T . b[n]. hook(m) after each of the 4 D / 32 MFMAs; last(): reads of the next
+// phase
+template <int D, typename Hook, typename Last>
+__device__ __forceinline__ void tr_phase(const TrReader<D>& o, const TrAhead<D>& first,
+                                         bf16x8 (&b)[2][2], f32x16 (&acc)[2][D / 32], Hook hook, Last last) {
+  constexpr int ND = D / 32, AHEAD = TrAhead<D>::N;
   bf16x8 a[2 * ND];
 #pragma unroll
-  for (int m = 0; m < AHEAD; ++m) a[m] = o.read_tr(st, m / ND, m % ND);
-  FENCE();
+  for (int m = 0; m < AHEAD; ++m) a[m] = first.a[m];
 #pragma unroll
   for (int m = 0; m < 2 * ND; ++m) {
     mfma_o<false>(acc[0][m % ND], a[m], b[0][m / ND]);
     FENCE();
-    if (m + AHEAD < 2 * ND) a[m + AHEAD] = o.read_tr(st, (m + AHEAD) / ND, (m + AHEAD) % ND);
+    if (m + AHEAD < 2 * ND) a[m + AHEAD] = o.read((m + AHEAD) / ND, (m + AHEAD) % ND);
+    if (m + AHEAD == 2 * ND) last();
     hook(2 * m);
     FENCE();
     mfma_o<false>(acc[1][m % ND], a[m], b[1][m / ND]);
@@ -509,21 +568,35 @@ __device__ __forceinline__ unsigned pack_bf(float lo, float hi) {
   return __builtin_bit_cast(unsigned, v);
 }
 
-// LDS of a key workgroup: q ring of 4 stages, dout ring of 2, P double-buffered, lse ring of 4, delta ring of 2; of a
-// query workgroup: k ring of 4, v ring of 2, dS double-buffered
+// LDS of a key workgroup: q ring of 5 stages, dout ring of 3, P double-buffered, lse and delta rings of 4; of a query
+// workgroup: k ring of 5, v ring of 3, dS double-buffered (D = 256: all 160 KB)
 template <int D>
 struct Lds {
-  static constexpr int A = 0, B = 4 * Stage<D>::BYTES, X = B + 2 * Stage<D>::BYTES, XBYTES = 16384;
-  static constexpr int LSE = X + 2 * XBYTES, DELTA = LSE + 4 * 256, TOTAL = DELTA + 2 * 256;
+  static constexpr int A = 0, B = 5 * Stage<D>::BYTES, X = B + 3 * Stage<D>::BYTES;
+  static constexpr int PBYTES = 8192, SBYTES = 16384;  // one buffer of P, of dS
+  static constexpr int LSE = X + 2 * PBYTES, DELTA = LSE + 4 * 256, TOTAL = X + 2 * SBYTES;
+  static_assert(DELTA + 4 * 256 <= TOTAL, "lse and delta lie behind P, where a query workgroup has its dS");
 };
 
-// A key workgroup: dk and dv of 128 keys of K/V head hk. Step i: wave 0 makes S(i + 1), then dv += dout(i)^T P(i) while
-// it makes P(i + 1); wave 1 makes dP(i), then dk += q(i - 1)^T dS(i - 1) while it makes dS(i) from P(i).
+// First of the `all` pieces of work that stand behind MFMA m of M, of which the first SKIP have none
+__device__ __forceinline__ constexpr int share(int m, int M, int all) {
+  return m <= SKIP ? 0 : ((m - SKIP) * all + (M - SKIP) - 1) / (M - SKIP);
+}
+
+// i mod M for i in [-M, 2 M)
+template <int M>
+__device__ __forceinline__ int wrap(int i) {
+  return i < 0 ? i + M : i >= M ? i - M : i;
+}
+
+// A key workgroup: dk and dv of 128 keys of K/V head hk. Step i: wave 0 makes S(i + 1), then (behind the barrier) adds
+// dout(i)^T P(i) to dv while it turns S(i + 1) into P(i + 1); wave 1 makes dP(i), then adds q(i - 1)^T dS(i - 1) to dk
+// while it makes dS(i) from dP(i) and P(i).
 template <int D>
 __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) {
   const AttnTrainParams& p = d.p;
   using L = Lds<D>;
-  constexpr int ND = D / 32, SB = Stage<D>::BYTES, EPH = 32 / (4 * ND);  // scores per hook
+  constexpr int ND = D / 32, SB = Stage<D>::BYTES, P = Stage<D>::PIECES;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lq = lane & 31, hh = lane >> 5, pair = wave >> 1;
   const int part = v % d.split_k;
@@ -541,57 +614,61 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
   const int all = tiles * group, per = (all + d.split_k - 1) / d.split_k;
   const int t0 = min(part * per, all), n = min(per, all - t0);
 
-  ReadOff<D> off;
-  off.init(lane);
-  Stage<D> sq, sd;
-  sq.init(p.q_row, wave, lane);
-  sd.init(p.do_row, wave, lane);
-  const unsigned lds0 = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_addr_of(smem));
-  const unsigned wlds = lds0 + wave * Stage<D>::PIECES * 1024;
-  const unsigned ld_off = lane < 32 ? lane * 4 : 0x7ffffff0u;
-  // Stages: rows of the group's heads in turn. Rows past the sequence end and stages past the last are zeros, lse and
-  // delta included: P = exp2(0 - 0) = 1 meets zero rows
-  Stream st_q, st_d, st_x;  // st_x: lse for wave 0, delta for the others (wave 1 copies it)
+  f32x16 acc[2][ND];
+  acc_zero<ND>(acc);
   if (n > 0) {
+    Stage<D> sq, sd;
+    sq.init(p.q_row, wave, lane);
+    sd.init(p.do_row, wave, lane);
+    const unsigned lds0 = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_addr_of(smem));
+    const unsigned wlds = lds0 + wave * 1024;
+    const unsigned ld_off = lane < 32 ? lane * 4 : 0x7ffffff0u;
+    // Stages: rows of the group's heads in turn. Rows past the sequence end and stages past the last are zeros, lse and
+    // delta included: P = exp2(0 - 0) = 1 meets zero rows
+    Stream st_q, st_d, st_x;  // st_x: lse for wave 0, delta for the others (wave 1 copies it)
     const long h0 = (long)hk * group;
     st_q.init(p.q + (long)q_start * p.q_row + h0 * p.q_head, t0, tiles, q_len, n, p.q_row * 2, p.q_head * 2);
     st_d.init(p.dout + (long)q_start * p.do_row + h0 * p.do_head, t0, tiles, q_len, n, p.do_row * 2, p.do_head * 2);
     st_x.init((wave == 0 ? d.lse2 : d.delta) + h0 * p.total_q + q_start, t0, tiles, q_len, n, 4, (long)p.total_q * 4);
-  }
-  i32x4 rq, rd, rx;
-  // the copies of q stage j and dout stage j - 1, in 2 PIECES + 1 pieces
-  auto open = [&]() {
-    rq = st_q.next();
-    rd = st_d.next();
-    rx = st_x.next();
-  };
-  auto copy = [&](int j, int i) {
-    constexpr int P = Stage<D>::PIECES;
-    if (i < P)
-      copy16(rq, sq.voff[i], wlds + L::A + (j & 3) * SB + i * 1024);
-    else if (i < 2 * P)
-      copy16(rd, sd.voff[i - P], wlds + L::B + ((j - 1) & 1) * SB + (i - P) * 1024);
-    else if (i == 2 * P) {
-      if (wave < 2) copy4(rx, ld_off, lds0 + (wave == 0 ? L::LSE + (j & 3) * 256 : L::DELTA + ((j - 1) & 1) * 256));
-    }
-  };
-
-  f32x16 acc[2][ND];
-  acc_zero<ND>(acc);
-  if (n > 0) {
-    // q stages -1 (zeros: dk(-1) adds nothing), 0 and 1, dout stage 0
+    i32x4 rq, rd, rx;
+    int q5 = 0, d3 = 0;  // step mod 5, mod 3
+    // stages i + 2 of q and i + 1 of dout, in 2 P + 1 pieces
+    auto open = [&]() {
+      rq = st_q.next();
+      rd = st_d.next();
+      rx = st_x.next();
+    };
+    auto copy = [&](int i, int k) {
+      if (k < P)
+        copy16(rq, sq.src(k), wlds + L::A + wrap<5>(q5 + 2) * SB + sq.dst(k));
+      else if (k < 2 * P)
+        copy16(rd, sd.src(k - P), wlds + L::B + wrap<3>(d3 + 1) * SB + sd.dst(k - P));
+      else if (k == 2 * P && wave < 2)
+        copy4(rx, ld_off, lds0 + (wave == 0 ? L::LSE + ((i + 2) & 3) * 256 : L::DELTA + ((i + 1) & 3) * 256));
+    };
+    // bytes from slot x of a ring to the next one
+    auto next5 = [&](int x) { return wrap<5>(x) == 4 ? -4 * SB : SB; };
+    auto next3 = [&](int x) { return wrap<3>(x) == 2 ? -2 * SB : SB; };
+    RowReader<D> rr;
+    TrReader<D> tr;
+    // before step 0: q stages -1 (zeros: dk(-1) adds nothing), 0, 1; dout stage 0
     {
-      constexpr int P = Stage<D>::PIECES;
       const i32x4 zero = make_rsrc(p.q, 0);
 #pragma unroll
-      for (int i = 0; i < P; ++i) copy16(zero, sq.voff[i], wlds + L::A + 3 * SB + i * 1024);
-      rq = st_q.next();
+      for (int k = 0; k < P; ++k) copy16(zero, sq.src(k), wlds + L::A + 4 * SB + sq.dst(k));
 #pragma unroll
-      for (int i = 0; i < P; ++i) copy16(rq, sq.voff[i], wlds + L::A + i * 1024);
-      if (wave == 0) copy4(st_x.next(), ld_off, lds0 + L::LSE);
-      open();
+      for (int j = 0; j < 2; ++j) {
+        rq = st_q.next();
 #pragma unroll
-      for (int i = 0; i <= 2 * P; ++i) copy(1, i);
+        for (int k = 0; k < P; ++k) copy16(rq, sq.src(k), wlds + L::A + j * SB + sq.dst(k));
+      }
+      rd = st_d.next();
+#pragma unroll
+      for (int k = 0; k < P; ++k) copy16(rd, sd.src(k), wlds + L::B + sd.dst(k));
+      for (int j = 0; j < (wave == 0 ? 2 : 1); ++j) {
+        rx = st_x.next();
+        if (wave < 2) copy4(rx, ld_off, lds0 + (wave == 0 ? L::LSE : L::DELTA) + j * 256);
+      }
     }
     // stationary rows: k for wave 0, v for wave 1
     bf16x8 f[2][D / 16];
@@ -604,9 +681,24 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
     bf16x8 bc[2][2];  // P (wave 0) or dS (wave 1) of the stage that the tr phase takes, B operands
     u32x4 bn[2][2];   // of the next
     f32x16 s[2];
+    RowAhead<D> ra;
+    TrAhead<D> ta;
     const float sl2 = p.scale * kLog2e;
-    char* const xch = smem + L::X + pair * 8192 + lane * 16;  // [buffer][pair][block][r4][lane] f32x4
+    // P of stage j, fp16: [j & 1][pair][r4][block][lane] 8 B
+    char* const xch = smem + L::X + pair * (L::PBYTES / 2) + lane * 8;
     auto none = [](int) {};
+    auto nothing = []() {};
+    // spreads the 32 scores over the MFMAs m >= SKIP of the tr phase
+    auto spread = [&](int m, auto one) {
+#pragma unroll
+      for (int e = share(m, 4 * ND, 32); e < share(m + 1, 4 * ND, 32); ++e) one(e);
+    };
+    auto next = [&]() {
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) bc[nb][ks] = __builtin_bit_cast(bf16x8, bn[nb][ks]);
+    };
     step_sync();
     if ((wave & 1) == 0) {
       // score e of stage j: group r4 = e >> 3 (rows 8 r4 + 4 hh + 0..3), block (e >> 2) & 1. Each call does the exp2 of
@@ -623,8 +715,11 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
       auto store = [&](int j, int e) {  // P of score e is there
         const int r4 = e >> 3, nb = (e >> 2) & 1, i = e & 3, r = 4 * r4 + i;
         if (i & 1) bn[nb][r >> 3][(r & 7) >> 1] = pack_bf(s[nb][r - 1], s[nb][r]);
-        if (i == 3)
-          *(f32x4*)(xch + (j & 1) * L::XBYTES + (nb * 4 + r4) * 1024) = f32x4{s[nb][r - 3], s[nb][r - 2], s[nb][r - 1], s[nb][r]};
+        if (i == 3) {
+          typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
+          *(f16x4*)(xch + (j & 1) * L::PBYTES + (r4 * 2 + nb) * 512) =
+              f16x4{(_Float16)s[nb][r - 3], (_Float16)s[nb][r - 2], (_Float16)s[nb][r - 1], (_Float16)s[nb][r]};
+        }
       };
       auto begin = [&](int j) { lse_n = *(const f32x4*)(smem + L::LSE + (j & 3) * 256 + 4 * hh * 4); };
       auto prob = [&](int j, int e) {
@@ -634,28 +729,27 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
         if (e > 0) store(j, e - 1);
         if (e == 31) store(j, 31);
       };
-      auto next = [&]() {
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-          for (int ks = 0; ks < 2; ++ks) bc[nb][ks] = __builtin_bit_cast(bf16x8, bn[nb][ks]);
-      };
+      rr.init(lane, lds0 + L::A);
+      tr.init(lane, lds0 + L::B);
       begin(0);
-      row_phase<D>(smem + L::A, off, f, s, none);
+      ra.read(rr);
+      row_phase<D>(rr, ra, f, s, none, nothing);
 #pragma unroll
       for (int e = 0; e < 32; ++e) prob(0, e);
       next();
-      step_sync();
+      rr.move(SB);  // q stage i + 1
+      ra.read(rr);
       for (int i = 0; i < n; ++i) {
         open();
         begin(i + 1);
-        row_phase<D>(smem + L::A + ((i + 1) & 3) * SB, off, f, s, [&](int k) { copy(i + 2, k); });
-        tr_phase<D>(smem + L::B + (i & 1) * SB, off, bc, acc, [&](int m) {
-#pragma unroll
-          for (int e = 0; e < EPH; ++e) prob(i + 1, m * EPH + e);
-        });
-        next();
+        row_phase<D>(rr, ra, f, s, [&](int k) { copy(i, k); }, [&]() { ta.read(tr); });
+        rr.move(next5(q5 + 1));
         step_sync();
+        tr_phase<D>(tr, ta, bc, acc, [&](int m) { spread(m, [&](int e) { prob(i + 1, e); }); }, [&]() { ra.read(rr); });
+        next();
+        tr.move(next3(d3));
+        q5 = wrap<5>(q5 + 1);
+        d3 = wrap<3>(d3 + 1);
       }
       step_sync();
     } else {
@@ -663,36 +757,42 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
       for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) bc[nb][ks] = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
-      step_sync();
-      f32x4 del, pr, del_n, pr_n;
+      rr.init(lane, lds0 + L::B);           // dout stage i
+      tr.init(lane, lds0 + L::A + 4 * SB);  // q stage i - 1
+      ra.read(rr);
+      f32x4 del, del_n;
+      typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
+      f16x4 pr, pr_n;
       for (int i = 0; i <= n; ++i) {
-        open();  // after the last stage: zeros
-        row_phase<D>(smem + L::B + (i & 1) * SB, off, f, s, [&](int k) { copy(i + 2, k); });
         auto rd = [&](int e) {  // delta and P of the 4 scores from e on
           const int r4 = e >> 3, nb = (e >> 2) & 1;
-          if (nb == 0) del_n = *(const f32x4*)(smem + L::DELTA + (i & 1) * 256 + (8 * r4 + 4 * hh) * 4);
-          pr_n = *(const f32x4*)(xch + (i & 1) * L::XBYTES + (nb * 4 + r4) * 1024);
+          if (nb == 0) del_n = *(const f32x4*)(smem + L::DELTA + (i & 3) * 256 + (8 * r4 + 4 * hh) * 4);
+          pr_n = *(const f16x4*)(xch + (i & 1) * L::PBYTES + (r4 * 2 + nb) * 512);
         };
-        rd(0);
-        tr_phase<D>(smem + L::A + ((i - 1) & 3) * SB, off, bc, acc, [&](int m) {
-#pragma unroll
-          for (int e0 = 0; e0 < EPH; ++e0) {
-            const int e = m * EPH + e0;
-            const int nb = (e >> 2) & 1, k = e & 3, r = 4 * (e >> 3) + k;
-            if (k == 0) {
-              pr = pr_n;
-              if (nb == 0) del = del_n;
-              if (e + 4 < 32) rd(e + 4);
-            }
-            s[nb][r] = pr[k] * (s[nb][r] - del[k]);
-            if (k & 1) bn[nb][r >> 3][(r & 7) >> 1] = pack_bf(s[nb][r - 1], s[nb][r]);
-          }
-        });
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-          for (int ks = 0; ks < 2; ++ks) bc[nb][ks] = __builtin_bit_cast(bf16x8, bn[nb][ks]);
+        open();  // after the last stage: zeros
+        row_phase<D>(rr, ra, f, s, [&](int k) { copy(i, k); }, [&]() { ta.read(tr); });
+        rr.move(next3(d3));
         step_sync();
+        rd(0);
+        tr_phase<D>(
+            tr, ta, bc, acc,
+            [&](int m) {
+              spread(m, [&](int e) {
+                const int nb = (e >> 2) & 1, k = e & 3, r = 4 * (e >> 3) + k;
+                if (k == 0) {
+                  pr = pr_n;
+                  if (nb == 0) del = del_n;
+                  if (e + 4 < 32) rd(e + 4);
+                }
+                s[nb][r] = (float)pr[k] * (s[nb][r] - del[k]);
+                if (k & 1) bn[nb][r >> 3][(r & 7) >> 1] = pack_bf(s[nb][r - 1], s[nb][r]);
+              });
+            },
+            [&]() { ra.read(rr); });
+        next();
+        tr.move(next5(q5 + 4));
+        q5 = wrap<5>(q5 + 1);
+        d3 = wrap<3>(d3 + 1);
       }
     }
   }
@@ -702,13 +802,14 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
     const int row = row0 + pair * 64 + nb * 32 + lq;
     const bool live = row < k_len;
     const long rc = k_start + min(row, k_len - 1);
+    const float f = wave & 1 ? p.scale * kUnshift : kUnshift;
     if (d.split_k > 1) {
       const long to = (((long)part * p.total_k + rc) * p.HK + hk) * D;
-      store_part<D>((wave & 1 ? d.part_k : d.part_v) + to, acc[nb], wave & 1 ? p.scale : 1.f, hh, live);
+      store_part<D>((wave & 1 ? d.part_k : d.part_v) + to, acc[nb], f, hh, live);
     } else if (wave & 1) {
-      store_row<D>(p.dk + rc * p.dk_row + (long)hk * p.dk_head, acc[nb], p.scale, hh, live);
+      store_row<D>(p.dk + rc * p.dk_row + (long)hk * p.dk_head, acc[nb], f, hh, live);
     } else {
-      store_row<D>(p.dv + rc * p.dv_row + (long)hk * p.dv_head, acc[nb], 1.f, hh, live);
+      store_row<D>(p.dv + rc * p.dv_row + (long)hk * p.dv_head, acc[nb], f, hh, live);
     }
   }
 }
@@ -719,7 +820,7 @@ template <int D>
 __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem) {
   const AttnTrainParams& p = d.p;
   using L = Lds<D>;
-  constexpr int ND = D / 32, NS = D / 16, SB = Stage<D>::BYTES;
+  constexpr int ND = D / 32, NS = D / 16, SB = Stage<D>::BYTES, P = Stage<D>::PIECES;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lq = lane & 31, hh = lane >> 5, pair = wave >> 1;
   const int part = v % d.split_q;
@@ -736,41 +837,45 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
   const int all = (k_len + 31) / 32, per = (all + d.split_q - 1) / d.split_q;
   const int t0 = min(part * per, all), n = min(per, all - t0);
 
-  ReadOff<D> off;
-  off.init(lane);
   Stage<D> sk, sv;
   sk.init(p.k_row, wave, lane);
   sv.init(p.v_row, wave, lane);
   const unsigned lds0 = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_addr_of(smem));
-  const unsigned wlds = lds0 + wave * Stage<D>::PIECES * 1024;
+  const unsigned wlds = lds0 + wave * 1024;
   Stream st_k, st_v;
   if (n > 0) {
     st_k.init(p.k + (long)k_start * p.k_row + (long)hk * p.k_head, t0, all, k_len, n, p.k_row * 2, 0);
     st_v.init(p.v + (long)k_start * p.v_row + (long)hk * p.v_head, t0, all, k_len, n, p.v_row * 2, 0);
   }
   i32x4 rk, rv;
+  int k5 = 0, v3 = 0;  // step mod 5, mod 3
   auto open = [&]() {
     rk = st_k.next();
     rv = st_v.next();
   };
-  auto copy = [&](int j, int i) {  // piece i of k and v stage j
-    constexpr int P = Stage<D>::PIECES;
-    if (i < P)
-      copy16(rk, sk.voff[i], wlds + L::A + (j & 3) * SB + i * 1024);
-    else if (i < 2 * P)
-      copy16(rv, sv.voff[i - P], wlds + L::B + (j & 1) * SB + (i - P) * 1024);
+  auto copy = [&](int j, int k) {  // piece k of k and v stage i + j
+    if (k < P)
+      copy16(rk, sk.src(k), wlds + L::A + wrap<5>(k5 + j) * SB + sk.dst(k));
+    else if (k < 2 * P)
+      copy16(rv, sv.src(k - P), wlds + L::B + wrap<3>(v3 + (j == 3 ? 0 : j)) * SB + sv.dst(k - P));
   };
   auto copy_all = [&](int j) {
     open();
 #pragma unroll
-    for (int i = 0; i < 2 * Stage<D>::PIECES; ++i) copy(j, i);
+    for (int k = 0; k < 2 * P; ++k) copy(j, k);
+  };
+  auto advance = [&]() {
+    k5 = wrap<5>(k5 + 1);
+    v3 = wrap<3>(v3 + 1);
   };
 
-  char* const xch = smem + L::X + pair * 8192 + lane * 16;  // [buffer][pair][block][hi 2, lo 2][lane] 16 B
+  // dS of stage j: [j & 1][pair][block][r4][lane] f32x4
+  char* const xch = smem + L::X + pair * (L::SBYTES / 2) + lane * 16;
   if ((wave & 1) == 0) {
     if (n <= 0) return;  // wave 1 stores the zeros
     copy_all(0);
     copy_all(1);
+    copy_all(2);
     bf16x8 qf[2][NS], df[2][NS];
     float lse[2], del[2];
 #pragma unroll
@@ -791,20 +896,9 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
     asm volatile("s_nop 4" ::: "memory");
     const float sl2 = p.scale * kLog2e;
     f32x16 sa[2], da[2], sb[2], db[2];
-    u32x4 hi, lo;
     // Half u of the 64 that make stage j's dS from its S and dP: element e = u >> 1 (block e >> 4, score e & 15); even
-    // halves do an exp2 and the next one's argument, odd ones the products and the split of the pair before
+    // halves do an exp2 and the next one's argument, odd ones the product
     float x, pe;
-    auto split = [&](int j, f32x16 (&s)[2], int e) {  // e odd: dS of e - 1 and e -> hi, lo
-      const int nb = e >> 4, r = e & 15, w = (r & 7) >> 1;
-      const unsigned h2 = hi[w];
-      lo[w] = pack_bf(s[nb][r - 1] - __uint_as_float(h2 << 16), s[nb][r] - __uint_as_float(h2 & 0xffff0000u));
-      if (w == 3) {
-        char* to = xch + (j & 1) * L::XBYTES + nb * 4096 + (r >> 3) * 1024;
-        *(u32x4*)to = hi;
-        *(u32x4*)(to + 2048) = lo;
-      }
-    };
     auto ds_half = [&](int j, f32x16 (&s)[2], f32x16 (&dp)[2], int u) {
       const int e = u >> 1, nb = e >> 4, r = e & 15;
       if ((u & 1) == 0) {
@@ -813,41 +907,40 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
         if (e < 31) x = __builtin_fmaf(s[(e + 1) >> 4][(e + 1) & 15], sl2, -lse[(e + 1) >> 4]);
       } else {
         s[nb][r] = pe * (dp[nb][r] - del[nb]);
-        if (e & 1)
-          hi[(r & 7) >> 1] = pack_bf(s[nb][r - 1], s[nb][r]);
-        else if (e > 0)
-          split(j, s, e - 1);
-        if (e == 31) split(j, s, 31);
+        if ((r & 3) == 3)
+          *(f32x4*)(xch + (j & 1) * L::SBYTES + (nb * 4 + (r >> 2)) * 1024) =
+              f32x4{s[nb][r - 3], s[nb][r - 2], s[nb][r - 1], s[nb][r]};
       }
     };
-    // S and dP of stage j into (s, dp); hook(u) after each of the 4 NS MFMAs
-    auto products = [&](int j, f32x16 (&s)[2], f32x16 (&dp)[2], auto hook) {
-      const char* ks = smem + L::A + (j & 3) * SB;
-      const char* vs = smem + L::B + (j & 1) * SB;
-      constexpr int AHEAD = 5;
-      bf16x8 a[2 * NS];
-      auto rd = [&](int m) { a[m] = off.read_row(m & 1 ? vs : ks, m >> 1); };
+    constexpr int AHEAD = 5;
+    bf16x8 first[AHEAD];
+    RowReader<D> kr, vr;
+    kr.init(lane, lds0 + L::A);
+    vr.init(lane, lds0 + L::B);
+    auto rd = [&](int m) { return m & 1 ? vr.read(m >> 1) : kr.read(m >> 1); };
+    auto read_first = [&]() {
 #pragma unroll
-      for (int m = 0; m < AHEAD; ++m) rd(m);
-      FENCE();
+      for (int m = 0; m < AHEAD; ++m) first[m] = rd(m);
+    };
+    // S and dP of the readers' stage into (s, dp); hook(u) after each of the 4 NS MFMAs. last() may move the readers on
+    auto products = [&](f32x16 (&s)[2], f32x16 (&dp)[2], auto hook, auto last) {
+      bf16x8 a[2 * NS];
+#pragma unroll
+      for (int m = 0; m < AHEAD; ++m) a[m] = first[m];
 #pragma unroll
       for (int m = 0; m < 2 * NS; ++m) {
         f32x16(&acc)[2] = m & 1 ? dp : s;
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb) {
           const bf16x8& f = m & 1 ? df[nb][m >> 1] : qf[nb][m >> 1];
-          if (m < 2)
-            mfma_s_first(acc[nb], a[m], f);
-          else
-            mfma_s(acc[nb], a[m], f);
+          acc[nb] = mfma(a[m], f, m < 2 ? zero16() : acc[nb]);
           FENCE();
-          if (nb == 0 && m + AHEAD < 2 * NS) rd(m + AHEAD);
+          if (nb == 0 && m + AHEAD < 2 * NS) a[m + AHEAD] = rd(m + AHEAD);
+          if (nb == 0 && m + AHEAD == 2 * NS) last();
           hook(2 * m + nb);
           FENCE();
         }
       }
-      mfma_read_fence(s[0], s[1]);
-      mfma_read_fence(dp[0], dp[1]);
     };
     auto mask = [&](int j, f32x16 (&s)[2]) {  // keys past the end: P = 0 (their exp2(-lse) may overflow)
       const int left = k_len - (t0 + j) * 32;
@@ -860,16 +953,27 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
     auto step = [&](int i, f32x16 (&s)[2], f32x16 (&dp)[2], f32x16 (&s2)[2], f32x16 (&dp2)[2]) {
       open();
       mask(i, s);
-      constexpr int UPH = 64 / (4 * NS);
-      products(i + 1, s2, dp2, [&](int m) {
+      products(
+          s2, dp2,
+          [&](int m) {
 #pragma unroll
-        for (int u = 0; u < UPH; ++u) ds_half(i, s, dp, m * UPH + u);
-        if (m & 1) copy(i + 2, m >> 1);
-      });
+            for (int u = share(m, 4 * NS, 64); u < share(m + 1, 4 * NS, 64); ++u) ds_half(i, s, dp, u);
+            if ((m & 1) && (m >> 1) < 2 * P) copy(3, m >> 1);
+          },
+          [&]() {
+            kr.move(wrap<5>(k5 + 1) == 4 ? -4 * SB : SB);
+            vr.move(wrap<3>(v3 + 1) == 2 ? -2 * SB : SB);
+            read_first();
+          });
+      advance();
       step_sync();
     };
     step_sync();
-    products(0, sa, da, [](int) {});
+    read_first();
+    products(sa, da, [](int) {}, []() {});
+    kr.move(SB);
+    vr.move(SB);
+    read_first();
     step_sync();
     int i = 0;
     for (; i + 1 < n; i += 2) {
@@ -884,43 +988,83 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
   if (n > 0) {
     copy_all(0);
     copy_all(1);
-    step_sync();
-    step_sync();
     copy_all(2);
+    step_sync();
+    step_sync();
+    copy_all(3);
+    bf16x8 a[ND];
+    TrReader<D> tr;  // k stage i - 1
+    tr.init(lane, lds0 + L::A);
+    auto rd = [&](int s, int dt) { a[dt] = tr.read(s, dt); };
+    advance();
     step_sync();
     for (int i = 1; i <= n; ++i) {
       open();  // after the last stage: zeros
-      {
-        const char* ks = smem + L::A + ((i - 1) & 3) * SB;
-        const char* x = xch + ((i - 1) & 1) * L::XBYTES;
-        bf16x8 hi[2][2], lo[2][2];
+      const char* x = xch + ((i - 1) & 1) * L::SBYTES;
+      f32x4 w[2][4];
 #pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
+      for (int r4 = 0; r4 < 4; ++r4)
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            hi[nb][s] = *(const bf16x8*)(x + nb * 4096 + s * 1024);
-            lo[nb][s] = *(const bf16x8*)(x + nb * 4096 + 2048 + s * 1024);
-          }
-        constexpr int AHEAD = 2;
-        bf16x8 a[2 * ND];
+        for (int nb = 0; nb < 2; ++nb) w[nb][r4] = *(const f32x4*)(x + (nb * 4 + r4) * 1024);
 #pragma unroll
-        for (int m = 0; m < AHEAD; ++m) a[m] = off.read_tr(ks, m / ND, m % ND);
+      for (int dt = 0; dt < ND; ++dt) rd(0, dt);
+      u32x4 hi[2][2], lo[2][2];
+      auto split_hi = [&](int s, int q) {  // pair q of 8: block q >> 2, scores 8 s + 2 (q & 3), + 1
+        const int nb = q >> 2, c = q & 3;
+        const f32x4& y = w[nb][2 * s + (c >> 1)];
+        hi[nb][s][c] = pack_bf(y[2 * (c & 1)], y[2 * (c & 1) + 1]);
+      };
+      auto split_lo = [&](int s, int q) {
+        const int nb = q >> 2, c = q & 3;
+        const f32x4& y = w[nb][2 * s + (c >> 1)];
+        const unsigned h2 = hi[nb][s][c];
+        lo[nb][s][c] = pack_bf(y[2 * (c & 1)] - __uint_as_float(h2 << 16),
+                               y[2 * (c & 1) + 1] - __uint_as_float(h2 & 0xffff0000u));
+      };
+#pragma unroll
+      for (int q = 0; q < 8; ++q) split_hi(0, q);
+      FENCE();
+      // VALU write -> asm MFMA read (the compiler does not look into asm): two wait states before each run of MFMAs
+      auto settle = []() {
         FENCE();
+        asm volatile("s_nop 1");
+        FENCE();
+      };
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        settle();
+        // hi: 2 ND MFMAs; beside them the low parts
 #pragma unroll
         for (int m = 0; m < 2 * ND; ++m) {
-          mfma_o<false>(acc[0][m % ND], a[m], hi[0][m / ND]);
+          bf16x8 bb = __builtin_bit_cast(bf16x8, hi[m & 1][s]);
+          mfma_o<false>(acc[m & 1][m >> 1], a[m >> 1], bb);
           FENCE();
-          if (m + AHEAD < 2 * ND) a[m + AHEAD] = off.read_tr(ks, (m + AHEAD) / ND, (m + AHEAD) % ND);
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (s == 0 && q * ND / 4 == m) split_lo(0, q);
+          if (s == 1 && (m & 1)) copy(3, P + (m >> 1));
           FENCE();
-          mfma_o<false>(acc[1][m % ND], a[m], hi[1][m / ND]);
+        }
+        settle();
+        // lo: the fragments once more, then their place takes the next half's; beside them the next half's split
+#pragma unroll
+        for (int m = 0; m < 2 * ND; ++m) {
+          bf16x8 bb = __builtin_bit_cast(bf16x8, lo[m & 1][s]);
+          mfma_o<false>(acc[m & 1][m >> 1], a[m >> 1], bb);
           FENCE();
-          copy(i + 2, m);
-          FENCE();
-          mfma_o<false>(acc[0][m % ND], a[m], lo[0][m / ND]);
-          mfma_o<false>(acc[1][m % ND], a[m], lo[1][m / ND]);
+          if (s == 0 && (m & 1)) rd(1, m >> 1);
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (s == 0 && q * ND / 4 == m) {
+              split_hi(1, q);
+              split_lo(1, q);
+            }
+          if (s == 0 && !(m & 1) && (m >> 1) < P) copy(3, m >> 1);
           FENCE();
         }
       }
+      tr.move(wrap<5>(k5 + 4) == 4 ? -4 * SB : SB);
+      advance();
       if (i < n) step_sync();
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may outlive the workgroup
@@ -931,10 +1075,11 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
     const int row = row0 + pair * 64 + nb * 32 + lq;
     const bool live = row < q_len;
     const long rc = q_start + min(row, q_len - 1);
+    const float f = p.scale * kUnshift;
     if (d.split_q > 1)
-      store_part<D>(d.part_q + (((long)part * p.total_q + rc) * p.H + h) * D, acc[nb], p.scale, hh, live);
+      store_part<D>(d.part_q + (((long)part * p.total_q + rc) * p.H + h) * D, acc[nb], f, hh, live);
     else
-      store_row<D>(p.dq + rc * p.dq_row + (long)h * p.dq_head, acc[nb], p.scale, hh, live);
+      store_row<D>(p.dq + rc * p.dq_row + (long)h * p.dq_head, acc[nb], f, hh, live);
   }
 }
 
