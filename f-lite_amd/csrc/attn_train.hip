@@ -632,7 +632,7 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
     st_x.init((wave == 0 ? d.lse2 : d.delta) + h0 * p.total_q + q_start, t0, tiles, q_len, n, 4, (long)p.total_q * 4);
     i32x4 rq, rd, rx;
     int q5 = 0, d3 = 0;  // step mod 5, mod 3
-    // stages i + 2 of q and i + 1 of dout, in 2 P + 1 pieces
+    // stages i + 3 of q and i + 2 of dout, in 2 P + 1 pieces: issued behind step i's barrier, in place at the next one
     auto open = [&]() {
       rq = st_q.next();
       rd = st_d.next();
@@ -640,32 +640,35 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
     };
     auto copy = [&](int i, int k) {
       if (k < P)
-        copy16(rq, sq.src(k), wlds + L::A + wrap<5>(q5 + 2) * SB + sq.dst(k));
+        copy16(rq, sq.src(k), wlds + L::A + wrap<5>(q5 + 3) * SB + sq.dst(k));
       else if (k < 2 * P)
-        copy16(rd, sd.src(k - P), wlds + L::B + wrap<3>(d3 + 1) * SB + sd.dst(k - P));
+        copy16(rd, sd.src(k - P), wlds + L::B + wrap<3>(d3 + 2) * SB + sd.dst(k - P));
       else if (k == 2 * P && wave < 2)
-        copy4(rx, ld_off, lds0 + (wave == 0 ? L::LSE + ((i + 2) & 3) * 256 : L::DELTA + ((i + 1) & 3) * 256));
+        copy4(rx, ld_off, lds0 + (wave == 0 ? L::LSE + ((i + 3) & 3) * 256 : L::DELTA + ((i + 2) & 3) * 256));
     };
     // bytes from slot x of a ring to the next one
     auto next5 = [&](int x) { return wrap<5>(x) == 4 ? -4 * SB : SB; };
     auto next3 = [&](int x) { return wrap<3>(x) == 2 ? -2 * SB : SB; };
     RowReader<D> rr;
     TrReader<D> tr;
-    // before step 0: q stages -1 (zeros: dk(-1) adds nothing), 0, 1; dout stage 0
+    // before step 0: q stages -1 (zeros: dk(-1) adds nothing), 0, 1, 2; dout stages 0, 1
     {
       const i32x4 zero = make_rsrc(p.q, 0);
 #pragma unroll
       for (int k = 0; k < P; ++k) copy16(zero, sq.src(k), wlds + L::A + 4 * SB + sq.dst(k));
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 3; ++j) {
         rq = st_q.next();
 #pragma unroll
         for (int k = 0; k < P; ++k) copy16(rq, sq.src(k), wlds + L::A + j * SB + sq.dst(k));
       }
-      rd = st_d.next();
 #pragma unroll
-      for (int k = 0; k < P; ++k) copy16(rd, sd.src(k), wlds + L::B + sd.dst(k));
-      for (int j = 0; j < (wave == 0 ? 2 : 1); ++j) {
+      for (int j = 0; j < 2; ++j) {
+        rd = st_d.next();
+#pragma unroll
+        for (int k = 0; k < P; ++k) copy16(rd, sd.src(k), wlds + L::B + j * SB + sd.dst(k));
+      }
+      for (int j = 0; j < (wave == 0 ? 3 : 2); ++j) {
         rx = st_x.next();
         if (wave < 2) copy4(rx, ld_off, lds0 + (wave == 0 ? L::LSE : L::DELTA) + j * 256);
       }
@@ -688,8 +691,10 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
     char* const xch = smem + L::X + pair * (L::PBYTES / 2) + lane * 8;
     auto none = [](int) {};
     auto nothing = []() {};
-    // spreads the 32 scores over the MFMAs m >= SKIP of the tr phase
-    auto spread = [&](int m, auto one) {
+    // work behind MFMA m of the tr phase: copies of step i, and the 32 scores spread over the MFMAs m >= SKIP
+    auto spread = [&](int i, int m, auto one) {
+      constexpr int E = (4 * ND) / (2 * P + 1);
+      if (m % E == 0 && m / E <= 2 * P) copy(i, m / E);
 #pragma unroll
       for (int e = share(m, 4 * ND, 32); e < share(m + 1, 4 * ND, 32); ++e) one(e);
     };
@@ -742,10 +747,10 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
       for (int i = 0; i < n; ++i) {
         open();
         begin(i + 1);
-        row_phase<D>(rr, ra, f, s, [&](int k) { copy(i, k); }, [&]() { ta.read(tr); });
+        row_phase<D>(rr, ra, f, s, none, [&]() { ta.read(tr); });
         rr.move(next5(q5 + 1));
         step_sync();
-        tr_phase<D>(tr, ta, bc, acc, [&](int m) { spread(m, [&](int e) { prob(i + 1, e); }); }, [&]() { ra.read(rr); });
+        tr_phase<D>(tr, ta, bc, acc, [&](int m) { spread(i, m, [&](int e) { prob(i + 1, e); }); }, [&]() { ra.read(rr); });
         next();
         tr.move(next3(d3));
         q5 = wrap<5>(q5 + 1);
@@ -770,14 +775,14 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
           pr_n = *(const f16x4*)(xch + (i & 1) * L::PBYTES + (r4 * 2 + nb) * 512);
         };
         open();  // after the last stage: zeros
-        row_phase<D>(rr, ra, f, s, [&](int k) { copy(i, k); }, [&]() { ta.read(tr); });
+        row_phase<D>(rr, ra, f, s, none, [&]() { ta.read(tr); });
         rr.move(next3(d3));
         step_sync();
         rd(0);
         tr_phase<D>(
             tr, ta, bc, acc,
             [&](int m) {
-              spread(m, [&](int e) {
+              spread(i, m, [&](int e) {
                 const int nb = (e >> 2) & 1, k = e & 3, r = 4 * (e >> 3) + k;
                 if (k == 0) {
                   pr = pr_n;
@@ -795,6 +800,7 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
         d3 = wrap<3>(d3 + 1);
       }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may outlive the workgroup
   }
   acc_fence<ND>(acc);
 #pragma unroll
