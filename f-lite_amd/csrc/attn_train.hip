@@ -38,18 +38,30 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int WROWS = 128;  // stationary rows of a workgroup
 constexpr int TR = 64;      // swept rows of an LDS tile
 constexpr int kThreads = 256;
-constexpr int kMaxSplit = 16;
+constexpr int kMaxRanges = 16;
+constexpr int kMinRange = 8;  // stages: what a workgroup's start and end cost
+constexpr int kCus = 256;
+
+// How a launch cuts its work. A unit is one 128-row tile ("full", or the rest of a sequence, "part") of one head with
+// its whole sweep; where units are few or long, a sweep is cut into ranges, whose fp32 partial gradients a last kernel
+// adds in range order.
+struct Cut {
+  int full;            // upper bound of the batch's full tiles
+  int heads;
+  int max_full, max_part;  // ranges that the workspace has room for
+  float* ws_full;      // [max_full][total][heads][D], with max_full > 1
+  float* ws_part;      // [max_part][B][128][heads][D], with max_part > 1
+  __host__ __device__ int full_blocks() const { return full * heads * max_full; }
+  __host__ __device__ int blocks(int B) const { return full_blocks() + B * heads * max_part; }
+};
 
 struct TrainDev {
   AttnTrainParams p;
-  int tiles_q, tiles_k;    // upper bounds of the packed batch's 128-row tiles
-  int split_q, split_k;    // ranges that a query / key workgroup's sweep is cut into
-  int n_key_blocks;        // backward: the first blocks of the launch are key workgroups
+  int tiles_q;             // forward: upper bound of the 128-row tiles
+  Cut q, k;
+  int* target;             // stages per range: of a full tile, of a part
   float* lse2;             // [H][total_q] lse * log2 e - kShift
   float* delta;            // [H][total_q]
-  float* part_q;           // [split_q][total_q][H][D] fp32, with split_q > 1
-  float* part_k;           // [split_k][total_k][HK][D]
-  float* part_v;
 };
 
 // One sequence's rows [start, start + len) of `total`, from a cumulative array that a caller may have filled wrongly:
@@ -85,6 +97,86 @@ __device__ __forceinline__ bool find_tile(const int* cu, int B, int total, int t
     t -= __shfl(sum, 63, 64);
   }
   return false;
+}
+
+// Full tile t of the packed batch -> (sequence, first row); false past the last one
+__device__ __forceinline__ bool find_full(const int* cu, int B, int total, int t, int* b, int* row0) {
+  const int lane = threadIdx.x & 63;
+  for (int base = 0; base < B; base += 64) {
+    int s, len = 0;
+    if (base + lane < B) seq_range(cu, base + lane, total, &s, &len);
+    const int n = len / WROWS;
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += up;
+    }
+    const unsigned long long hit = __ballot(t < sum);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      *b = base + l;
+      *row0 = (t - (__shfl(sum, l, 64) - __shfl(n, l, 64))) * WROWS;
+      return true;
+    }
+    t -= __shfl(sum, 63, 64);
+  }
+  return false;
+}
+
+// Sequence that holds `row`, -1: none
+__device__ __forceinline__ int find_seq(const int* cu, int B, int total, int row) {
+  int lo = 0, hi = B;  // the last b with cu[b] <= row
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    (cu[mid] <= row ? lo : hi) = mid;
+  }
+  int s, len;
+  seq_range(cu, lo, total, &s, &len);
+  return row >= s && row < s + len ? lo : -1;
+}
+
+// Ranges of a sweep of `stages`
+__device__ __forceinline__ int ranges_of(int stages, int target, int most) {
+  return min(max((stages + target - 1) / target, 1), most);
+}
+
+// One unit and range of the sweep over it
+struct Unit {
+  int b, h, row0, part;
+  bool full;
+};
+// Block v of `c` -> its unit; false: nothing to do. own: the tiles' cu_seqlens
+__device__ __forceinline__ bool find_unit(const Cut& c, int v, const int* own, int B, int total, Unit* u) {
+  const int nf = c.full_blocks();
+  u->full = v < nf;
+  if (u->full) {
+    u->part = v % c.max_full;
+    v /= c.max_full;
+    u->h = v / c.full;
+    if (!find_full(own, B, total, v % c.full, &u->b, &u->row0)) return false;
+  } else {
+    v -= nf;
+    u->part = v % c.max_part;
+    v /= c.max_part;
+    u->b = v % B;
+    u->h = v / B;
+    int s, len;
+    seq_range(own, u->b, total, &s, &len);
+    if (len % WROWS == 0) return false;
+    u->row0 = len - len % WROWS;
+  }
+  u->b = __builtin_amdgcn_readfirstlane(u->b);
+  u->row0 = __builtin_amdgcn_readfirstlane(u->row0);
+  return true;
+}
+// Row `row` of sequence b, head h, range 0 in the partial gradients; *step: floats from range to range
+template <int D>
+__device__ __forceinline__ float* part_row(const Cut& c, bool full, int B, int total, int start, int b, int row, int h,
+                                           long* step) {
+  *step = (long)(full ? total : B * WROWS) * c.heads * D;
+  const long r = full ? (long)start + row : (long)b * WROWS + row % WROWS;
+  return (full ? c.ws_full : c.ws_part) + (r * c.heads + h) * D;
 }
 
 // XOR of the 16-B chunk index of tile row r. The low 4 bits of a row map one to one onto the XOR (row reads of 16 lanes
@@ -206,6 +298,20 @@ __device__ __forceinline__ void store_part(float* dst, const f32x16 (&acc)[D / 3
     __syncthreads();                                 \
   } while (0)
 
+// Zeros (lse: -inf) in the rows before the first and behind the last sequence, by `blocks` workgroups of which this is
+// number i
+__device__ __forceinline__ void zero_outside(bf16_t* out, long row_stride, long head_stride, const int* cu, int B, int total,
+                                             int H, int D, float* lse, int i, int blocks) {
+  const int first = min(max(cu[0], 0), total), behind = min(max(cu[B], first), total);
+  const long n = (long)(first + total - behind) * H * (D / 8);
+  for (long e = (long)i * kThreads + threadIdx.x; e < n; e += (long)blocks * kThreads) {
+    const int c = (int)(e % (D / 8)) * 8, h = (int)(e / (D / 8) % H), r = (int)(e / (D / 8) / H);
+    const int row = r < first ? r : behind + r - first;
+    *(u32x4*)(out + (long)row * row_stride + (long)h * head_stride + c) = u32x4{0u, 0u, 0u, 0u};
+    if (lse != nullptr && c == 0) lse[(long)h * total + row] = -INFINITY;
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ forward
 template <int D>
 __global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
@@ -214,7 +320,12 @@ __global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
   constexpr int TB = TR * D * 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lq = lane & 31, hh = lane >> 5;
-  const int v = xcd_remap(blockIdx.x, gridDim.x);
+  const int n_tiles = d.tiles_q * p.H;
+  if ((int)blockIdx.x >= n_tiles) {
+    zero_outside(p.o, p.o_row, p.o_head, p.cu_q, p.B, p.total_q, p.H, D, p.lse, blockIdx.x - n_tiles, gridDim.x - n_tiles);
+    return;
+  }
+  const int v = xcd_remap(blockIdx.x, n_tiles);
   const int h = v / d.tiles_q;
   int b, row0;
   if (!find_tile(p.cu_q, p.B, p.total_q, v % d.tiles_q, &b, &row0)) return;
@@ -289,11 +400,39 @@ __global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// (lse * log2 e, delta) of every query row; rows outside all sequences are not read by anyone
+// First launch of the backward pass: lse * log2 e and delta of every query row (those outside all sequences are read by
+// nobody); the ranges' length; zeros outside
 template <int D>
-__global__ __launch_bounds__(kThreads) void attn_delta_kernel(TrainDev d) {
+__global__ __launch_bounds__(kThreads) void attn_delta_kernel(TrainDev d, int row_blocks) {
   const AttnTrainParams& p = d.p;
   constexpr int LANES = D / 8;
+  if ((int)blockIdx.x >= row_blocks) {
+    const int i = blockIdx.x - row_blocks, n = gridDim.x - row_blocks;
+    if (i == 0 && threadIdx.x < 64) {
+      // Stages of all units, over the CUs: a range of a full tile is at most half of a CU's share, one of a part (they
+      // fill the end of the launch) a 32nd; none is shorter than kMinRange
+      double sum = 0.;
+      for (int b = threadIdx.x; b < p.B; b += 64) {
+        int s, ql, kl;
+        seq_range(p.cu_q, b, p.total_q, &s, &ql);
+        seq_range(p.cu_k, b, p.total_k, &s, &kl);
+        sum += ((double)((ql + WROWS - 1) / WROWS) * ((kl + 31) / 32) + (double)((kl + WROWS - 1) / WROWS) * ((ql + 31) / 32)) * p.H;
+      }
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+      if (threadIdx.x == 0) {
+        const double share = fmin(sum / kCus, 1e9);
+        d.target[0] = max((int)(share / 2), kMinRange);
+        d.target[1] = max((int)(share / 32), kMinRange);
+      }
+    }
+    if (p.zero_outside) {
+      zero_outside(p.dq, p.dq_row, p.dq_head, p.cu_q, p.B, p.total_q, p.H, D, nullptr, i, n);
+      zero_outside(p.dk, p.dk_row, p.dk_head, p.cu_k, p.B, p.total_k, p.HK, D, nullptr, i, n);
+      zero_outside(p.dv, p.dv_row, p.dv_head, p.cu_k, p.B, p.total_k, p.HK, D, nullptr, i, n);
+    }
+    return;
+  }
   const long item = ((long)blockIdx.x * kThreads + threadIdx.x) / LANES;
   const int c = threadIdx.x % LANES;
   if (item >= (long)p.total_q * p.H) return;
@@ -599,20 +738,18 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
   constexpr int ND = D / 32, SB = Stage<D>::BYTES, P = Stage<D>::PIECES;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lq = lane & 31, hh = lane >> 5, pair = wave >> 1;
-  const int part = v % d.split_k;
-  v /= d.split_k;
-  const int hk = v / d.tiles_k;
-  int b, row0;
-  if (!find_tile(p.cu_k, p.B, p.total_k, v % d.tiles_k, &b, &row0)) return;
-  b = __builtin_amdgcn_readfirstlane(b);
-  row0 = __builtin_amdgcn_readfirstlane(row0);
+  Unit u;
+  if (!find_unit(d.k, v, p.cu_k, p.B, p.total_k, &u)) return;
+  const int hk = u.h, b = u.b, row0 = u.row0;
   int q_start, q_len, k_start, k_len;
   seq_range(p.cu_q, b, p.total_q, &q_start, &q_len);
   seq_range(p.cu_k, b, p.total_k, &k_start, &k_len);
   const int group = p.H / p.HK;
   const int tiles = (q_len + 31) / 32;  // stages of one head
-  const int all = tiles * group, per = (all + d.split_k - 1) / d.split_k;
-  const int t0 = min(part * per, all), n = min(per, all - t0);
+  const int all = tiles * group;
+  const int ranges = ranges_of(all, d.target[u.full ? 0 : 1], u.full ? d.k.max_full : d.k.max_part);
+  if (u.part >= ranges) return;
+  const int per = (all + ranges - 1) / ranges, t0 = min(u.part * per, all), n = min(per, all - t0);
 
   f32x16 acc[2][ND];
   acc_zero<ND>(acc);
@@ -809,9 +946,12 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
     const bool live = row < k_len;
     const long rc = k_start + min(row, k_len - 1);
     const float f = wave & 1 ? p.scale * kUnshift : kUnshift;
-    if (d.split_k > 1) {
-      const long to = (((long)part * p.total_k + rc) * p.HK + hk) * D;
-      store_part<D>((wave & 1 ? d.part_k : d.part_v) + to, acc[nb], f, hh, live);
+    if (ranges > 1) {
+      // dv's partials follow all of dk's
+      long step;
+      float* to = part_row<D>(d.k, u.full, p.B, p.total_k, k_start, b, min(row, k_len - 1), hk, &step);
+      to += (u.part + (wave & 1 ? 0 : u.full ? d.k.max_full : d.k.max_part)) * step;
+      store_part<D>(to, acc[nb], f, hh, live);
     } else if (wave & 1) {
       store_row<D>(p.dk + rc * p.dk_row + (long)hk * p.dk_head, acc[nb], f, hh, live);
     } else {
@@ -829,19 +969,17 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
   constexpr int ND = D / 32, NS = D / 16, SB = Stage<D>::BYTES, P = Stage<D>::PIECES;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lq = lane & 31, hh = lane >> 5, pair = wave >> 1;
-  const int part = v % d.split_q;
-  v /= d.split_q;
-  const int h = v / d.tiles_q;
-  int b, row0;
-  if (!find_tile(p.cu_q, p.B, p.total_q, v % d.tiles_q, &b, &row0)) return;
-  b = __builtin_amdgcn_readfirstlane(b);
-  row0 = __builtin_amdgcn_readfirstlane(row0);
+  Unit u;
+  if (!find_unit(d.q, v, p.cu_q, p.B, p.total_q, &u)) return;
+  const int h = u.h, b = u.b, row0 = u.row0;
   int q_start, q_len, k_start, k_len;
   seq_range(p.cu_q, b, p.total_q, &q_start, &q_len);
   seq_range(p.cu_k, b, p.total_k, &k_start, &k_len);
   const int hk = h / (p.H / p.HK);
-  const int all = (k_len + 31) / 32, per = (all + d.split_q - 1) / d.split_q;
-  const int t0 = min(part * per, all), n = min(per, all - t0);
+  const int all = (k_len + 31) / 32;
+  const int ranges = ranges_of(all, d.target[u.full ? 0 : 1], u.full ? d.q.max_full : d.q.max_part);
+  if (u.part >= ranges) return;
+  const int per = (all + ranges - 1) / ranges, t0 = min(u.part * per, all), n = min(per, all - t0);
 
   Stage<D> sk, sv;
   sk.init(p.k_row, wave, lane);
@@ -1082,9 +1220,11 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
     const bool live = row < q_len;
     const long rc = q_start + min(row, q_len - 1);
     const float f = p.scale * kUnshift;
-    if (d.split_q > 1)
-      store_part<D>(d.part_q + (((long)part * p.total_q + rc) * p.H + h) * D, acc[nb], f, hh, live);
-    else
+    if (ranges > 1) {
+      long step;
+      float* to = part_row<D>(d.q, u.full, p.B, p.total_q, q_start, b, min(row, q_len - 1), h, &step);
+      store_part<D>(to + u.part * step, acc[nb], f, hh, live);
+    } else
       store_row<D>(p.dq + rc * p.dq_row + (long)h * p.dq_head, acc[nb], f, hh, live);
   }
 }
@@ -1092,78 +1232,113 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
 template <int D>
 __global__ __launch_bounds__(kThreads, 1) void attn_bwd_kernel(TrainDev d) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  if ((int)blockIdx.x < d.n_key_blocks)
-    key_block<D>(d, xcd_remap(blockIdx.x, d.n_key_blocks), smem);
-  else
-    query_block<D>(d, xcd_remap(blockIdx.x - d.n_key_blocks, gridDim.x - d.n_key_blocks), smem);
+  // heavy units first: full tiles of keys, parts of keys, then the queries' (their parts end the launch)
+  const int nk = d.k.blocks(d.p.B), kf = d.k.full_blocks(), qf = d.q.full_blocks(), nq = d.q.blocks(d.p.B);
+  int v = blockIdx.x;
+  if (v < nk) {
+    key_block<D>(d, v < kf ? xcd_remap(v, kf) : kf + xcd_remap(v - kf, nk - kf), smem);
+  } else {
+    v -= nk;
+    query_block<D>(d, v < qf ? xcd_remap(v, qf) : qf + xcd_remap(v - qf, nq - qf), smem);
+  }
 }
 
-// Adds the ranges' partial gradients in order. Rows outside all sequences have no partials and are left alone.
+// Adds the ranges' partial gradients in order: one item = 8 columns of a row and head, of all rows (full tiles) or of the
+// 128-row slots of the sequences' parts
+struct JoinItems {
+  int q_full, q_part, k_full, k_part;  // workgroups; 0: that kind has no ranges
+};
 template <int D>
-__global__ __launch_bounds__(kThreads) void attn_join_kernel(const float* part, int n, bf16_t* out, long row_stride,
-                                                             long head_stride, const int* cu, int B, int total, int H) {
+__global__ __launch_bounds__(kThreads) void attn_join_kernel(TrainDev d, JoinItems n) {
+  const AttnTrainParams& p = d.p;
   constexpr int LANES = D / 8;
-  const long item = ((long)blockIdx.x * kThreads + threadIdx.x) / LANES;
-  const int c = threadIdx.x % LANES;
-  if (item >= (long)total * H) return;
-  const int row = (int)(item / H), h = (int)(item % H);
-  bool inside = false;
-  for (int b = 0; b < B && !inside; ++b) {
-    int s, len;
-    seq_range(cu, b, total, &s, &len);
-    inside = row >= s && row < s + len;
+  int blk = blockIdx.x;
+  const bool is_q = blk < n.q_full + n.q_part;
+  blk -= is_q ? 0 : n.q_full + n.q_part;
+  const bool full = blk < (is_q ? n.q_full : n.k_full);
+  blk -= full ? 0 : is_q ? n.q_full : n.k_full;
+  const Cut& c = is_q ? d.q : d.k;
+  const long item = ((long)blk * kThreads + threadIdx.x) / LANES;
+  const int col = threadIdx.x % LANES * 8;
+  const int total = is_q ? p.total_q : p.total_k;
+  const int* own = is_q ? p.cu_q : p.cu_k;
+  const long slot = item / c.heads;
+  const int h = (int)(item % c.heads);
+  int b, start, len, row;
+  if (full) {
+    if (slot >= total) return;
+    b = find_seq(own, p.B, total, (int)slot);
+    if (b < 0) return;
+    seq_range(own, b, total, &start, &len);
+    row = (int)slot - start;
+    if (row >= len - len % WROWS) return;
+  } else {
+    if (slot >= (long)p.B * WROWS) return;
+    b = (int)(slot / WROWS);
+    seq_range(own, b, total, &start, &len);
+    row = len - len % WROWS + (int)(slot % WROWS);
+    if (row >= len) return;
   }
-  if (!inside) return;
-  f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
-  const long step = (long)total * H * D;
-  const float* src = part + item * D + 8 * c;
-  for (int i = 0; i < n; ++i) {
-    a += *(const f32x4*)(src + i * step);
-    b += *(const f32x4*)(src + i * step + 4);
+  int s2, swept;
+  seq_range(is_q ? p.cu_k : p.cu_q, b, is_q ? p.total_k : p.total_q, &s2, &swept);
+  const int most = full ? c.max_full : c.max_part;
+  const int ranges = ranges_of((swept + 31) / 32 * (is_q ? 1 : p.H / p.HK), d.target[full ? 0 : 1], most);
+  if (ranges < 2) return;
+  long step;
+  const float* src = part_row<D>(c, full, p.B, total, start, b, row, h, &step) + col;
+  const long r = (long)start + row;
+  for (int out = 0; out < (is_q ? 1 : 2); ++out, src += most * step) {
+    f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+    for (int i = 0; i < ranges; ++i) {
+      x += *(const f32x4*)(src + i * step);
+      y += *(const f32x4*)(src + i * step + 4);
+    }
+    bf16_t* to = is_q ? p.dq + r * p.dq_row + (long)h * p.dq_head
+                 : out ? p.dv + r * p.dv_row + (long)h * p.dv_head
+                       : p.dk + r * p.dk_row + (long)h * p.dk_head;
+    *(u32x4*)(to + col) = u32x4{pack2bf(x[0], x[1]), pack2bf(x[2], x[3]), pack2bf(y[0], y[1]), pack2bf(y[2], y[3])};
   }
-  const u32x4 w = {pack2bf(a[0], a[1]), pack2bf(a[2], a[3]), pack2bf(b[0], b[1]), pack2bf(b[2], b[3])};
-  *(u32x4*)(out + (long)row * row_stride + (long)h * head_stride + 8 * c) = w;
 }
-
-// zeros (lse: -inf) in the rows outside all sequences
-__global__ __launch_bounds__(kThreads) void attn_zero_kernel(bf16_t* out, long row_stride, long head_stride, const int* cu,
-                                                             int B, int total, int H, int D, float* lse) {
-  const long item = ((long)blockIdx.x * kThreads + threadIdx.x) * 8;
-  if (item >= (long)total * H * D) return;
-  const int row = (int)(item / ((long)H * D)), h = (int)(item / D % H), c = (int)(item % D);
-  for (int b = 0; b < B; ++b) {
-    int s, len;
-    seq_range(cu, b, total, &s, &len);
-    if (row >= s && row < s + len) return;
-  }
-  *(u32x4*)(out + (long)row * row_stride + (long)h * head_stride + c) = u32x4{0u, 0u, 0u, 0u};
-  if (lse != nullptr && c == 0) lse[(long)h * total + row] = -INFINITY;
-}
-
-constexpr int kCus = 256;
 
 struct Plan {
-  int tiles_q, tiles_k, split_q, split_k;
-  long ld_bytes, part_q_bytes, part_k_bytes;  // part_k_bytes: dk and dv each
+  Cut q, k;
+  long head_bytes, lse_bytes, qf_bytes, qp_bytes, kf_bytes, kp_bytes;  // kf, kp: dk and dv
+  long total() const { return head_bytes + lse_bytes + qf_bytes + qp_bytes + kf_bytes + kp_bytes; }
 };
 
-// Ranges per sweep: as many as fill the CUs (a workgroup takes a whole CU), none shorter than two tiles of the average
-// sequence.
+// Room for ranges, from the average lengths (attn_delta_kernel knows the real ones and uses what it needs of it): three
+// times what the average unit would take, none where that is under one, and none shorter than kMinRange stages in a
+// sequence four times the average.
 Plan make_plan(const AttnTrainParams& p) {
   Plan x;
-  x.tiles_q = p.total_q / WROWS + p.B;
-  x.tiles_k = p.total_k / WROWS + p.B;
-  const long nq = (long)(p.total_q / WROWS + 1) * p.H, nk = (long)(p.total_k / WROWS + 1) * p.HK;
-  const long sweep_q = p.total_k / p.B / TR, sweep_k = (long)(p.total_q / p.B / TR) * (p.H / p.HK);
-  auto ranges = [&](long tiles) {
-    return (int)std::max(1L, std::min({(long)kMaxSplit, kCus / (nq + nk), tiles / 2}));
-  };
-  x.split_q = ranges(sweep_q);
-  x.split_k = ranges(sweep_k);
   auto pad = [](long n) { return (n + 255) / 256 * 256; };
-  x.ld_bytes = pad((long)p.H * p.total_q * 8);
-  x.part_q_bytes = x.split_q > 1 ? pad((long)x.split_q * p.total_q * p.H * p.dim * 4) : 0;
-  x.part_k_bytes = x.split_k > 1 ? pad((long)x.split_k * p.total_k * p.HK * p.dim * 4) : 0;
+  const double sweep_q = p.total_k / 32. / p.B, sweep_k = p.total_q / 32. / p.B * (p.H / p.HK);
+  const double units_q = ((double)(p.total_q / WROWS) + p.B) * p.H, units_k = ((double)(p.total_k / WROWS) + p.B) * p.HK;
+  const double share = std::max(1., (units_q * sweep_q + units_k * sweep_k) / kCus);
+  auto cut = [&](int total, int heads, double sweep) {
+    Cut c{};
+    c.full = total / WROWS;
+    c.heads = heads;
+    const double longest = std::min(sweep * 4, sweep * p.B) / kMinRange;
+    auto ranges = [&](double want) { return (int)std::max(1., std::min({(double)kMaxRanges, want, longest})); };
+    c.max_full = ranges(3 * sweep / (share / 2));
+    c.max_part = ranges((double)kCus / ((double)p.B * heads));
+    return c;
+  };
+  x.q = cut(p.total_q, p.H, sweep_q);
+  x.k = cut(p.total_k, p.HK, sweep_k);
+  auto full_bytes = [&](const Cut& c, int total) {
+    return c.max_full > 1 ? pad((long)c.max_full * total * c.heads * p.dim * 4) : 0;
+  };
+  auto part_bytes = [&](const Cut& c) {
+    return c.max_part > 1 ? pad((long)c.max_part * p.B * WROWS * c.heads * p.dim * 4) : 0;
+  };
+  x.head_bytes = 256;
+  x.lse_bytes = pad((long)p.H * p.total_q * 8);
+  x.qf_bytes = full_bytes(x.q, p.total_q);
+  x.qp_bytes = part_bytes(x.q);
+  x.kf_bytes = 2 * full_bytes(x.k, p.total_k);
+  x.kp_bytes = 2 * part_bytes(x.k);
   return x;
 }
 
@@ -1172,8 +1347,8 @@ int check(const AttnTrainParams& p) {
   FLITE_REQUIRE(p.B > 0 && p.H > 0 && p.HK > 0 && p.H % p.HK == 0,
                 "attention: batch, heads and kv heads must be positive, heads a multiple of kv heads");
   FLITE_REQUIRE(p.total_q >= 0 && p.total_k >= 0, "attention: rows must not be negative");
-  FLITE_REQUIRE(((long)p.total_q / WROWS + p.B) * p.H < (1L << 30) / kMaxSplit &&
-                    ((long)p.total_k / WROWS + p.B) * p.HK < (1L << 30) / kMaxSplit,
+  FLITE_REQUIRE(((long)p.total_q / WROWS + p.B) * p.H < (1L << 29) / kMaxRanges &&
+                    ((long)p.total_k / WROWS + p.B) * p.HK < (1L << 29) / kMaxRanges,
                 "attention: too many rows, sequences or heads");
   FLITE_REQUIRE(p.cu_q && p.cu_k, "attention: cu_seqlens missing");
   return 0;
@@ -1198,12 +1373,15 @@ int lds_limit(F* f, int bytes, std::atomic<unsigned long long>& done) {
   return 0;
 }
 
+constexpr int kZeroBlocks = 32;
+
 template <int D>
 int launch_fwd(const TrainDev& d, hipStream_t s) {
   constexpr int lds = 4 * TR * D * 2;
   static std::atomic<unsigned long long> done{0};
   if (lds_limit(attn_lse_kernel<D>, lds, done)) return 1;
-  hipLaunchKernelGGL(attn_lse_kernel<D>, dim3(d.tiles_q * d.p.H), dim3(kThreads), lds, s, d);
+  hipLaunchKernelGGL(attn_lse_kernel<D>, dim3(d.tiles_q * d.p.H + (d.p.zero_outside ? kZeroBlocks : 0)), dim3(kThreads), lds,
+                     s, d);
   FLITE_HIP_CHECK(hipGetLastError());
   return 0;
 }
@@ -1214,38 +1392,28 @@ int launch_bwd(const TrainDev& d, hipStream_t s) {
   constexpr int lds = Lds<D>::TOTAL;
   static std::atomic<unsigned long long> done{0};
   if (lds_limit(attn_bwd_kernel<D>, lds, done)) return 1;
-  auto blocks = [](long rows_heads) { return dim3((unsigned)((rows_heads * (D / 8) + kThreads - 1) / kThreads)); };
-  if (p.total_q > 0)
-    hipLaunchKernelGGL(attn_delta_kernel<D>, blocks((long)p.total_q * p.H), dim3(kThreads), 0, s, d);
-  const int n = d.n_key_blocks + (p.total_q > 0 ? d.tiles_q * p.H * d.split_q : 0);
-  if (n > 0) hipLaunchKernelGGL(attn_bwd_kernel<D>, dim3(n), dim3(kThreads), lds, s, d);
-  if (d.split_q > 1 && p.total_q > 0)
-    hipLaunchKernelGGL(attn_join_kernel<D>, blocks((long)p.total_q * p.H), dim3(kThreads), 0, s, d.part_q, d.split_q,
-                       p.dq, p.dq_row, p.dq_head, p.cu_q, p.B, p.total_q, p.H);
-  if (d.split_k > 1 && p.total_k > 0) {
-    hipLaunchKernelGGL(attn_join_kernel<D>, blocks((long)p.total_k * p.HK), dim3(kThreads), 0, s, d.part_k, d.split_k,
-                       p.dk, p.dk_row, p.dk_head, p.cu_k, p.B, p.total_k, p.HK);
-    hipLaunchKernelGGL(attn_join_kernel<D>, blocks((long)p.total_k * p.HK), dim3(kThreads), 0, s, d.part_v, d.split_k,
-                       p.dv, p.dv_row, p.dv_head, p.cu_k, p.B, p.total_k, p.HK);
-  }
+  auto blocks = [](long rows_heads) { return (int)((rows_heads * (D / 8) + kThreads - 1) / kThreads); };
+  const int q_rows = blocks((long)p.total_q * p.H);
+  hipLaunchKernelGGL(attn_delta_kernel<D>, dim3(q_rows + (p.zero_outside ? kZeroBlocks : 1)), dim3(kThreads), 0, s, d, q_rows);
+  FLITE_HIP_CHECK(hipGetLastError());
+  hipLaunchKernelGGL(attn_bwd_kernel<D>, dim3(d.k.blocks(p.B) + d.q.blocks(p.B)), dim3(kThreads), lds, s, d);
+  FLITE_HIP_CHECK(hipGetLastError());
+  JoinItems j;
+  j.q_full = d.q.max_full > 1 ? q_rows : 0;
+  j.q_part = d.q.max_part > 1 ? blocks((long)p.B * WROWS * p.H) : 0;
+  j.k_full = d.k.max_full > 1 ? blocks((long)p.total_k * p.HK) : 0;
+  j.k_part = d.k.max_part > 1 ? blocks((long)p.B * WROWS * p.HK) : 0;
+  const int join = j.q_full + j.q_part + j.k_full + j.k_part;
+  if (join > 0) hipLaunchKernelGGL(attn_join_kernel<D>, dim3(join), dim3(kThreads), 0, s, d, j);
   FLITE_HIP_CHECK(hipGetLastError());
   return 0;
-}
-
-void zero_outside(bf16_t* out, long row, long head, const int* cu, int B, int total, int H, int D, float* lse,
-                  hipStream_t s) {
-  if (total <= 0) return;
-  const long n = (long)total * H * D / 8;
-  hipLaunchKernelGGL(attn_zero_kernel, dim3((unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, s, out, row,
-                     head, cu, B, total, H, D, lse);
 }
 
 }  // namespace
 
 long attn_train_workspace_bytes(const AttnTrainParams& p) {
   if (check(p)) return -1;
-  const Plan x = make_plan(p);
-  return x.ld_bytes + x.part_q_bytes + 2 * x.part_k_bytes;
+  return make_plan(p).total();
 }
 
 int attn_train_fwd(const AttnTrainParams& p, hipStream_t s) {
@@ -1259,8 +1427,7 @@ int attn_train_fwd(const AttnTrainParams& p, hipStream_t s) {
   if (!any_q) return 0;
   TrainDev d{};
   d.p = p;
-  d.tiles_q = make_plan(p).tiles_q;
-  if (p.zero_outside) zero_outside(p.o, p.o_row, p.o_head, p.cu_q, p.B, p.total_q, p.H, p.dim, p.lse, s);
+  d.tiles_q = p.total_q / WROWS + p.B;
   if (p.dim == 64) return launch_fwd<64>(d, s);
   if (p.dim == 128) return launch_fwd<128>(d, s);
   return launch_fwd<256>(d, s);
@@ -1279,26 +1446,25 @@ int attn_train_bwd(const AttnTrainParams& p, void* ws, long ws_bytes, hipStream_
   if (int rc = check_rows(p.dv, p.dv_row, p.dv_head, p.dim, any_k, "dv")) return rc;
   FLITE_REQUIRE(p.lse || !any_q, "attention: missing lse");
   const Plan x = make_plan(p);
-  FLITE_REQUIRE((ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= x.ld_bytes + x.part_q_bytes + 2 * x.part_k_bytes) ||
-                    x.ld_bytes + x.part_q_bytes + 2 * x.part_k_bytes == 0,
+  FLITE_REQUIRE(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= x.total(),
                 "attention backward: workspace missing, not 256-byte aligned, or too small");
   TrainDev d{};
   d.p = p;
-  d.tiles_q = x.tiles_q;
-  d.tiles_k = x.tiles_k;
-  d.split_q = x.split_q;
-  d.split_k = x.split_k;
-  d.n_key_blocks = any_k ? x.tiles_k * p.HK * x.split_k : 0;
-  d.lse2 = (float*)ws;
+  d.q = x.q;
+  d.k = x.k;
+  char* at = (char*)ws;
+  auto take = [&](long n) {
+    char* r = at;
+    at += n;
+    return r;
+  };
+  d.target = (int*)take(x.head_bytes);
+  d.lse2 = (float*)take(x.lse_bytes);
   d.delta = d.lse2 + (long)p.H * p.total_q;
-  d.part_q = (float*)((char*)ws + x.ld_bytes);
-  d.part_k = (float*)((char*)ws + x.ld_bytes + x.part_q_bytes);
-  d.part_v = (float*)((char*)ws + x.ld_bytes + x.part_q_bytes + x.part_k_bytes);
-  if (p.zero_outside) {
-    zero_outside(p.dq, p.dq_row, p.dq_head, p.cu_q, p.B, p.total_q, p.H, p.dim, nullptr, s);
-    zero_outside(p.dk, p.dk_row, p.dk_head, p.cu_k, p.B, p.total_k, p.HK, p.dim, nullptr, s);
-    zero_outside(p.dv, p.dv_row, p.dv_head, p.cu_k, p.B, p.total_k, p.HK, p.dim, nullptr, s);
-  }
+  d.q.ws_full = (float*)take(x.qf_bytes);
+  d.q.ws_part = (float*)take(x.qp_bytes);
+  d.k.ws_full = (float*)take(x.kf_bytes);
+  d.k.ws_part = (float*)take(x.kp_bytes);
   if (p.dim == 64) return launch_bwd<64>(d, s);
   if (p.dim == 128) return launch_bwd<128>(d, s);
   return launch_bwd<256>(d, s);
