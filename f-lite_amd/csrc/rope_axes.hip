@@ -185,15 +185,19 @@ Kernel pick(bool norm, bool bwd) {
 int rope_axes(const RopeAxesParams& p, const int* axis_pairs, const double* bases, bool x_bf16, bool interleaved,
               bool norm, bool bwd, hipStream_t s) {
   FLITE_REQUIRE(p.dim > 0 && p.dim % 16 == 0 && p.dim <= 256, "rope_axes: head size must be a multiple of 16, at most 256");
-  FLITE_REQUIRE(p.axes >= 1 && p.axes <= 8 && axis_pairs && bases, "rope_axes: 1 to 8 axes");
+  FLITE_REQUIRE(p.axes >= 1 && p.axes <= 8, "rope_axes: 1 to 8 axes");
   RopeAxesDev d;
   d.p = p;
   int n = 0;
   for (int a = 0; a < p.axes; ++a) {
     FLITE_REQUIRE(axis_pairs[a] >= 0 && axis_pairs[a] <= p.dim / 2 - n, "rope_axes: more pairs than the head holds");
     FLITE_REQUIRE(bases[a] > 0.0 && std::isfinite(bases[a]), "rope_axes: bases must be positive");
+    // base^(-i / n) as a product of two powers, 3 ulp: a pow per pair would cost more host time than the launch
+    double low[8], high = 0.;
+    for (int i = 0; i < std::min(axis_pairs[a], 8); ++i) low[i] = pow(bases[a], -(double)i / axis_pairs[a]);
     for (int i = 0; i < axis_pairs[a]; ++i, ++n) {
-      d.turns[n] = pow(bases[a], -(double)i / axis_pairs[a]) * 0.15915494309189533577;  // 1 / (2 pi)
+      if (i % 8 == 0) high = pow(bases[a], -(double)i / axis_pairs[a]) * 0.15915494309189533577;  // 1 / (2 pi)
+      d.turns[n] = high * low[i % 8];
       d.axis[n] = (unsigned char)a;
     }
   }

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -68,7 +69,7 @@ class RopeAxesArgs(ctypes.Structure):
 
     _fields_ = (
         [(n, _vp) for n in ("x", "out", "y", "rstd", "positions")]
-        + [("axis_pairs", ctypes.POINTER(_i)), ("bases", ctypes.POINTER(_d))]
+        + [("bases", _d * 8), ("axis_pairs", _i * 8)]
         + [(n, _l) for n in ("x_row", "x_head", "out_row", "out_head", "y_row", "y_head", "rows", "tokens")]
         + [(n, _i) for n in ("axes", "heads", "rope_heads", "head_dim", "is_bf16", "positions_f32", "interleaved",
                              "norm")]
@@ -87,6 +88,13 @@ class NormArgs(ctypes.Structure):
     )
 
 
+# The three structures as native struct formats: packing one costs a microsecond, filling its ctypes fields ten
+_ATTN_TRAIN = struct.Struct("@9P16l2P6ifi")
+_ROPE_AXES = struct.Struct("@5P8d8i8l8if4x")
+_NORM = struct.Struct("@12P7l3if")
+assert (_ATTN_TRAIN.size, _ROPE_AXES.size, _NORM.size) == tuple(
+    ctypes.sizeof(c) for c in (AttnTrain, RopeAxesArgs, NormArgs))
+
 # name -> (restype, argtypes); every symbol declared in include/flite.h
 SIGNATURES = {
     "flite_last_error": (_cp, []),
@@ -102,14 +110,14 @@ SIGNATURES = {
                                       _f, _vp, _l]),
     "flite_rmsnorm_modulate": (_i, [_vp, _vp, _i, _l, _vp, _l, _vp, _vp, _vp, _l, _l, _l, _i, _f]),
     "flite_rope_qknorm": (_i, [_vp, _vp, _l, _l, _i, _i, _vp, _vp, _l, _f]),
-    "flite_attn_lse_fwd": (_i, [_vp, ctypes.POINTER(AttnTrain)]),
-    "flite_attn_lse_bwd_workspace_bytes": (_l, [ctypes.POINTER(AttnTrain)]),
-    "flite_attn_lse_bwd": (_i, [_vp, ctypes.POINTER(AttnTrain), _vp, _l]),
-    "flite_rope_axes_fwd": (_i, [_vp, ctypes.POINTER(RopeAxesArgs)]),
-    "flite_rope_axes_bwd": (_i, [_vp, ctypes.POINTER(RopeAxesArgs)]),
-    "flite_layernorm_modulate": (_i, [_vp, ctypes.POINTER(NormArgs)]),
+    "flite_attn_lse_fwd": (_i, [_vp, _vp]),
+    "flite_attn_lse_bwd_workspace_bytes": (_l, [_vp]),
+    "flite_attn_lse_bwd": (_i, [_vp, _vp, _vp, _l]),
+    "flite_rope_axes_fwd": (_i, [_vp, _vp]),
+    "flite_rope_axes_bwd": (_i, [_vp, _vp]),
+    "flite_layernorm_modulate": (_i, [_vp, _vp]),
     "flite_norm_bwd_workspace_bytes": (_l, [_l, _l, _i]),
-    "flite_norm_modulate_bwd": (_i, [_vp, ctypes.POINTER(NormArgs), _vp, _l]),
+    "flite_norm_modulate_bwd": (_i, [_vp, _vp, _vp, _l]),
     "flite_gather_rows": (_i, [_vp, _vp, _vp, _vp, _l, _i]),
     "flite_t5_attention": (_i, [_vp, _vp, _l, _vp, _l, _vp, _l, _vp, _l, _vp, _vp, _vp, _i, _i, _i]),
     "flite_embed_rows_f32": (_i, [_vp, _vp, _vp, _vp, _l, _i, _l]),
@@ -496,79 +504,86 @@ def apg_euler_dev_(acc, uncond, cond, guidance, threshold, n_total, ws, dt):
 # training operators (include/flite.h): the backward pass of attention, rotary positions and norms, and the forward
 # passes that go with it. Plain functions of tensors: nothing is recorded for autograd.
 # ------------------------------------------------------------------------------------------------
-def _one_device(**tensors):
-    """Every given tensor on one ROCm device, which is returned."""
+def _one_device(names, *tensors):
+    """The ROCm device number of every given tensor (None: not given); refuses CPU tensors and a mix."""
     dev = None
-    for name, t in tensors.items():
+    for i, t in enumerate(tensors):
         if t is None:
             continue
-        require_gpu(t, name, contiguous=False)
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise FliteError(f"{name}: on {t.device}, the other tensors are on {dev}")
+        d = t.get_device() if isinstance(t, torch.Tensor) else -1
+        if d != dev:
+            name = names.split()[i]
+            if d < 0:
+                require_gpu(t, name)
+            if dev is not None:
+                raise FliteError(f"{name}: on cuda:{d}, the tensors before it are on cuda:{dev}")
+            dev = d
     return dev
+
+
+def _call(dev, name, *args):
+    """Calls a C entry point on the current stream of device `dev`, with that device current."""
+    fn = getattr(_lib or load(), name)
+    if torch.cuda.current_device() == dev:
+        status = fn(torch._C._cuda_getCurrentRawStream(dev), *args)
+    else:
+        with torch.cuda.device(dev):
+            status = fn(torch._C._cuda_getCurrentRawStream(dev), *args)
+    if status:
+        check(status, name)
 
 
 def _own_storage(name, t):
     """Refuses an output whose elements share memory (an expanded tensor)."""
-    if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+    if 0 in t.stride() and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
         raise FliteError(f"{name}: an output must not be an expanded tensor")
 
 
-def _heads_like(name, t, dtype, shape=None):
-    """A [rows, heads, head_dim] tensor with contiguous elements and 16-byte aligned rows and heads."""
-    if t.dim() != 3 or (shape is not None and tuple(t.shape) != tuple(shape)):
+def _heads(name, t, dtype, shape=None):
+    """(address, row stride, head stride) of a [rows, heads, head_dim] tensor with contiguous elements and 16-byte aligned
+    rows and heads. The stride of a dimension of size 1 says nothing: head_dim stands for it."""
+    s = t.shape
+    if len(s) != 3 or (shape is not None and s != shape):
         raise FliteError(f"{name}: expected {'[rows, heads, head_dim]' if shape is None else tuple(shape)}, got "
-                         f"{tuple(t.shape)}")
+                         f"{tuple(s)}")
     if t.dtype != dtype:
         raise FliteError(f"{name}: expected {dtype}, got {t.dtype}")
-    if t.numel() and (t.stride(2) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[2])
-                      or (t.shape[0] > 1 and t.stride(0) % 8) or (t.shape[1] > 1 and t.stride(1) % 8)
-                      or t.data_ptr() % 16):
+    n, h, d = s
+    row, head, one = t.stride()
+    ptr = t.data_ptr()
+    if not (n and h and d):
+        return ptr, d, d
+    if n == 1:
+        row = d
+    if h == 1:
+        head = d
+    if (one != 1 and d > 1) or row < d or row & 7 or head & 7 or ptr & 15:
         raise FliteError(f"{name}: elements must be contiguous, rows not expanded, strides multiples of 8 and the data "
-                         f"16-byte aligned (strides {tuple(t.stride())})")
+                         f"16-byte aligned (strides {t.stride()})")
+    return ptr, row, head
 
 
-def _strides(t):
-    """(row, head) strides of a [rows, heads, head_dim] tensor; those of dimensions of size 1 say nothing."""
-    n, h, d = t.shape
-    head = t.stride(1) if h > 1 and n else d
-    return (t.stride(0) if n > 1 else d), head
-
-
-def _attn_train_args(q, k, v, cu_q, cu_k, scale):
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _heads_like(name, t, torch.bfloat16)
-    if v.shape != k.shape or q.shape[2] != k.shape[2]:
+def _attn_sizes(q, k, v, cu_q, cu_k):
+    """(batch, heads, kv_heads, head_dim, total_q, total_k) after the checks that forward and backward share."""
+    n, h, d = q.shape if q.dim() == 3 else (0, 0, 0)
+    nk, hk = k.shape[:2] if k.dim() == 3 else (0, 0)
+    if k.shape != v.shape or k.dim() != 3 or k.shape[2] != d:
         raise FliteError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
-    if q.shape[2] not in (64, 128, 256):
-        raise FliteError(f"attention: head size must be 64, 128 or 256, got {q.shape[2]}")
-    if k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
-        raise FliteError(f"attention: {q.shape[1]} query heads are no multiple of {k.shape[1]} key heads")
+    if d not in (64, 128, 256):
+        raise FliteError(f"attention: head size must be 64, 128 or 256, got {d}")
+    if hk == 0 or h == 0 or h % hk:
+        raise FliteError(f"attention: {h} query heads are no multiple of {hk} key heads")
+    b = cu_q.shape[0] if cu_q.dim() == 1 else 0
     for name, t in (("cu_q", cu_q), ("cu_k", cu_k)):
-        require_gpu(t, name, torch.int32)
-        if t.dim() != 1 or t.numel() < 2 or t.numel() != cu_q.numel():
-            raise FliteError(f"{name}: expected [batch + 1] int32, batch >= 1, as long as the other")
-    a = AttnTrain()
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        setattr(a, name, t.data_ptr())
-        row, head = _strides(t)
-        setattr(a, f"{name}_row", row)
-        setattr(a, f"{name}_head", head)
-    a.cu_q, a.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
-    a.batch = cu_q.numel() - 1
-    a.total_q, a.heads, a.head_dim = q.shape
-    a.total_k, a.kv_heads = k.shape[:2]
-    a.scale = float(scale)
-    return a
+        if t.dtype != torch.int32 or t.shape != (b,) or b < 2 or (t.stride(0) != 1):
+            raise FliteError(f"{name}: expected contiguous int32 [batch + 1], batch >= 1, as long as the other")
+    return b - 1, h, hk, d, n, nk
 
 
-def _set_heads(a, name, t):
-    setattr(a, name, t.data_ptr())
-    row, head = _strides(t)
-    setattr(a, f"{name}_row", row)
-    setattr(a, f"{name}_head", head)
+def _lse_ptr(lse, h, n):
+    if lse.dtype != torch.float32 or lse.shape != (h, n) or not lse.is_contiguous():
+        raise FliteError(f"lse: expected contiguous fp32 {(h, n)}, got {lse.dtype} {tuple(lse.shape)}")
+    return lse.data_ptr()
 
 
 def attn_varlen_lse(q, k, v, cu_q, cu_k, scale, out=None, lse=None):
@@ -578,23 +593,23 @@ def attn_varlen_lse(q, k, v, cu_q, cu_k, scale, out=None, lse=None):
     head i // (h / h_kv)), any row and head strides. Sequence b is rows cu_q[b]:cu_q[b+1] of q and cu_k[b]:cu_k[b+1] of
     k and v; either may be empty (no keys: out 0, lse -inf). Rows outside all sequences: 0 and -inf, or left as they
     were in an `out` and `lse` that the caller gives (both or neither)."""
-    dev = _one_device(q=q, k=k, v=v, cu_q=cu_q, cu_k=cu_k, out=out, lse=lse)
-    a = _attn_train_args(q, k, v, cu_q, cu_k, scale)
+    dev = _one_device("q k v cu_q cu_k out lse", q, k, v, cu_q, cu_k, out, lse)
+    b, h, hk, d, n, nk = _attn_sizes(q, k, v, cu_q, cu_k)
+    pq, q0, q1 = _heads("q", q, torch.bfloat16)
+    pk, k0, k1 = _heads("k", k, torch.bfloat16)
+    pv, v0, v1 = _heads("v", v, torch.bfloat16)
     if (out is None) != (lse is None):
         raise FliteError("attention: give both out and lse, or neither")
-    with torch.cuda.device(dev):
-        if out is None:
-            out = torch.empty(q.shape, device=dev, dtype=torch.bfloat16)
-            lse = torch.empty(q.shape[1], q.shape[0], device=dev, dtype=torch.float32)
-            a.zero_outside = 1
-        _heads_like("out", out, torch.bfloat16, q.shape)
+    new = out is None
+    if new:
+        out = torch.empty(q.shape, device=q.device, dtype=torch.bfloat16)
+        lse = torch.empty((h, n), device=q.device, dtype=torch.float32)
+    else:
         _own_storage("out", out)
-        require_gpu(lse, "lse", torch.float32)
-        if tuple(lse.shape) != (q.shape[1], q.shape[0]):
-            raise FliteError(f"lse: expected {(q.shape[1], q.shape[0])}, got {tuple(lse.shape)}")
-        _set_heads(a, "out", out)
-        a.lse = lse.data_ptr()
-        check(load().flite_attn_lse_fwd(stream_ptr(dev), ctypes.byref(a)), "flite_attn_lse_fwd")
+    po, o0, o1 = _heads("out", out, torch.bfloat16, q.shape)
+    args = _ATTN_TRAIN.pack(pq, pk, pv, po, _lse_ptr(lse, h, n), 0, 0, 0, 0, q0, q1, k0, k1, v0, v1, o0, o1, 0, 0, 0, 0,
+                            0, 0, 0, 0, cu_q.data_ptr(), cu_k.data_ptr(), b, h, hk, d, n, nk, scale, new)
+    _call(dev, "flite_attn_lse_fwd", args)
     return out, lse
 
 
@@ -603,66 +618,75 @@ def attn_varlen_bwd(dout, q, k, v, out, lse, cu_q, cu_k, scale, dq=None, dk=None
     dk and dv are the sums over the query heads that share a key head. The probabilities are made again from q, k and
     lse. Gradient rows outside all sequences: 0, or left as they were in a dq / dk / dv that the caller gives (all
     three or none). The result does not depend on timing: no atomics."""
-    dev = _one_device(dout=dout, q=q, k=k, v=v, out=out, lse=lse, cu_q=cu_q, cu_k=cu_k, dq=dq, dk=dk, dv=dv)
-    a = _attn_train_args(q, k, v, cu_q, cu_k, scale)
-    _heads_like("dout", dout, torch.bfloat16, q.shape)
-    _heads_like("out", out, torch.bfloat16, q.shape)
-    require_gpu(lse, "lse", torch.float32)
-    if tuple(lse.shape) != (q.shape[1], q.shape[0]):
-        raise FliteError(f"lse: expected {(q.shape[1], q.shape[0])}, got {tuple(lse.shape)}")
-    given = [t is not None for t in (dq, dk, dv)]
-    if any(given) and not all(given):
+    dev = _one_device("dout q k v out lse cu_q cu_k dq dk dv", dout, q, k, v, out, lse, cu_q, cu_k, dq, dk, dv)
+    b, h, hk, d, n, nk = _attn_sizes(q, k, v, cu_q, cu_k)
+    bf16 = torch.bfloat16
+    pq, q0, q1 = _heads("q", q, bf16)
+    pk, k0, k1 = _heads("k", k, bf16)
+    pv, v0, v1 = _heads("v", v, bf16)
+    pg, g0, g1 = _heads("dout", dout, bf16, q.shape)
+    po, o0, o1 = _heads("out", out, bf16, q.shape)
+    new = dq is None
+    if (dk is None) != new or (dv is None) != new:
         raise FliteError("attention: give all of dq, dk and dv, or none")
-    with torch.cuda.device(dev):
-        if not any(given):
-            dq, dk, dv = (torch.empty(t.shape, device=dev, dtype=torch.bfloat16) for t in (q, k, v))
-            a.zero_outside = 1
-        for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-            _heads_like(name, t, torch.bfloat16, like.shape)
+    if new:
+        dq = torch.empty(q.shape, device=q.device, dtype=bf16)
+        dk = torch.empty(k.shape, device=q.device, dtype=bf16)
+        dv = torch.empty(k.shape, device=q.device, dtype=bf16)
+    else:
+        for name, t in (("dq", dq), ("dk", dk), ("dv", dv)):
             _own_storage(name, t)
-            _set_heads(a, name, t)
-        _set_heads(a, "dout", dout)
-        _set_heads(a, "out", out)
-        a.lse = lse.data_ptr()
-        n = int(load().flite_attn_lse_bwd_workspace_bytes(ctypes.byref(a)))
-        if n < 0:
-            check(2, "flite_attn_lse_bwd_workspace_bytes")
-        ws = torch.empty(n, device=dev, dtype=torch.uint8)
-        check(load().flite_attn_lse_bwd(stream_ptr(dev), ctypes.byref(a), ws.data_ptr(), n), "flite_attn_lse_bwd")
+    a, a0, a1 = _heads("dq", dq, bf16, q.shape)
+    c, c0, c1 = _heads("dk", dk, bf16, k.shape)
+    e, e0, e1 = _heads("dv", dv, bf16, k.shape)
+    args = _ATTN_TRAIN.pack(pq, pk, pv, po, _lse_ptr(lse, h, n), pg, a, c, e, q0, q1, k0, k1, v0, v1, o0, o1, g0, g1, a0,
+                            a1, c0, c1, e0, e1, cu_q.data_ptr(), cu_k.data_ptr(), b, h, hk, d, n, nk, scale, new)
+    size = (_lib or load()).flite_attn_lse_bwd_workspace_bytes(args)
+    if size < 0:
+        check(2, "flite_attn_lse_bwd_workspace_bytes")
+    ws = torch.empty(size, device=q.device, dtype=torch.uint8)
+    _call(dev, "flite_attn_lse_bwd", args, ws.data_ptr(), size)
     return dq, dk, dv
 
 
-def _rope_axes_args(x, positions, axis_pairs, base, interleaved, rope_heads, out):
-    if x.dim() != 3 or x.dtype not in (torch.bfloat16, torch.float32):
-        raise FliteError(f"rope_axes: x must be bf16 or fp32 [rows, heads, head_dim], got {x.dtype} {tuple(x.shape)}")
-    _heads_like("x", x, x.dtype)
-    require_gpu(positions, "positions")
-    if positions.dtype not in (torch.int32, torch.float32) or positions.dim() != 2:
-        raise FliteError("rope_axes: positions must be int32 or fp32 [tokens, axes]")
-    axis_pairs = [int(n) for n in axis_pairs]
+def _rope_axes(entry, x, positions, axis_pairs, base, interleaved, rope_heads, out, y, rstd, norm, eps):
+    dev = _one_device("x positions out y rstd", x, positions, out, y, rstd)
+    dt = x.dtype
+    if dt not in (torch.bfloat16, torch.float32):
+        raise FliteError(f"rope_axes: expected bf16 or fp32 heads, got {dt}")
+    px, x0, x1 = _heads("x", x, dt)
     rows, heads, dim = x.shape
-    tokens = positions.shape[0]
-    if positions.shape[1] != len(axis_pairs):
-        raise FliteError(f"rope_axes: {positions.shape[1]} columns of positions for {len(axis_pairs)} axes")
+    n = len(axis_pairs)
+    if positions.dtype not in (torch.int32, torch.float32) or positions.dim() != 2 or not positions.is_contiguous():
+        raise FliteError("rope_axes: positions must be contiguous int32 or fp32 [tokens, axes]")
+    tokens, axes = positions.shape
+    if axes != n or not 1 <= n <= 8:
+        raise FliteError(f"rope_axes: {axes} columns of positions for {n} axes (1 to 8)")
     if rows and (tokens == 0 or rows % tokens):
         raise FliteError(f"rope_axes: {rows} rows are no multiple of {tokens} tokens")
-    bases = [float(b) for b in base] if isinstance(base, (tuple, list)) else [float(base)] * len(axis_pairs)
-    if len(bases) != len(axis_pairs):
-        raise FliteError(f"rope_axes: {len(bases)} bases for {len(axis_pairs)} axes")
-    _heads_like("out", out, x.dtype, x.shape)
-    _own_storage("out", out)
-    a = RopeAxesArgs()
-    n = len(axis_pairs)
-    a.axis_pairs, a.bases = (_i * n)(*axis_pairs), (_d * n)(*bases)
-    _set_heads(a, "x", x)
-    _set_heads(a, "out", out)
-    a.positions = positions.data_ptr()
-    a.positions_f32 = int(positions.dtype == torch.float32)
-    a.rows, a.tokens, a.axes = rows, max(tokens, 1), n
-    a.heads, a.head_dim = heads, dim
-    a.rope_heads = heads if rope_heads is None else int(rope_heads)
-    a.is_bf16, a.interleaved = int(x.dtype == torch.bfloat16), int(bool(interleaved))
-    return a
+    bases = tuple(base) if isinstance(base, (tuple, list)) else (base,) * n
+    if len(bases) != n:
+        raise FliteError(f"rope_axes: {len(bases)} bases for {n} axes")
+    if out is None:
+        out = torch.empty(x.shape, device=x.device, dtype=dt)
+    elif out is not x:
+        _own_storage("out", out)
+    po, o0, o1 = _heads("out", out, dt, x.shape)
+    py = y0 = y1 = pr = 0
+    if norm:
+        if y is not None:
+            py, y0, y1 = _heads("y", y, dt, x.shape)
+        if rstd is None:
+            rstd = torch.empty((rows, heads), device=x.device, dtype=torch.float32)
+        elif rstd.dtype != torch.float32 or rstd.shape != (rows, heads) or not rstd.is_contiguous():
+            raise FliteError(f"rstd: expected contiguous fp32 {(rows, heads)}, got {rstd.dtype} {tuple(rstd.shape)}")
+        pr = rstd.data_ptr()
+    fill = (0,) * (8 - n)
+    args = _ROPE_AXES.pack(px, po, py, pr, positions.data_ptr(), *bases, *fill, *axis_pairs, *fill, x0, x1, o0, o1, y0,
+                           y1, rows, tokens or 1, n, heads, heads if rope_heads is None else rope_heads, dim,
+                           dt == torch.bfloat16, positions.dtype == torch.float32, bool(interleaved), bool(norm), eps)
+    _call(dev, entry, args)
+    return out, rstd
 
 
 def rope_axes(x, positions, axis_pairs, base=10000.0, interleaved=False, norm=False, eps=1e-6, rope_heads=None,
@@ -675,81 +699,71 @@ def rope_axes(x, positions, axis_pairs, base=10000.0, interleaved=False, norm=Fa
     turns by position * base^(-i / n) (`base`: one number, or one per axis) in the sense of the model's 2-D RoPE; the
     pairs of all axes follow one another, as elements (j, j + pairs) or, interleaved, (2 j, 2 j + 1), and elements past
     them stay. Heads from rope_heads on are normed only. out=x works in place; rstd is [rows, heads] fp32."""
-    dev = _one_device(x=x, positions=positions, out=out)
-    with torch.cuda.device(dev):
-        out = torch.empty(x.shape, device=dev, dtype=x.dtype) if out is None else out
-        a = _rope_axes_args(x, positions, axis_pairs, base, interleaved, rope_heads, out)
-        rstd = torch.empty(x.shape[:2], device=dev, dtype=torch.float32) if norm else None
-        a.norm, a.eps, a.rstd = int(bool(norm)), float(eps), _ptr(rstd)
-        check(load().flite_rope_axes_fwd(stream_ptr(dev), ctypes.byref(a)), "flite_rope_axes_fwd")
-    return out, rstd
+    return _rope_axes("flite_rope_axes_fwd", x, positions, axis_pairs, base, interleaved, rope_heads, out, None, None,
+                      norm, eps)
 
 
 def rope_axes_bwd(dy, positions, axis_pairs, base=10000.0, interleaved=False, y=None, rstd=None, rope_heads=None,
                   out=None):
     """The gradient of rope_axes' x from the gradient `dy` of its output. After norm=True, `y` and `rstd` are what
     rope_axes returned; without the norm both are None. out=dy works in place."""
-    dev = _one_device(dy=dy, positions=positions, y=y, rstd=rstd, out=out)
     if (y is None) != (rstd is None):
         raise FliteError("rope_axes_bwd: give both y and rstd (norm), or neither")
-    with torch.cuda.device(dev):
-        out = torch.empty(dy.shape, device=dev, dtype=dy.dtype) if out is None else out
-        a = _rope_axes_args(dy, positions, axis_pairs, base, interleaved, rope_heads, out)
-        if y is not None:
-            _heads_like("y", y, dy.dtype, dy.shape)
-            require_gpu(rstd, "rstd", torch.float32)
-            if tuple(rstd.shape) != tuple(dy.shape[:2]):
-                raise FliteError(f"rstd: expected {tuple(dy.shape[:2])}, got {tuple(rstd.shape)}")
-            _set_heads(a, "y", y)
-            a.norm, a.rstd = 1, rstd.data_ptr()
-        check(load().flite_rope_axes_bwd(stream_ptr(dev), ctypes.byref(a)), "flite_rope_axes_bwd")
-    return out
+    return _rope_axes("flite_rope_axes_bwd", dy, positions, axis_pairs, base, interleaved, rope_heads, out, y, rstd,
+                      y is not None, 0.0)[0]
+
+
+_NORM_X = (torch.bfloat16, torch.float32)
 
 
 def _norm_rows(name, t, dtypes, shape=None):
-    if t.dim() != 2 or t.dtype not in dtypes or (shape is not None and tuple(t.shape) != tuple(shape)):
+    """(address, row stride) of a [rows, dim] tensor with contiguous, 16-byte aligned rows."""
+    s = t.shape
+    if len(s) != 2 or t.dtype not in dtypes or (shape is not None and s != shape):
         raise FliteError(f"{name}: expected {' or '.join(str(d) for d in dtypes)} "
-                         f"{'[rows, dim]' if shape is None else tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    if t.numel() and (t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1]))
-                      or t.data_ptr() % 16):
-        raise FliteError(f"{name}: rows must be contiguous, not expanded and 16-byte aligned, their stride a multiple of "
-                         f"8 (strides {tuple(t.stride())})")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+                         f"{'[rows, dim]' if shape is None else tuple(shape)}, got {t.dtype} {tuple(s)}")
+    row, one = t.stride()
+    ptr = t.data_ptr()
+    if s[0] < 2:
+        row = s[1]
+    if one != 1 or row < s[1] or row & 7 or ptr & 15:
+        if t.numel():
+            raise FliteError(f"{name}: rows must be contiguous, not expanded and 16-byte aligned, their stride a multiple "
+                             f"of 8 (strides {t.stride()})")
+    return ptr, row
 
 
-def _norm_args(x, w, b, mods, seg_rows, eps):
-    """NormArgs of x, w, b and the modulation rows `mods` (name -> fp32 [dim] or [segments, dim]), and the segments."""
-    a = NormArgs()
-    a.ldx = _norm_rows("x", x, (torch.bfloat16, torch.float32))
+def _norm_vec(name, t, dim):
+    if t is None:
+        return 0
+    ptr = t.data_ptr()
+    if t.dtype != torch.bfloat16 or t.shape != (dim,) or t.stride(0) != 1 or ptr & 15:
+        raise FliteError(f"{name}: expected contiguous, 16-byte aligned bf16 {(dim,)}, got {t.dtype} {tuple(t.shape)}")
+    return ptr
+
+
+def _norm_mod(name, t, dim, segs):
+    """(address, row stride) of the modulation rows, fp32 [dim] or [segs, dim]."""
+    if t is None:
+        return 0, None
+    ptr = t.data_ptr()
+    if t.dtype != torch.float32 or t.shape not in ((dim,), (segs, dim)) or t.stride(-1) != 1 or ptr & 15:
+        raise FliteError(f"{name}: expected contiguous, 16-byte aligned fp32 rows {(dim,)} or {(segs, dim)}, got "
+                         f"{t.dtype} {tuple(t.shape)}")
+    step = t.stride(0) if t.dim() == 2 and segs > 1 else 0
+    if step & 3:
+        raise FliteError(f"{name}: the row stride must be a multiple of 4, got {step}")
+    return ptr, step
+
+
+def _norm_sizes(x, seg_rows):
+    px, ldx = _norm_rows("x", x, _NORM_X)
     rows, dim = x.shape
     if dim == 0 or dim % 8 or dim > 8192:
         raise FliteError(f"norm: dim must be a multiple of 8, at most 8192, got {dim}")
     if seg_rows < 0:
         raise FliteError(f"norm: seg_rows {seg_rows} < 0")
-    segs = (rows + seg_rows - 1) // seg_rows if seg_rows else 1
-    for name, t in (("w", w), ("b", b)):
-        if t is not None:
-            require_gpu(t, name, torch.bfloat16)
-            if tuple(t.shape) != (dim,) or t.data_ptr() % 16:
-                raise FliteError(f"{name}: expected {(dim,)}, 16-byte aligned, got {tuple(t.shape)}")
-            setattr(a, name, t.data_ptr())
-    stride = None
-    for name, t in mods.items():
-        if t is None:
-            continue
-        require_gpu(t, name, torch.float32, contiguous=False)
-        if tuple(t.shape) not in ((dim,), (segs, dim)) or t.stride(-1) != 1 or t.data_ptr() % 16:
-            raise FliteError(f"{name}: expected contiguous, 16-byte aligned rows {(dim,)} or {(segs, dim)}, got "
-                             f"{tuple(t.shape)}")
-        step = t.stride(0) if t.dim() == 2 and segs > 1 else 0
-        if step % 4 or (stride is not None and step != stride):
-            raise FliteError("norm: shift and scale must have one row stride, a multiple of 4")
-        stride = step
-        setattr(a, name, t.data_ptr())
-    a.mod_seg_stride = stride or 0
-    a.x, a.x_is_bf16 = x.data_ptr(), int(x.dtype == torch.bfloat16)
-    a.rows, a.dim, a.seg_rows, a.eps = rows, dim, int(seg_rows), float(eps)
-    return a, segs
+    return px, ldx, rows, dim, (rows + seg_rows - 1) // seg_rows if seg_rows else 1
 
 
 def layernorm_modulate(x, w=None, b=None, shift=None, scale=None, seg_rows=0, eps=1e-6, out=None):
@@ -758,13 +772,21 @@ def layernorm_modulate(x, w=None, b=None, shift=None, scale=None, seg_rows=0, ep
 
     x [rows, dim] fp32 or bf16, dim a multiple of 8 up to 8192; w, b bf16 [dim]; shift, scale fp32 [dim], or
     [segments, dim] with one row per seg_rows rows."""
-    dev = _one_device(x=x, w=w, b=b, shift=shift, scale=scale, out=out)
-    a, _ = _norm_args(x, w, b, {"shift": shift, "scale": scale}, seg_rows, eps)
-    with torch.cuda.device(dev):
-        out = torch.empty(x.shape, device=dev, dtype=torch.bfloat16) if out is None else out
-        a.ldy = _norm_rows("out", out, (torch.bfloat16,), x.shape)
-        a.y = out.data_ptr()
-        check(load().flite_layernorm_modulate(stream_ptr(dev), ctypes.byref(a)), "flite_layernorm_modulate")
+    dev = _one_device("x w b shift scale out", x, w, b, shift, scale, out)
+    px, ldx, rows, dim, segs = _norm_sizes(x, seg_rows)
+    pw, pb = _norm_vec("w", w, dim), _norm_vec("b", b, dim)
+    psh, s0 = _norm_mod("shift", shift, dim, segs)
+    psc, s1 = _norm_mod("scale", scale, dim, segs)
+    if s0 is not None and s1 is not None and s0 != s1:
+        raise FliteError("norm: shift and scale must have the same row stride")
+    if out is None:
+        out = torch.empty(x.shape, device=x.device, dtype=torch.bfloat16)
+    else:
+        _own_storage("out", out)
+    po, ldo = _norm_rows("out", out, (torch.bfloat16,), x.shape)
+    args = _NORM.pack(px, po, 0, 0, pw, pb, psh, psc, 0, 0, 0, 0, ldx, ldo, 0, 0, s0 or s1 or 0, seg_rows, rows, dim,
+                      x.dtype == torch.bfloat16, 0, eps)
+    _call(dev, "flite_layernorm_modulate", args)
     return out
 
 
@@ -775,33 +797,35 @@ def norm_modulate_bwd(dy, x, w=None, b=None, scale=None, seg_rows=0, eps=1e-6, r
     others are fp32 and None where their input is: dw, db [dim]; dscale and dshift have the shape of `scale`. A forward
     pass with a shift but no scale says shift=True (dshift is then [segments, dim]). Row statistics are made again from
     x; the sums over rows are fp32, in a fixed order."""
-    dev = _one_device(dy=dy, x=x, w=w, b=b, scale=scale, dx=dx)
+    dev = _one_device("dy x w b scale dx", dy, x, w, b, scale, dx)
     if rms and b is not None:
         raise FliteError("norm_modulate_bwd: the RMS norm has no bias")
     shared = scale is not None and scale.dim() == 1
     if shared:  # one row for all segments: its gradient is the sum over all rows
         seg_rows = 0
-    a, segs = _norm_args(x, w, b, {"scale": scale}, seg_rows, eps)
-    a.lddy = _norm_rows("dy", dy, (torch.bfloat16,), x.shape)
-    a.dy = dy.data_ptr()
-    lib = load()
-    with torch.cuda.device(dev):
-        dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if dx is None else dx
-        a.lddx = _norm_rows("dx", dx, (x.dtype,), x.shape)
-        a.dx = dx.data_ptr()
-        a.rms = int(bool(rms))
-        new = lambda want, *s: torch.empty(s, device=dev, dtype=torch.float32) if want else None  # noqa: E731
-        dim = x.shape[1]
-        dw, db = new(w is not None, dim), new(b is not None, dim)
-        mod = (dim,) if shared else (segs, dim)
-        dscale, dshift = new(scale is not None, *mod), new(scale is not None or shift, *mod)
-        a.dw, a.db, a.dshift, a.dscale = _ptr(dw), _ptr(db), _ptr(dshift), _ptr(dscale)
-        n = 0
-        if any(t is not None for t in (dw, db, dshift, dscale)):
-            n = int(lib.flite_norm_bwd_workspace_bytes(x.shape[0], int(seg_rows), dim))
-        ws = torch.empty(n // 4, device=dev, dtype=torch.float32)
-        check(lib.flite_norm_modulate_bwd(stream_ptr(dev), ctypes.byref(a), ws.data_ptr(), n),
-              "flite_norm_modulate_bwd")
+    px, ldx, rows, dim, segs = _norm_sizes(x, seg_rows)
+    pw, pb = _norm_vec("w", w, dim), _norm_vec("b", b, dim)
+    psc, step = _norm_mod("scale", scale, dim, segs)
+    pg, ldg = _norm_rows("dy", dy, (torch.bfloat16,), x.shape)
+    if dx is None:
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    else:
+        _own_storage("dx", dx)
+    pdx, lddx = _norm_rows("dx", dx, (x.dtype,), x.shape)
+    mod = (dim,) if shared else (segs, dim)
+    f32 = dict(device=x.device, dtype=torch.float32)
+    dw = None if w is None else torch.empty(dim, **f32)
+    db = None if b is None else torch.empty(dim, **f32)
+    dscale = None if scale is None else torch.empty(mod, **f32)
+    dshift = torch.empty(mod, **f32) if shift or scale is not None else None
+    size = ws = 0
+    if dw is not None or db is not None or dshift is not None:
+        size = (_lib or load()).flite_norm_bwd_workspace_bytes(rows, seg_rows, dim)
+        buf = torch.empty(size // 4, **f32)
+        ws = buf.data_ptr()
+    args = _NORM.pack(px, 0, pg, pdx, pw, pb, 0, psc, _ptr(dw) or 0, _ptr(db) or 0, _ptr(dshift) or 0, _ptr(dscale) or 0,
+                      ldx, 0, ldg, lddx, step or 0, seg_rows, rows, dim, x.dtype == torch.bfloat16, bool(rms), eps)
+    _call(dev, "flite_norm_modulate_bwd", args, ws, size)
     return dx, dw, db, dshift, dscale
 
 

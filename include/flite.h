@@ -180,8 +180,8 @@ typedef struct flite_rope_axes_args {
   const void* y;           /* backward with norm */
   float* rstd;             /* with norm */
   const void* positions;   /* device [tokens][axes], int32 or (positions_f32) fp32 */
-  const int* axis_pairs;   /* host [axes] */
-  const double* bases;     /* host [axes] */
+  double bases[8];         /* of the axes */
+  int axis_pairs[8];
   long x_row, x_head, out_row, out_head, y_row, y_head; /* elements, multiples of 8 */
   long rows, tokens;
   int axes, heads, rope_heads, head_dim;

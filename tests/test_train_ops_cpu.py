@@ -72,7 +72,7 @@ def rope_args(**kw):
     a = nat.RopeAxesArgs()
     a.x = a.out = a.y = a.rstd = a.positions = PTR
     pairs, bases = kw.pop("pairs", (8, 12, 12)), kw.pop("bases", (1e4, 1e4, 1e4))
-    a.axis_pairs, a.bases = (ctypes.c_int * len(pairs))(*pairs), (ctypes.c_double * len(bases))(*bases)
+    a.axis_pairs, a.bases = (ctypes.c_int * 8)(*pairs[:8]), (ctypes.c_double * 8)(*bases[:8])
     a.x_row = a.out_row = a.y_row = 256
     a.x_head = a.out_head = a.y_head = 64
     a.rows, a.tokens, a.axes, a.heads, a.rope_heads, a.head_dim = 10, 5, len(pairs), 4, 4, 64
