@@ -466,6 +466,12 @@ __global__ __launch_bounds__(kThreads) void attn_delta_kernel(TrainDev d, int ro
 // have been in LDS for a whole step, the first fragments of a step are read before its barrier, scores are turned into
 // P or dS in the step after their products. What a step costs beyond its 2048 MFMA cycles is the barrier.
 
+// Steps that a copy may take beyond the one it is issued in. A copy takes 1.2 to 2 us (L2 or HBM), a step 0.9 us and more
+// with D = 256, 0.4 with 128, 0.2 with 64, and LDS has room for more stages where they are small (D = 128, ragged batch:
+// 1.37 us a step without).
+template <int D>
+constexpr int kExtra = D == 256 ? 0 : D == 128 ? 2 : 4;
+
 template <int D>
 struct Stage {
   static constexpr int BYTES = 32 * D * 2;      // 32 swept rows
@@ -540,9 +546,11 @@ struct Stream {
   }
 };
 
-// The step barrier: own LDS writes and copies done, then everyone's
+// The step barrier: own LDS writes done, own copies but the last N (those of the last kExtra steps); then everyone's
+template <int N = 0>
 __device__ __forceinline__ void step_sync() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  static_assert(N < 64, "vmcnt");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
 // LDS addresses of a lane's reads in a stage, moved along from stage to stage in place (no registers for sums); k-steps
@@ -707,14 +715,16 @@ __device__ __forceinline__ unsigned pack_bf(float lo, float hi) {
   return __builtin_bit_cast(unsigned, v);
 }
 
-// LDS of a key workgroup: q ring of 5 stages, dout ring of 3, P double-buffered, lse and delta rings of 4; of a query
-// workgroup: k ring of 5, v ring of 3, dS double-buffered (D = 256: all 160 KB)
+// LDS of a key workgroup: q ring of 5 stages, dout ring of 3, P double-buffered, lse and delta rings; of a query
+// workgroup: k ring of 5, v ring of 3, dS double-buffered (D = 256: all 160 KB). Rings are kExtra stages longer.
 template <int D>
 struct Lds {
-  static constexpr int A = 0, B = 5 * Stage<D>::BYTES, X = B + 3 * Stage<D>::BYTES;
+  static constexpr int RA = 5 + kExtra<D>, RB = 3 + kExtra<D>;
+  static constexpr int A = 0, B = RA * Stage<D>::BYTES, X = B + RB * Stage<D>::BYTES;
   static constexpr int PBYTES = 8192, SBYTES = 16384;  // one buffer of P, of dS
-  static constexpr int LSE = X + 2 * PBYTES, DELTA = LSE + 4 * 256, TOTAL = X + 2 * SBYTES;
-  static_assert(DELTA + 4 * 256 <= TOTAL, "lse and delta lie behind P, where a query workgroup has its dS");
+  static constexpr int LSE = X + 2 * PBYTES, DELTA = LSE + 8 * 256, TOTAL = X + 2 * SBYTES;
+  static_assert(DELTA + 8 * 256 <= TOTAL, "lse and delta lie behind P, where a query workgroup has its dS");
+  static_assert(TOTAL <= 160 * 1024 && 3 + kExtra<D> < 8, "LDS of a CU; the rings of lse and delta");
 };
 
 // First of the `all` pieces of work that stand behind MFMA m of M, of which the first SKIP have none
@@ -735,7 +745,7 @@ template <int D>
 __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) {
   const AttnTrainParams& p = d.p;
   using L = Lds<D>;
-  constexpr int ND = D / 32, SB = Stage<D>::BYTES, P = Stage<D>::PIECES;
+  constexpr int ND = D / 32, SB = Stage<D>::BYTES, P = Stage<D>::PIECES, E = kExtra<D>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lq = lane & 31, hh = lane >> 5, pair = wave >> 1;
   Unit u;
@@ -768,8 +778,9 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
     st_d.init(p.dout + (long)q_start * p.do_row + h0 * p.do_head, t0, tiles, q_len, n, p.do_row * 2, p.do_head * 2);
     st_x.init((wave == 0 ? d.lse2 : d.delta) + h0 * p.total_q + q_start, t0, tiles, q_len, n, 4, (long)p.total_q * 4);
     i32x4 rq, rd, rx;
-    int q5 = 0, d3 = 0;  // step mod 5, mod 3
-    // stages i + 3 of q and i + 2 of dout, in 2 P + 1 pieces: issued behind step i's barrier, in place at the next one
+    int qi = 0, di = 0;  // step mod RA, mod RB
+    // stages i + 3 + E of q and i + 2 + E of dout, in 2 P + 1 pieces: issued behind step i's barrier, in place E + 1
+    // barriers later
     auto open = [&]() {
       rq = st_q.next();
       rd = st_d.next();
@@ -777,35 +788,35 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
     };
     auto copy = [&](int i, int k) {
       if (k < P)
-        copy16(rq, sq.src(k), wlds + L::A + wrap<5>(q5 + 3) * SB + sq.dst(k));
+        copy16(rq, sq.src(k), wlds + L::A + wrap<L::RA>(qi + 3 + E) * SB + sq.dst(k));
       else if (k < 2 * P)
-        copy16(rd, sd.src(k - P), wlds + L::B + wrap<3>(d3 + 2) * SB + sd.dst(k - P));
+        copy16(rd, sd.src(k - P), wlds + L::B + wrap<L::RB>(di + 2 + E) * SB + sd.dst(k - P));
       else if (k == 2 * P && wave < 2)
-        copy4(rx, ld_off, lds0 + (wave == 0 ? L::LSE + ((i + 3) & 3) * 256 : L::DELTA + ((i + 2) & 3) * 256));
+        copy4(rx, ld_off, lds0 + (wave == 0 ? L::LSE + ((i + 3 + E) & 7) * 256 : L::DELTA + ((i + 2 + E) & 7) * 256));
     };
     // bytes from slot x of a ring to the next one
-    auto next5 = [&](int x) { return wrap<5>(x) == 4 ? -4 * SB : SB; };
-    auto next3 = [&](int x) { return wrap<3>(x) == 2 ? -2 * SB : SB; };
+    auto next_a = [&](int x) { return wrap<L::RA>(x) == L::RA - 1 ? (1 - L::RA) * SB : SB; };
+    auto next_b = [&](int x) { return wrap<L::RB>(x) == L::RB - 1 ? (1 - L::RB) * SB : SB; };
     RowReader<D> rr;
     TrReader<D> tr;
-    // before step 0: q stages -1 (zeros: dk(-1) adds nothing), 0, 1, 2; dout stages 0, 1
+    // before step 0: q stages -1 (zeros: dk(-1) adds nothing), 0 .. 2 + E; dout stages 0 .. 1 + E
     {
       const i32x4 zero = make_rsrc(p.q, 0);
 #pragma unroll
-      for (int k = 0; k < P; ++k) copy16(zero, sq.src(k), wlds + L::A + 4 * SB + sq.dst(k));
+      for (int k = 0; k < P; ++k) copy16(zero, sq.src(k), wlds + L::A + (L::RA - 1) * SB + sq.dst(k));
 #pragma unroll
-      for (int j = 0; j < 3; ++j) {
+      for (int j = 0; j < 3 + E; ++j) {
         rq = st_q.next();
 #pragma unroll
         for (int k = 0; k < P; ++k) copy16(rq, sq.src(k), wlds + L::A + j * SB + sq.dst(k));
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 2 + E; ++j) {
         rd = st_d.next();
 #pragma unroll
         for (int k = 0; k < P; ++k) copy16(rd, sd.src(k), wlds + L::B + j * SB + sd.dst(k));
       }
-      for (int j = 0; j < (wave == 0 ? 3 : 2); ++j) {
+      for (int j = 0; j < (wave == 0 ? 3 : 2) + E; ++j) {
         rx = st_x.next();
         if (wave < 2) copy4(rx, ld_off, lds0 + (wave == 0 ? L::LSE : L::DELTA) + j * 256);
       }
@@ -830,8 +841,8 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
     auto nothing = []() {};
     // work behind MFMA m of the tr phase: copies of step i, and the 32 scores spread over the MFMAs m >= SKIP
     auto spread = [&](int i, int m, auto one) {
-      constexpr int E = (4 * ND) / (2 * P + 1);
-      if (m % E == 0 && m / E <= 2 * P) copy(i, m / E);
+      constexpr int GAP = (4 * ND) / (2 * P + 1);
+      if (m % GAP == 0 && m / GAP <= 2 * P) copy(i, m / GAP);
 #pragma unroll
       for (int e = share(m, 4 * ND, 32); e < share(m + 1, 4 * ND, 32); ++e) one(e);
     };
@@ -852,7 +863,7 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
         if ((e & 7) == 0) lse = lse_n;
         x = __builtin_fmaf(s[nb][4 * r4 + i], sl2, -lse[i]);
         if ((e & 7) == 0 && r4 < 3)
-          lse_n = *(const f32x4*)(smem + L::LSE + (j & 3) * 256 + (8 * (r4 + 1) + 4 * hh) * 4);
+          lse_n = *(const f32x4*)(smem + L::LSE + (j & 7) * 256 + (8 * (r4 + 1) + 4 * hh) * 4);
       };
       auto store = [&](int j, int e) {  // P of score e is there
         const int r4 = e >> 3, nb = (e >> 2) & 1, i = e & 3, r = 4 * r4 + i;
@@ -863,7 +874,7 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
               f16x4{(_Float16)s[nb][r - 3], (_Float16)s[nb][r - 2], (_Float16)s[nb][r - 1], (_Float16)s[nb][r]};
         }
       };
-      auto begin = [&](int j) { lse_n = *(const f32x4*)(smem + L::LSE + (j & 3) * 256 + 4 * hh * 4); };
+      auto begin = [&](int j) { lse_n = *(const f32x4*)(smem + L::LSE + (j & 7) * 256 + 4 * hh * 4); };
       auto prob = [&](int j, int e) {
         if (e == 0) arg(j, 0);
         s[(e >> 2) & 1][4 * (e >> 3) + (e & 3)] = __builtin_amdgcn_exp2f(x);
@@ -885,13 +896,16 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
         open();
         begin(i + 1);
         row_phase<D>(rr, ra, f, s, none, [&]() { ta.read(tr); });
-        rr.move(next5(q5 + 1));
-        step_sync();
+        rr.move(next_a(qi + 1));
+        if (wave == 0)
+          step_sync<E*(2 * P + 1)>();
+        else
+          step_sync<E * 2 * P>();
         tr_phase<D>(tr, ta, bc, acc, [&](int m) { spread(i, m, [&](int e) { prob(i + 1, e); }); }, [&]() { ra.read(rr); });
         next();
-        tr.move(next3(d3));
-        q5 = wrap<5>(q5 + 1);
-        d3 = wrap<3>(d3 + 1);
+        tr.move(next_b(di));
+        qi = wrap<L::RA>(qi + 1);
+        di = wrap<L::RB>(di + 1);
       }
       step_sync();
     } else {
@@ -900,7 +914,7 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) bc[nb][ks] = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
       rr.init(lane, lds0 + L::B);           // dout stage i
-      tr.init(lane, lds0 + L::A + 4 * SB);  // q stage i - 1
+      tr.init(lane, lds0 + L::A + (L::RA - 1) * SB);  // q stage i - 1
       ra.read(rr);
       f32x4 del, del_n;
       typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
@@ -908,13 +922,16 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
       for (int i = 0; i <= n; ++i) {
         auto rd = [&](int e) {  // delta and P of the 4 scores from e on
           const int r4 = e >> 3, nb = (e >> 2) & 1;
-          if (nb == 0) del_n = *(const f32x4*)(smem + L::DELTA + (i & 3) * 256 + (8 * r4 + 4 * hh) * 4);
+          if (nb == 0) del_n = *(const f32x4*)(smem + L::DELTA + (i & 7) * 256 + (8 * r4 + 4 * hh) * 4);
           pr_n = *(const f16x4*)(xch + (i & 1) * L::PBYTES + (r4 * 2 + nb) * 512);
         };
         open();  // after the last stage: zeros
         row_phase<D>(rr, ra, f, s, none, [&]() { ta.read(tr); });
-        rr.move(next3(d3));
-        step_sync();
+        rr.move(next_b(di));
+        if (wave == 1)
+          step_sync<E*(2 * P + 1)>();
+        else
+          step_sync<E * 2 * P>();
         rd(0);
         tr_phase<D>(
             tr, ta, bc, acc,
@@ -932,9 +949,9 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
             },
             [&]() { ra.read(rr); });
         next();
-        tr.move(next5(q5 + 4));
-        q5 = wrap<5>(q5 + 1);
-        d3 = wrap<3>(d3 + 1);
+        tr.move(next_a(qi - 1));
+        qi = wrap<L::RA>(qi + 1);
+        di = wrap<L::RB>(di + 1);
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may outlive the workgroup
@@ -966,7 +983,7 @@ template <int D>
 __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem) {
   const AttnTrainParams& p = d.p;
   using L = Lds<D>;
-  constexpr int ND = D / 32, NS = D / 16, SB = Stage<D>::BYTES, P = Stage<D>::PIECES;
+  constexpr int ND = D / 32, NS = D / 16, SB = Stage<D>::BYTES, P = Stage<D>::PIECES, E = kExtra<D>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lq = lane & 31, hh = lane >> 5, pair = wave >> 1;
   Unit u;
@@ -992,16 +1009,16 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
     st_v.init(p.v + (long)k_start * p.v_row + (long)hk * p.v_head, t0, all, k_len, n, p.v_row * 2, 0);
   }
   i32x4 rk, rv;
-  int k5 = 0, v3 = 0;  // step mod 5, mod 3
+  int ki = 0, vi = 0;  // step mod RA, mod RB
   auto open = [&]() {
     rk = st_k.next();
     rv = st_v.next();
   };
   auto copy = [&](int j, int k) {  // piece k of k and v stage i + j
     if (k < P)
-      copy16(rk, sk.src(k), wlds + L::A + wrap<5>(k5 + j) * SB + sk.dst(k));
+      copy16(rk, sk.src(k), wlds + L::A + wrap<L::RA>(ki + j) * SB + sk.dst(k));
     else if (k < 2 * P)
-      copy16(rv, sv.src(k - P), wlds + L::B + wrap<3>(v3 + (j == 3 ? 0 : j)) * SB + sv.dst(k - P));
+      copy16(rv, sv.src(k - P), wlds + L::B + wrap<L::RB>(vi + (j == L::RB ? 0 : j)) * SB + sv.dst(k - P));
   };
   auto copy_all = [&](int j) {
     open();
@@ -1009,17 +1026,16 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
     for (int k = 0; k < 2 * P; ++k) copy(j, k);
   };
   auto advance = [&]() {
-    k5 = wrap<5>(k5 + 1);
-    v3 = wrap<3>(v3 + 1);
+    ki = wrap<L::RA>(ki + 1);
+    vi = wrap<L::RB>(vi + 1);
   };
 
   // dS of stage j: [j & 1][pair][block][r4][lane] f32x4
   char* const xch = smem + L::X + pair * (L::SBYTES / 2) + lane * 16;
   if ((wave & 1) == 0) {
     if (n <= 0) return;  // wave 1 stores the zeros
-    copy_all(0);
-    copy_all(1);
-    copy_all(2);
+#pragma unroll
+    for (int j = 0; j < 3 + E; ++j) copy_all(j);
     bf16x8 qf[2][NS], df[2][NS];
     float lse[2], del[2];
 #pragma unroll
@@ -1102,15 +1118,15 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
           [&](int m) {
 #pragma unroll
             for (int u = share(m, 4 * NS, 64); u < share(m + 1, 4 * NS, 64); ++u) ds_half(i, s, dp, u);
-            if ((m & 1) && (m >> 1) < 2 * P) copy(3, m >> 1);
+            if ((m & 1) && (m >> 1) < 2 * P) copy(3 + E, m >> 1);
           },
           [&]() {
-            kr.move(wrap<5>(k5 + 1) == 4 ? -4 * SB : SB);
-            vr.move(wrap<3>(v3 + 1) == 2 ? -2 * SB : SB);
+            kr.move(wrap<L::RA>(ki + 1) == L::RA - 1 ? (1 - L::RA) * SB : SB);
+            vr.move(wrap<L::RB>(vi + 1) == L::RB - 1 ? (1 - L::RB) * SB : SB);
             read_first();
           });
       advance();
-      step_sync();
+      step_sync<E * 2 * P>();
     };
     step_sync();
     read_first();
@@ -1130,18 +1146,17 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
   f32x16 acc[2][ND];
   acc_zero<ND>(acc);
   if (n > 0) {
-    copy_all(0);
-    copy_all(1);
-    copy_all(2);
+#pragma unroll
+    for (int j = 0; j < 3 + E; ++j) copy_all(j);
     step_sync();
     step_sync();
-    copy_all(3);
+    copy_all(3 + E);
     bf16x8 a[ND];
     TrReader<D> tr;  // k stage i - 1
     tr.init(lane, lds0 + L::A);
     auto rd = [&](int s, int dt) { a[dt] = tr.read(s, dt); };
     advance();
-    step_sync();
+    step_sync<E * 2 * P>();
     for (int i = 1; i <= n; ++i) {
       open();  // after the last stage: zeros
       const char* x = xch + ((i - 1) & 1) * L::SBYTES;
@@ -1186,7 +1201,7 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
 #pragma unroll
           for (int q = 0; q < 8; ++q)
             if (s == 0 && q * ND / 4 == m) split_lo(0, q);
-          if (s == 1 && (m & 1)) copy(3, P + (m >> 1));
+          if (s == 1 && (m & 1)) copy(3 + E, P + (m >> 1));
           FENCE();
         }
         settle();
@@ -1203,13 +1218,13 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
               split_hi(1, q);
               split_lo(1, q);
             }
-          if (s == 0 && !(m & 1) && (m >> 1) < P) copy(3, m >> 1);
+          if (s == 0 && !(m & 1) && (m >> 1) < P) copy(3 + E, m >> 1);
           FENCE();
         }
       }
-      tr.move(wrap<5>(k5 + 4) == 4 ? -4 * SB : SB);
+      tr.move(wrap<L::RA>(ki - 1) == L::RA - 1 ? (1 - L::RA) * SB : SB);
       advance();
-      if (i < n) step_sync();
+      if (i < n) step_sync<E * 2 * P>();
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may outlive the workgroup
   }
