@@ -41,6 +41,7 @@ constexpr int kThreads = 256;
 constexpr int kMaxRanges = 16;
 constexpr int kMinRange = 8;  // stages: what a workgroup's start and end cost
 constexpr int kCus = 256;
+constexpr int kFullShare = 2;  // ranges of full tiles that make up a CU's share of the work
 
 // How a launch cuts its work. A unit is one 128-row tile ("full", or the rest of a sequence, "part") of one head with
 // its whole sweep; where units are few or long, a sweep is cut into ranges, whose fp32 partial gradients a last kernel
@@ -59,7 +60,8 @@ struct TrainDev {
   AttnTrainParams p;
   int tiles_q;             // forward: upper bound of the 128-row tiles
   Cut q, k;
-  int* target;             // stages per range: of a full tile, of a part
+  int* target;             // stages per range: of a full tile, of a part; [2]: groups, [3]: blocks that have work
+  int4* groups;            // [4 B] (Group)
   float* lse2;             // [H][total_q] lse * log2 e - kShift
   float* delta;            // [H][total_q]
 };
@@ -99,31 +101,6 @@ __device__ __forceinline__ bool find_tile(const int* cu, int B, int total, int t
   return false;
 }
 
-// Full tile t of the packed batch -> (sequence, first row); false past the last one
-__device__ __forceinline__ bool find_full(const int* cu, int B, int total, int t, int* b, int* row0) {
-  const int lane = threadIdx.x & 63;
-  for (int base = 0; base < B; base += 64) {
-    int s, len = 0;
-    if (base + lane < B) seq_range(cu, base + lane, total, &s, &len);
-    const int n = len / WROWS;
-    int sum = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int up = __shfl_up(sum, o, 64);
-      if (lane >= o) sum += up;
-    }
-    const unsigned long long hit = __ballot(t < sum);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      *b = base + l;
-      *row0 = (t - (__shfl(sum, l, 64) - __shfl(n, l, 64))) * WROWS;
-      return true;
-    }
-    t -= __shfl(sum, 63, 64);
-  }
-  return false;
-}
-
 // Sequence that holds `row`, -1: none
 __device__ __forceinline__ int find_seq(const int* cu, int B, int total, int row) {
   int lo = 0, hi = B;  // the last b with cu[b] <= row
@@ -141,35 +118,49 @@ __device__ __forceinline__ int ranges_of(int stages, int target, int most) {
   return min(max((stages + target - 1) / target, 1), most);
 }
 
+// The backward pass's work list: groups of equal units (the full tiles of a sequence, or its part, as keys or as queries),
+// the longest ranges first. Made on the device, which alone knows the lengths; the launch has an upper bound of blocks.
+struct Group {
+  static constexpr int PART = 1, QUERY = 2;
+  static __device__ int4 make(int first, int b, int kind, int ranges, int tiles) {
+    return make_int4(first, b * 4 + kind, ranges, tiles);
+  }
+};
 // One unit and range of the sweep over it
 struct Unit {
-  int b, h, row0, part;
-  bool full;
+  int b, h, tile, part, ranges;
+  bool full, query;
 };
-// Block v of `c` -> its unit; false: nothing to do. own: the tiles' cu_seqlens
-__device__ __forceinline__ bool find_unit(const Cut& c, int v, const int* own, int B, int total, Unit* u) {
-  const int nf = c.full_blocks();
-  u->full = v < nf;
-  if (u->full) {
-    u->part = v % c.max_full;
-    v /= c.max_full;
-    u->h = v / c.full;
-    if (!find_full(own, B, total, v % c.full, &u->b, &u->row0)) return false;
-  } else {
-    v -= nf;
-    u->part = v % c.max_part;
-    v /= c.max_part;
-    u->b = v % B;
-    u->h = v / B;
-    int s, len;
-    seq_range(own, u->b, total, &s, &len);
-    if (len % WROWS == 0) return false;
-    u->row0 = len - len % WROWS;
+// Block v -> its unit; false: nothing to do
+__device__ __forceinline__ bool find_unit(const TrainDev& d, int v, Unit* u) {
+  const int lane = threadIdx.x & 63;
+  const int n = d.target[2], blocks = d.target[3];
+  if (v >= blocks) return false;
+  for (int base = 0; base < n; base += 64) {
+    // the group of v is the last one that starts at or before it; the entry behind it tells its size
+    const int4 g = d.groups[min(base + lane, n - 1)];
+    const int next = base + lane + 1 < n ? d.groups[base + lane + 1].x : blocks;
+    const unsigned long long hit = __ballot(base + lane < n && g.x <= v && v < next);
+    if (hit == 0) continue;
+    const int l = __builtin_ctzll(hit);
+    const int first = __builtin_amdgcn_readfirstlane(__shfl(g.x, l, 64));
+    const int size = __builtin_amdgcn_readfirstlane(__shfl(next, l, 64)) - first;
+    const int id = __builtin_amdgcn_readfirstlane(__shfl(g.y, l, 64));
+    const int tiles = __builtin_amdgcn_readfirstlane(__shfl(g.w, l, 64));
+    u->ranges = __builtin_amdgcn_readfirstlane(__shfl(g.z, l, 64));
+    u->b = id >> 2;
+    u->full = !(id & Group::PART);
+    u->query = (id & Group::QUERY) != 0;
+    v = xcd_remap(v - first, size);  // neighbours in the group (tiles of a head) on one XCD
+    u->part = v % u->ranges;
+    v /= u->ranges;
+    u->tile = v % tiles;
+    u->h = v / tiles;
+    return true;
   }
-  u->b = __builtin_amdgcn_readfirstlane(u->b);
-  u->row0 = __builtin_amdgcn_readfirstlane(u->row0);
-  return true;
+  return false;
 }
+
 // Row `row` of sequence b, head h, range 0 in the partial gradients; *step: floats from range to range
 template <int D>
 __device__ __forceinline__ float* part_row(const Cut& c, bool full, int B, int total, int start, int b, int row, int h,
@@ -400,32 +391,97 @@ __global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward
+// One workgroup: the ranges' lengths and the work list
+__device__ __forceinline__ void make_groups(const TrainDev& d) {
+  const AttnTrainParams& p = d.p;
+  __shared__ double sums[kThreads / 64];
+  __shared__ int cost[kThreads], count[kThreads], waves[kThreads / 64];
+  const int tid = threadIdx.x;
+  // Stages of all units, over the CUs: a range of a full tile is at most half of a CU's share, one of a part (they fill
+  // the end of the launch) a 32nd; none is shorter than kMinRange
+  double sum = 0.;
+  for (int b = tid; b < p.B; b += kThreads) {
+    int s, ql, kl;
+    seq_range(p.cu_q, b, p.total_q, &s, &ql);
+    seq_range(p.cu_k, b, p.total_k, &s, &kl);
+    sum += ((double)((ql + WROWS - 1) / WROWS) * ((kl + 31) / 32) + (double)((kl + WROWS - 1) / WROWS) * ((ql + 31) / 32)) * p.H;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if ((tid & 63) == 0) sums[tid >> 6] = sum;
+  __syncthreads();
+  sum = 0.;
+  for (int w = 0; w < kThreads / 64; ++w) sum += sums[w];
+  const double share = fmin(sum / kCus, 1e9);
+  const int t_full = max((int)(share / kFullShare), kMinRange), t_part = max((int)(share / 32), kMinRange);
+  // entry e: kind e / B (keys full, keys part, queries full, queries part) of sequence e % B
+  const int n = 4 * p.B;
+  int first = 0;
+  for (int base = 0; base < n; base += kThreads) {
+    const int e = base + tid;
+    int b = 0, kind = 0, ranges = 1, tiles = 0, blocks = 0, len = 0;
+    if (e < n) {
+      kind = e / p.B;
+      b = e % p.B;
+      const bool query = (kind & Group::QUERY) != 0, part = (kind & Group::PART) != 0;
+      int s, ql, kl;
+      seq_range(p.cu_q, b, p.total_q, &s, &ql);
+      seq_range(p.cu_k, b, p.total_k, &s, &kl);
+      const Cut& c = query ? d.q : d.k;
+      const int own = query ? ql : kl, stages = ((query ? kl : ql) + 31) / 32 * (query ? 1 : p.H / p.HK);
+      tiles = part ? (own % WROWS ? 1 : 0) : own / WROWS;
+      ranges = ranges_of(stages, part ? t_part : t_full, part ? c.max_part : c.max_full);
+      blocks = tiles * c.heads * ranges;
+      len = (stages + ranges - 1) / ranges;
+    }
+    // rank: by length, then by number (only where all groups fit one round of threads: else they keep their order)
+    int rank = tid;
+    __syncthreads();
+    if (n <= kThreads) {
+      cost[tid] = e < n && blocks > 0 ? len : -1;
+      __syncthreads();
+      const int mine = cost[tid];
+      rank = e < n ? 0 : tid;
+      for (int i = 0; e < n && i < n; ++i) rank += cost[i] > mine || (cost[i] == mine && i < tid);
+    }
+    count[rank] = blocks;
+    __syncthreads();
+    int upto = count[tid];  // blocks of the ranks up to tid
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(upto, o, 64);
+      if ((tid & 63) >= o) upto += up;
+    }
+    if ((tid & 63) == 63) waves[tid >> 6] = upto;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < kThreads / 64; ++w) {
+      if (w < (tid >> 6)) upto += waves[w];
+      all += waves[w];
+    }
+    count[tid] = upto;
+    __syncthreads();
+    if (e < n) d.groups[base + rank] = Group::make(first + count[rank] - blocks, b, kind, ranges, max(tiles, 1));
+    first += all;
+    __syncthreads();
+  }
+  if (tid == 0) {
+    d.target[0] = t_full;
+    d.target[1] = t_part;
+    d.target[2] = n;
+    d.target[3] = first;
+  }
+}
+
 // First launch of the backward pass: lse * log2 e and delta of every query row (those outside all sequences are read by
 // nobody); the ranges' length; zeros outside
 template <int D>
-__global__ __launch_bounds__(kThreads) void attn_delta_kernel(TrainDev d, int row_blocks) {
+__global__ __launch_bounds__(kThreads) void attn_delta_kernel(TrainDev d, int n) {  // the first n workgroups: the rest
   const AttnTrainParams& p = d.p;
   constexpr int LANES = D / 8;
-  if ((int)blockIdx.x >= row_blocks) {
-    const int i = blockIdx.x - row_blocks, n = gridDim.x - row_blocks;
-    if (i == 0 && threadIdx.x < 64) {
-      // Stages of all units, over the CUs: a range of a full tile is at most half of a CU's share, one of a part (they
-      // fill the end of the launch) a 32nd; none is shorter than kMinRange
-      double sum = 0.;
-      for (int b = threadIdx.x; b < p.B; b += 64) {
-        int s, ql, kl;
-        seq_range(p.cu_q, b, p.total_q, &s, &ql);
-        seq_range(p.cu_k, b, p.total_k, &s, &kl);
-        sum += ((double)((ql + WROWS - 1) / WROWS) * ((kl + 31) / 32) + (double)((kl + WROWS - 1) / WROWS) * ((ql + 31) / 32)) * p.H;
-      }
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-      if (threadIdx.x == 0) {
-        const double share = fmin(sum / kCus, 1e9);
-        d.target[0] = max((int)(share / 2), kMinRange);
-        d.target[1] = max((int)(share / 32), kMinRange);
-      }
-    }
+  if ((int)blockIdx.x < n) {
+    const int i = blockIdx.x;
+    if (i == 0) make_groups(d);
     if (p.zero_outside) {
       zero_outside(p.dq, p.dq_row, p.dq_head, p.cu_q, p.B, p.total_q, p.H, D, nullptr, i, n);
       zero_outside(p.dk, p.dk_row, p.dk_head, p.cu_k, p.B, p.total_k, p.HK, D, nullptr, i, n);
@@ -433,7 +489,7 @@ __global__ __launch_bounds__(kThreads) void attn_delta_kernel(TrainDev d, int ro
     }
     return;
   }
-  const long item = ((long)blockIdx.x * kThreads + threadIdx.x) / LANES;
+  const long item = ((long)(blockIdx.x - n) * kThreads + threadIdx.x) / LANES;
   const int c = threadIdx.x % LANES;
   if (item >= (long)p.total_q * p.H) return;
   const int row = (int)(item / p.H), h = (int)(item % p.H);
@@ -742,23 +798,20 @@ __device__ __forceinline__ int wrap(int i) {
 // dout(i)^T P(i) to dv while it turns S(i + 1) into P(i + 1); wave 1 makes dP(i), then adds q(i - 1)^T dS(i - 1) to dk
 // while it makes dS(i) from dP(i) and P(i).
 template <int D>
-__device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) {
+__device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char* smem) {
   const AttnTrainParams& p = d.p;
   using L = Lds<D>;
   constexpr int ND = D / 32, SB = Stage<D>::BYTES, P = Stage<D>::PIECES, E = kExtra<D>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lq = lane & 31, hh = lane >> 5, pair = wave >> 1;
-  Unit u;
-  if (!find_unit(d.k, v, p.cu_k, p.B, p.total_k, &u)) return;
-  const int hk = u.h, b = u.b, row0 = u.row0;
+  const int hk = u.h, b = u.b;
   int q_start, q_len, k_start, k_len;
   seq_range(p.cu_q, b, p.total_q, &q_start, &q_len);
   seq_range(p.cu_k, b, p.total_k, &k_start, &k_len);
+  const int row0 = u.full ? u.tile * WROWS : k_len - k_len % WROWS;
   const int group = p.H / p.HK;
   const int tiles = (q_len + 31) / 32;  // stages of one head
-  const int all = tiles * group;
-  const int ranges = ranges_of(all, d.target[u.full ? 0 : 1], u.full ? d.k.max_full : d.k.max_part);
-  if (u.part >= ranges) return;
+  const int all = tiles * group, ranges = u.ranges;
   const int per = (all + ranges - 1) / ranges, t0 = min(u.part * per, all), n = min(per, all - t0);
 
   f32x16 acc[2][ND];
@@ -980,22 +1033,19 @@ __device__ __forceinline__ void key_block(const TrainDev& d, int v, char* smem) 
 // A query workgroup: dq of 128 queries of head h. Step i: wave 0 makes S and dP of stage i + 1 while it makes dS(i);
 // wave 1 adds k(i - 1)^T dS(i - 1) to dq.
 template <int D>
-__device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem) {
+__device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, char* smem) {
   const AttnTrainParams& p = d.p;
   using L = Lds<D>;
   constexpr int ND = D / 32, NS = D / 16, SB = Stage<D>::BYTES, P = Stage<D>::PIECES, E = kExtra<D>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lq = lane & 31, hh = lane >> 5, pair = wave >> 1;
-  Unit u;
-  if (!find_unit(d.q, v, p.cu_q, p.B, p.total_q, &u)) return;
-  const int h = u.h, b = u.b, row0 = u.row0;
+  const int h = u.h, b = u.b;
   int q_start, q_len, k_start, k_len;
   seq_range(p.cu_q, b, p.total_q, &q_start, &q_len);
   seq_range(p.cu_k, b, p.total_k, &k_start, &k_len);
+  const int row0 = u.full ? u.tile * WROWS : q_len - q_len % WROWS;
   const int hk = h / (p.H / p.HK);
-  const int all = (k_len + 31) / 32;
-  const int ranges = ranges_of(all, d.target[u.full ? 0 : 1], u.full ? d.q.max_full : d.q.max_part);
-  if (u.part >= ranges) return;
+  const int all = (k_len + 31) / 32, ranges = u.ranges;
   const int per = (all + ranges - 1) / ranges, t0 = min(u.part * per, all), n = min(per, all - t0);
 
   Stage<D> sk, sv;
@@ -1247,15 +1297,12 @@ __device__ __forceinline__ void query_block(const TrainDev& d, int v, char* smem
 template <int D>
 __global__ __launch_bounds__(kThreads, 1) void attn_bwd_kernel(TrainDev d) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  // heavy units first: full tiles of keys, parts of keys, then the queries' (their parts end the launch)
-  const int nk = d.k.blocks(d.p.B), kf = d.k.full_blocks(), qf = d.q.full_blocks(), nq = d.q.blocks(d.p.B);
-  int v = blockIdx.x;
-  if (v < nk) {
-    key_block<D>(d, v < kf ? xcd_remap(v, kf) : kf + xcd_remap(v - kf, nk - kf), smem);
-  } else {
-    v -= nk;
-    query_block<D>(d, v < qf ? xcd_remap(v, qf) : qf + xcd_remap(v - qf, nq - qf), smem);
-  }
+  Unit u;
+  if (!find_unit(d, blockIdx.x, &u)) return;
+  if (u.query)
+    query_block<D>(d, u, smem);
+  else
+    key_block<D>(d, u, smem);
 }
 
 // Adds the ranges' partial gradients in order: one item = 8 columns of a row and head, of all rows (full tiles) or of the
@@ -1336,7 +1383,7 @@ Plan make_plan(const AttnTrainParams& p) {
     c.heads = heads;
     const double longest = std::min(sweep * 4, sweep * p.B) / kMinRange;
     auto ranges = [&](double want) { return (int)std::max(1., std::min({(double)kMaxRanges, want, longest})); };
-    c.max_full = ranges(3 * sweep / (share / 2));
+    c.max_full = ranges(3 * sweep / (share / kFullShare));
     c.max_part = ranges((double)kCus / ((double)p.B * heads));
     return c;
   };
@@ -1348,7 +1395,7 @@ Plan make_plan(const AttnTrainParams& p) {
   auto part_bytes = [&](const Cut& c) {
     return c.max_part > 1 ? pad((long)c.max_part * p.B * WROWS * c.heads * p.dim * 4) : 0;
   };
-  x.head_bytes = 256;
+  x.head_bytes = pad(256 + (long)p.B * 4 * 16);
   x.lse_bytes = pad((long)p.H * p.total_q * 8);
   x.qf_bytes = full_bytes(x.q, p.total_q);
   x.qp_bytes = part_bytes(x.q);
@@ -1409,7 +1456,8 @@ int launch_bwd(const TrainDev& d, hipStream_t s) {
   if (lds_limit(attn_bwd_kernel<D>, lds, done)) return 1;
   auto blocks = [](long rows_heads) { return (int)((rows_heads * (D / 8) + kThreads - 1) / kThreads); };
   const int q_rows = blocks((long)p.total_q * p.H);
-  hipLaunchKernelGGL(attn_delta_kernel<D>, dim3(q_rows + (p.zero_outside ? kZeroBlocks : 1)), dim3(kThreads), 0, s, d, q_rows);
+  const int extra = p.zero_outside ? kZeroBlocks : 1;
+  hipLaunchKernelGGL(attn_delta_kernel<D>, dim3(extra + q_rows), dim3(kThreads), 0, s, d, extra);
   FLITE_HIP_CHECK(hipGetLastError());
   hipLaunchKernelGGL(attn_bwd_kernel<D>, dim3(d.k.blocks(p.B) + d.q.blocks(p.B)), dim3(kThreads), lds, s, d);
   FLITE_HIP_CHECK(hipGetLastError());
@@ -1474,6 +1522,7 @@ int attn_train_bwd(const AttnTrainParams& p, void* ws, long ws_bytes, hipStream_
     return r;
   };
   d.target = (int*)take(x.head_bytes);
+  d.groups = (int4*)(d.target + 64);
   d.lse2 = (float*)take(x.lse_bytes);
   d.delta = d.lse2 + (long)p.H * p.total_q;
   d.q.ws_full = (float*)take(x.qf_bytes);
