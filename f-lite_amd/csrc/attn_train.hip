@@ -36,7 +36,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kShift = 15.f, kUnshift = 1.f / 32768.f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int WROWS = 128;  // stationary rows of a workgroup
-constexpr int TR = 64;      // swept rows of an LDS tile
 constexpr int kThreads = 256;
 constexpr int kMaxRanges = 16;
 constexpr int kMinRange = 8;  // stages: what a workgroup's start and end cost
@@ -58,7 +57,12 @@ struct Cut {
 
 struct TrainDev {
   AttnTrainParams p;
-  int tiles_q;             // forward: upper bound of the 128-row tiles
+  // forward
+  int tiles;               // upper bound of the 256-row tiles
+  int most, stages;        // ranges of a sweep, at most; stages of a range
+  float* part_o;           // [most][total_q][H][D] with most > 1: sums of 2^(S - m) v
+  float2* part_ml;         // [most][H][total_q]: m and the sum of 2^(S - m), S in units of log2
+  // backward
   Cut q, k;
   int* target;             // stages per range: of a full tile, of a part; [2]: groups, [3]: blocks that have work
   int4* groups;            // [4 B] (Group)
@@ -75,14 +79,15 @@ __device__ __forceinline__ void seq_range(const int* cu, int b, int total, int* 
   *len = e - s;
 }
 
-// Tile t of the packed batch -> (sequence, first row); false past the last tile. Tiles number the sequences' 128-row
+// Tile t of R rows of the packed batch -> (sequence, first row); false past the last one. Tiles number the sequences'
 // pieces in order.
+template <int R>
 __device__ __forceinline__ bool find_tile(const int* cu, int B, int total, int t, int* b, int* row0) {
   const int lane = threadIdx.x & 63;
   for (int base = 0; base < B; base += 64) {
     int s, len = 0;
     if (base + lane < B) seq_range(cu, base + lane, total, &s, &len);
-    const int n = (len + WROWS - 1) / WROWS;
+    const int n = (len + R - 1) / R;
     int sum = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -93,7 +98,7 @@ __device__ __forceinline__ bool find_tile(const int* cu, int B, int total, int t
     if (hit) {
       const int l = __builtin_ctzll(hit);
       *b = base + l;
-      *row0 = (t - (__shfl(sum, l, 64) - __shfl(n, l, 64))) * WROWS;
+      *row0 = (t - (__shfl(sum, l, 64) - __shfl(n, l, 64))) * R;
       return true;
     }
     t -= __shfl(sum, 63, 64);
@@ -181,22 +186,6 @@ __device__ __forceinline__ int swz(int r) {
     return ((r & 3) << 2) | ((r >> 2) & 3);
 }
 
-// Copies TR rows of D elements from `base` (row stride `stride` elements) into LDS at `lds`, swizzled; rows >= rows_left
-// become zeros (the buffer range check).
-template <int D>
-__device__ __forceinline__ void stage(const bf16_t* base, long stride, long rows_left, unsigned lds, int wave, int lane) {
-  constexpr int CPR = D / 8;                 // 16-B chunks per row
-  constexpr int PIECES = TR * D * 2 / 1024;  // 1-KiB copies per tile
-  const i32x4 rs = make_rsrc(base, (unsigned)min(max(rows_left, 0L) * stride * 2, 0x7fffffffL));
-#pragma unroll
-  for (int i = 0; i < PIECES / 4; ++i) {
-    const int piece = wave * (PIECES / 4) + i;
-    const int pos = piece * 64 + lane;
-    const int row = pos / CPR, ch = (pos % CPR) ^ swz<D>(row);
-    blds16(rs, (unsigned)(row * stride * 2 + ch * 16), lds + piece * 1024);
-  }
-}
-
 // Fragments of the stationary rows: lane (row lq, half hh) holds elements 16 s + 8 hh .. + 7
 template <int D>
 __device__ __forceinline__ void load_frags(const bf16_t* row, int hh, bf16x8 (&f)[D / 16]) {
@@ -204,55 +193,19 @@ __device__ __forceinline__ void load_frags(const bf16_t* row, int hh, bf16x8 (&f
   for (int s = 0; s < D / 16; ++s) f[s] = *(const bf16x8*)(row + 16 * s + 8 * hh);
 }
 
-// LDS offsets of a lane's reads, relative to a 32-row half tile
+// Scores are made of the stationary rows with the scale's sign, and scaled by its magnitude (score_scale): the largest
+// product is the largest score, and a masked one, -inf, stays so. A scale of zero takes rows of zeros.
 template <int D>
-struct LaneOff {
-  int row[D / 16];  // row-wise: chunk 2 s + hh of row lq
-  int tr[2][D / 32];  // transposed: columns 32 dt .., rows 4 (G >> 1) + vq of an even / odd 8-row group
-  __device__ __forceinline__ LaneOff(int lane) {
-    const int lq = lane & 31, hh = lane >> 5;
+__device__ __forceinline__ void take_sign(bf16x8 (&f)[D / 16], float scale) {
+  const unsigned keep = scale == 0.f ? 0u : ~0u, flip = scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) row[s] = lq * D * 2 + (((2 * s + hh) ^ swz<D>(lq)) << 4);
-    const int G = lane >> 4, vq = (lane & 15) >> 2, vp = lane & 3;
-    const int r0 = 4 * (G >> 1) + vq;
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-      for (int o = 0; o < 2; ++o)
-        tr[o][dt] = (r0 + 8 * o) * D * 2 + (((4 * dt + 2 * (G & 1) + (vp >> 1)) ^ swz<D>(r0 + 8 * o)) << 4) + (vp & 1) * 8;
-  }
-};
-
-// acc[32 tile rows x 32 stationary rows] = tile rows . stationary rows
-template <int D>
-__device__ __forceinline__ f32x16 row_product(const char* half, const LaneOff<D>& o, const bf16x8 (&f)[D / 16]) {
-  f32x16 acc;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
-#pragma unroll
-  for (int s = 0; s < D / 16; ++s)
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(half + o.row[s]), f[s], acc, 0, 0, 0);
-  return acc;
-}
-
-// acc[D x 32 stationary rows] += (tile half)^T . m, m[32 tile rows x 32 stationary rows] in the accumulator layout
-template <int D>
-__device__ __forceinline__ void tr_product(const char* half, const LaneOff<D>& o, const f32x16& m, f32x16 (&acc)[D / 32]) {
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    // rounded to bf16 for the matrix unit (relative 2^-9); accumulators, P and dS themselves are fp32
-    bf16x8 b;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = (__bf16)m[8 * s + j];
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt) {
-      const s16x4 lo = ds_tr16(half + 16 * s * D * 2 + o.tr[0][dt]);
-      const s16x4 hi = ds_tr16(half + 16 * s * D * 2 + o.tr[1][dt]);
-      const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-      acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc[dt], 0, 0, 0);
-    }
+  for (int s = 0; s < D / 16; ++s) {
+    u32x4 w = __builtin_bit_cast(u32x4, f[s]);
+    w = (w & keep) ^ flip;
+    f[s] = __builtin_bit_cast(bf16x8, w);
   }
 }
+__device__ __forceinline__ float score_scale(float scale) { return scale == 0.f ? 1.f : fabsf(scale) * kLog2e; }
 
 // The lane's stationary row of acc[D x rows], times f: bf16 to `dst` (the row's start)
 template <int D>
@@ -283,12 +236,6 @@ __device__ __forceinline__ void store_part(float* dst, const f32x16 (&acc)[D / 3
           f32x4{acc[i][4 * r4] * f, acc[i][4 * r4 + 1] * f, acc[i][4 * r4 + 2] * f, acc[i][4 * r4 + 3] * f};
 }
 
-#define TILE_SYNC()                                  \
-  do {                                               \
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); \
-    __syncthreads();                                 \
-  } while (0)
-
 // Zeros (lse: -inf) in the rows before the first and behind the last sequence, by `blocks` workgroups of which this is
 // number i
 __device__ __forceinline__ void zero_outside(bf16_t* out, long row_stride, long head_stride, const int* cu, int B, int total,
@@ -301,93 +248,6 @@ __device__ __forceinline__ void zero_outside(bf16_t* out, long row_stride, long 
     *(u32x4*)(out + (long)row * row_stride + (long)h * head_stride + c) = u32x4{0u, 0u, 0u, 0u};
     if (lse != nullptr && c == 0) lse[(long)h * total + row] = -INFINITY;
   }
-}
-
-// ------------------------------------------------------------------------------------------------ forward
-template <int D>
-__global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const AttnTrainParams& p = d.p;
-  constexpr int TB = TR * D * 2;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int lq = lane & 31, hh = lane >> 5;
-  const int n_tiles = d.tiles_q * p.H;
-  if ((int)blockIdx.x >= n_tiles) {
-    zero_outside(p.o, p.o_row, p.o_head, p.cu_q, p.B, p.total_q, p.H, D, p.lse, blockIdx.x - n_tiles, gridDim.x - n_tiles);
-    return;
-  }
-  const int v = xcd_remap(blockIdx.x, n_tiles);
-  const int h = v / d.tiles_q;
-  int b, row0;
-  if (!find_tile(p.cu_q, p.B, p.total_q, v % d.tiles_q, &b, &row0)) return;
-  int q_start, q_len, k_start, k_len;
-  seq_range(p.cu_q, b, p.total_q, &q_start, &q_len);
-  seq_range(p.cu_k, b, p.total_k, &k_start, &k_len);
-  const int hk = h / (p.H / p.HK);
-  const int row = row0 + wave * 32 + lq;
-  const bool live = row < q_len;
-
-  bf16x8 qf[D / 16];
-  load_frags<D>(p.q + (long)(q_start + min(row, q_len - 1)) * p.q_row + (long)h * p.q_head, hh, qf);
-  const LaneOff<D> off(lane);
-  const unsigned lds0 = lds_addr_of(smem);
-  const bf16_t* kp = p.k + (long)k_start * p.k_row + (long)hk * p.k_head;
-  const bf16_t* vp = p.v + (long)k_start * p.v_row + (long)hk * p.v_head;
-  auto fetch = [&](int t, int buf) {
-    const long r = (long)t * TR;
-    stage<D>(kp + r * p.k_row, p.k_row, k_len - r, lds0 + buf * 2 * TB, wave, lane);
-    stage<D>(vp + r * p.v_row, p.v_row, k_len - r, lds0 + buf * 2 * TB + TB, wave, lane);
-  };
-  const float sl2 = p.scale * kLog2e;
-  float m = -INFINITY, l = 0.f;
-  f32x16 acc[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
-
-  const int nt = (k_len + TR - 1) / TR;
-  if (nt > 0) fetch(0, 0);
-  TILE_SYNC();
-  for (int t = 0; t < nt; ++t) {
-    if (t + 1 < nt) fetch(t + 1, (t + 1) & 1);
-    const char* kt = smem + (t & 1) * 2 * TB;
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      f32x16 s = row_product<D>(kt + hf * 32 * D * 2, off, qf);
-      float top = -INFINITY;
-      const int k_left = k_len - t * TR - hf * 32 - 4 * hh;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[r] = 8 * (r >> 2) + (r & 3) < k_left ? s[r] * sl2 : -INFINITY;
-        top = fmaxf(top, s[r]);
-      }
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float m_new = fmaxf(m, top);
-      if (__any(m_new > m)) {
-        const float alpha = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
-        l *= alpha;
-        m = m_new;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][r] *= alpha;
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        // a half tile without keys, before the first key, has m = -inf: its scores are -inf too
-        s[r] = s[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s[r] - m);
-        l += s[r];
-      }
-      tr_product<D>(kt + TB + hf * 32 * D * 2, off, s, acc);
-    }
-    TILE_SYNC();
-  }
-  l += __shfl_xor(l, 32, 64);
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no keys: zeros; NaN stays
-  store_row<D>(p.o + (long)(q_start + row) * p.o_row + (long)h * p.o_head, acc, inv, hh, live);
-  if (live && hh == 0)
-    p.lse[(long)h * p.total_q + q_start + row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 // ------------------------------------------------------------------------------------------------ backward
@@ -881,13 +741,14 @@ __device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char
       const long rc = k_start + min(row0 + pair * 64 + nb * 32 + lq, k_len - 1);
       load_frags<D>(wave & 1 ? p.v + rc * p.v_row + (long)hk * p.v_head : p.k + rc * p.k_row + (long)hk * p.k_head, hh,
                     f[nb]);
+      if (!(wave & 1)) take_sign<D>(f[nb], p.scale);
     }
     bf16x8 bc[2][2];  // P (wave 0) or dS (wave 1) of the stage that the tr phase takes, B operands
     u32x4 bn[2][2];   // of the next
     f32x16 s[2];
     RowAhead<D> ra;
     TrAhead<D> ta;
-    const float sl2 = p.scale * kLog2e;
+    const float sl2 = score_scale(p.scale);
     // P of stage j, fp16: [j & 1][pair][r4][block][lane] 8 B
     char* const xch = smem + L::X + pair * (L::PBYTES / 2) + lane * 8;
     auto none = [](int) {};
@@ -1092,6 +953,7 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
     for (int nb = 0; nb < 2; ++nb) {
       const long rc = q_start + min(row0 + pair * 64 + nb * 32 + lq, q_len - 1);
       load_frags<D>(p.q + rc * p.q_row + (long)h * p.q_head, hh, qf[nb]);
+      take_sign<D>(qf[nb], p.scale);
       load_frags<D>(p.dout + rc * p.do_row + (long)h * p.do_head, hh, df[nb]);
       lse[nb] = d.lse2[(long)h * p.total_q + rc];
       del[nb] = d.delta[(long)h * p.total_q + rc];
@@ -1104,7 +966,7 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
         asm volatile("" : "+a"(df[nb][s]));
       }
     asm volatile("s_nop 4" ::: "memory");
-    const float sl2 = p.scale * kLog2e;
+    const float sl2 = score_scale(p.scale);
     f32x16 sa[2], da[2], sb[2], db[2];
     // Half u of the 64 that make stage j's dS from its S and dP: element e = u >> 1 (block e >> 4, score e & 15); even
     // halves do an exp2 and the next one's argument, odd ones the product
@@ -1362,6 +1224,251 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(TrainDev d, JoinIte
   }
 }
 
+// ------------------------------------------------------------------------------------------------ forward
+// A workgroup owns 256 queries of one head, a wave 64 of them and both products: S = k . q^T row-wise, out^T = v^T . P
+// transposed, as a key workgroup's wave 0 does. P = 2^(S - m) with m the largest score of the query's first 32 keys: any m
+// will do while P and the sums stay in fp32's range, which they do up to S = m + 40 (bf16 rounds P to the same relative
+// 2^-9 there), so the accumulators are never scaled anew. Where a later score is larger still, the workgroup sweeps its
+// keys once more, with m the largest score of them all, which it then knows.
+template <int D>
+struct FwdLds {
+  static constexpr int E = D == 256 ? 1 : D == 128 ? 3 : 4;  // steps that a copy may take beyond its own
+  static constexpr int R = 3 + E, A = 0, B = R * Stage<D>::BYTES, FLAG = 2 * R * Stage<D>::BYTES, TOTAL = FLAG + 16;
+};
+
+template <int D>
+__global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const AttnTrainParams& p = d.p;
+  using L = FwdLds<D>;
+  constexpr int ND = D / 32, SB = Stage<D>::BYTES, P = Stage<D>::PIECES, E = L::E;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int lq = lane & 31, hh = lane >> 5;
+  const int n_units = d.tiles * p.H * d.most;
+  if ((int)blockIdx.x >= n_units) {
+    zero_outside(p.o, p.o_row, p.o_head, p.cu_q, p.B, p.total_q, p.H, D, p.lse, blockIdx.x - n_units, gridDim.x - n_units);
+    return;
+  }
+  int v = xcd_remap(blockIdx.x, n_units);
+  const int part = v % d.most;
+  v /= d.most;
+  const int h = v / d.tiles;
+  int b, row0;
+  if (!find_tile<256>(p.cu_q, p.B, p.total_q, v % d.tiles, &b, &row0)) return;
+  b = __builtin_amdgcn_readfirstlane(b);
+  row0 = __builtin_amdgcn_readfirstlane(row0);
+  int q_start, q_len, k_start, k_len;
+  seq_range(p.cu_q, b, p.total_q, &q_start, &q_len);
+  seq_range(p.cu_k, b, p.total_k, &k_start, &k_len);
+  const int hk = h / (p.H / p.HK);
+  const int all = (k_len + 31) / 32, ranges = ranges_of(all, d.stages, d.most);
+  if (part >= ranges) return;
+  const int per = (all + ranges - 1) / ranges, t0 = min(part * per, all), n = min(per, all - t0);
+
+  f32x16 acc[2][ND];
+  float m[2] = {-INFINITY, -INFINITY}, l[2], most[2] = {-INFINITY, -INFINITY};
+  bool again = false;
+  do {
+    acc_zero<ND>(acc);
+    l[0] = l[1] = 0.f;
+    if (n <= 0) break;
+    const unsigned lds0 = (unsigned)__builtin_amdgcn_readfirstlane((int)lds_addr_of(smem));
+    const unsigned wlds = lds0 + wave * 1024;
+    Stage<D> sk, sv;
+    sk.init(p.k_row, wave, lane);
+    sv.init(p.v_row, wave, lane);
+    Stream st_k, st_v;
+    st_k.init(p.k + (long)k_start * p.k_row + (long)hk * p.k_head, t0, all, k_len, n, p.k_row * 2, 0);
+    st_v.init(p.v + (long)k_start * p.v_row + (long)hk * p.v_head, t0, all, k_len, n, p.v_row * 2, 0);
+    i32x4 rk, rv;
+    int ri = 0;  // step mod R
+    // stages i + 3 + E of k and i + 2 + E of v: issued behind step i's barrier, in place E + 1 barriers later
+    auto open = [&]() {
+      rk = st_k.next();
+      rv = st_v.next();
+    };
+    auto copy = [&](int k) {
+      if (k < P)
+        copy16(rk, sk.src(k), wlds + L::A + ri * SB + sk.dst(k));
+      else if (k < 2 * P)
+        copy16(rv, sv.src(k - P), wlds + L::B + wrap<L::R>(ri - 1) * SB + sv.dst(k - P));
+    };
+    auto move = [&](int x) { return wrap<L::R>(x) == L::R - 1 ? (1 - L::R) * SB : SB; };
+#pragma unroll
+    for (int j = 0; j < L::R; ++j) {
+      rk = st_k.next();
+#pragma unroll
+      for (int k = 0; k < P; ++k) copy16(rk, sk.src(k), wlds + L::A + j * SB + sk.dst(k));
+    }
+#pragma unroll
+    for (int j = 0; j < L::R - 1; ++j) {
+      rv = st_v.next();
+#pragma unroll
+      for (int k = 0; k < P; ++k) copy16(rv, sv.src(k), wlds + L::B + j * SB + sv.dst(k));
+    }
+    bf16x8 f[2][D / 16];
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+      const long rc = q_start + min(row0 + wave * 64 + nb * 32 + lq, q_len - 1);
+      load_frags<D>(p.q + rc * p.q_row + (long)h * p.q_head, hh, f[nb]);
+      take_sign<D>(f[nb], p.scale);
+    }
+    const float sl2 = score_scale(p.scale);
+    bf16x8 bc[2][2];
+    u32x4 bn[2][2];
+    f32x16 s[2];
+    RowReader<D> rr;
+    TrReader<D> tr;
+    RowAhead<D> ra;
+    TrAhead<D> ta;
+    rr.init(lane, lds0 + L::A);
+    tr.init(lane, lds0 + L::B);
+    auto none = [](int) {};
+    auto nothing = []() {};
+    auto next = [&]() {
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) bc[nb][ks] = __builtin_bit_cast(bf16x8, bn[nb][ks]);
+    };
+    auto mask = [&](int j) {  // keys past the end of the sequence or the range
+      const int left = j < n ? k_len - (t0 + j) * 32 : 0;
+      if (left >= 32) return;
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[nb][r] = 8 * (r >> 2) + 4 * hh + (r & 3) < left ? s[nb][r] : -INFINITY;
+    };
+    // Softmax of a stage in 40 pieces: maxima of 4 scores (8), P of one score (32)
+    float sub[2], x;
+    auto arg = [&](int e) {
+      const int nb = (e >> 2) & 1, r = 4 * (e >> 3) + (e & 3);
+      x = __builtin_fmaf(s[nb][r], sl2, -sub[nb]);
+    };
+    auto maxima = [&](int u) {
+      const int nb = u >> 2, r = 4 * (u & 3);
+      most[nb] = fmaxf(most[nb], fmaxf(fmaxf(s[nb][r], s[nb][r + 1]), fmaxf(s[nb][r + 2], s[nb][r + 3])));
+    };
+    auto prob = [&](int e) {
+      const int nb = (e >> 2) & 1, r = 4 * (e >> 3) + (e & 3);
+      if (e == 0) arg(0);
+      s[nb][r] = __builtin_amdgcn_exp2f(x);
+      if (e < 31) arg(e + 1);
+      if (e > 0) {
+        const int e1 = e - 1, n1 = (e1 >> 2) & 1, r1 = 4 * (e1 >> 3) + (e1 & 3);
+        l[n1] += s[n1][r1];
+        if (r1 & 1) bn[n1][r1 >> 3][(r1 & 7) >> 1] = pack_bf(s[n1][r1 - 1], s[n1][r1]);
+      }
+      if (e == 31) {
+        l[nb] += s[nb][r];
+        bn[nb][r >> 3][(r & 7) >> 1] = pack_bf(s[nb][r - 1], s[nb][r]);
+      }
+    };
+    // largest score of the query: the lane halves hold different keys
+    auto both = [&](float v) {
+      const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+      return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+    };
+    step_sync();
+    ra.read(rr);
+    row_phase<D>(rr, ra, f, s, none, nothing);
+    mask(0);
+    if (!again) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) maxima(u);
+    }
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+      m[nb] = both(most[nb]) * sl2;
+      sub[nb] = m[nb] == -INFINITY ? 0.f : m[nb];  // only -inf scores so far: P = exp2(-inf) = 0
+    }
+#pragma unroll
+    for (int e = 0; e < 32; ++e) prob(e);
+    next();
+    rr.move(SB);  // k stage i + 1
+    ra.read(rr);
+    for (int i = 0; i < n; ++i) {
+      open();
+      row_phase<D>(rr, ra, f, s, none, [&]() { ta.read(tr); });
+      rr.move(move(ri + 1));
+      mask(i + 1);
+      step_sync<E * 2 * P>();
+      tr_phase<D>(
+          tr, ta, bc, acc,
+          [&](int k) {
+            constexpr int GAP = (4 * ND) / (2 * P);
+            if (k % GAP == 0 && k / GAP < 2 * P) copy(k / GAP);
+#pragma unroll
+            for (int u = share(k, 4 * ND, 40); u < share(k + 1, 4 * ND, 40); ++u) u < 8 ? maxima(u) : prob(u - 8);
+          },
+          [&]() { ra.read(rr); });
+      next();
+      tr.move(move(ri));
+      ri = wrap<L::R>(ri + 1);
+    }
+    // a score far above m in any wave (all copies land here, too: none may outlive the sweep)
+    const bool far = __any(both(most[0]) * sl2 > m[0] + 40.f || both(most[1]) * sl2 > m[1] + 40.f);
+    volatile LDS_AS unsigned char* flag = (volatile LDS_AS unsigned char*)(unsigned long)(lds0 + L::FLAG);
+    if (lane == 0) flag[wave] = far && !again;
+    step_sync();
+    again = (flag[0] | flag[1] | flag[2] | flag[3]) != 0;
+    step_sync();
+  } while (again);
+  acc_fence<ND>(acc);
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb) {
+    const int row = row0 + wave * 64 + nb * 32 + lq;
+    const bool live = row < q_len;
+    const long rc = q_start + min(row, q_len - 1);
+    const float sum = l[nb] + __shfl_xor(l[nb], 32, 64);  // the lane halves hold complementary keys
+    if (ranges > 1) {
+      store_part<D>(d.part_o + (((long)part * p.total_q + rc) * p.H + h) * D, acc[nb], 1.f, hh, live);
+      if (live && hh == 0) d.part_ml[((long)part * p.H + h) * p.total_q + rc] = make_float2(m[nb], sum);
+      continue;
+    }
+    store_row<D>(p.o + rc * p.o_row + (long)h * p.o_head, acc[nb], sum == 0.f ? 0.f : 1.f / sum, hh, live);
+    if (live && hh == 0) p.lse[(long)h * p.total_q + rc] = sum == 0.f ? -INFINITY : (m[nb] + log2f(sum)) * kLn2;
+  }
+}
+
+// Joins the ranges of rows that were cut: out and lse from their sums, in range order
+template <int D>
+__global__ __launch_bounds__(kThreads) void attn_lse_join_kernel(TrainDev d) {
+  const AttnTrainParams& p = d.p;
+  constexpr int LANES = D / 8;
+  const long item = ((long)blockIdx.x * kThreads + threadIdx.x) / LANES;
+  const int col = threadIdx.x % LANES * 8;
+  if (item >= (long)p.total_q * p.H) return;
+  const int row = (int)(item / p.H), h = (int)(item % p.H);
+  const int b = find_seq(p.cu_q, p.B, p.total_q, row);
+  if (b < 0) return;
+  int s, k_len;
+  seq_range(p.cu_k, b, p.total_k, &s, &k_len);
+  const int ranges = ranges_of((k_len + 31) / 32, d.stages, d.most);
+  if (ranges < 2) return;
+  const float2* ml = d.part_ml + (long)h * p.total_q + row;
+  const long ml_step = (long)p.H * p.total_q, step = (long)p.total_q * p.H * D;
+  float m = -INFINITY;
+  for (int i = 0; i < ranges; ++i) m = fmaxf(m, ml[i * ml_step].x);
+  const float sub = m == -INFINITY ? 0.f : m;
+  const float* src = d.part_o + item * D + col;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+  float sum = 0.f;
+  for (int i = 0; i < ranges; ++i) {
+    const float2 r = ml[i * ml_step];
+    const float w = __builtin_amdgcn_exp2f(r.x - sub);
+    sum += r.y * w;
+    x += *(const f32x4*)(src + i * step) * w;
+    y += *(const f32x4*)(src + i * step + 4) * w;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  x *= inv;
+  y *= inv;
+  *(u32x4*)(p.o + (long)row * p.o_row + (long)h * p.o_head + col) =
+      u32x4{pack2bf(x[0], x[1]), pack2bf(x[2], x[3]), pack2bf(y[0], y[1]), pack2bf(y[2], y[3])};
+  if (col == 0) p.lse[(long)h * p.total_q + row] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+}
+
 struct Plan {
   Cut q, k;
   long head_bytes, lse_bytes, qf_bytes, qp_bytes, kf_bytes, kp_bytes;  // kf, kp: dk and dv
@@ -1404,6 +1511,28 @@ Plan make_plan(const AttnTrainParams& p) {
   return x;
 }
 
+// The forward pass's ranges, from the average lengths: as long as a CU's share of the work, in sequences up to four times the
+// average, and none shorter than kFwdRange stages: a short batch of 512 keys takes 74 us in all in ranges of 8, 69 whole
+// (each range costs its start and its share of the join). A sequence of 7 queries and 3000 keys between longer ones: 101 us
+// whole, 59 + 6.5 in ranges.
+constexpr int kFwdRange = 16;
+struct FwdPlan {
+  int tiles, most, stages;
+  long o_bytes, ml_bytes;
+};
+FwdPlan make_fwd_plan(const AttnTrainParams& p) {
+  FwdPlan x;
+  x.tiles = p.total_q / 256 + p.B;
+  const double sweep = p.total_k / 32. / p.B, units = (double)x.tiles * p.H;
+  x.stages = (int)std::max((double)kFwdRange, std::min(units * sweep / kCus, 1e9));
+  const double longest = std::min(sweep * 4, sweep * p.B) / x.stages;
+  x.most = (int)std::max(1., std::min((double)kMaxRanges, longest));
+  auto pad = [](long n) { return (n + 255) / 256 * 256; };
+  x.o_bytes = x.most > 1 ? pad((long)x.most * p.total_q * p.H * p.dim * 4) : 0;
+  x.ml_bytes = x.most > 1 ? pad((long)x.most * p.total_q * p.H * 8) : 0;
+  return x;
+}
+
 int check(const AttnTrainParams& p) {
   FLITE_REQUIRE(p.dim == 64 || p.dim == 128 || p.dim == 256, "attention: head size must be 64, 128 or 256");
   FLITE_REQUIRE(p.B > 0 && p.H > 0 && p.HK > 0 && p.H % p.HK == 0,
@@ -1439,11 +1568,16 @@ constexpr int kZeroBlocks = 32;
 
 template <int D>
 int launch_fwd(const TrainDev& d, hipStream_t s) {
-  constexpr int lds = 4 * TR * D * 2;
+  constexpr int lds = FwdLds<D>::TOTAL;
   static std::atomic<unsigned long long> done{0};
   if (lds_limit(attn_lse_kernel<D>, lds, done)) return 1;
-  hipLaunchKernelGGL(attn_lse_kernel<D>, dim3(d.tiles_q * d.p.H + (d.p.zero_outside ? kZeroBlocks : 0)), dim3(kThreads), lds,
+  const AttnTrainParams& p = d.p;
+  hipLaunchKernelGGL(attn_lse_kernel<D>, dim3(d.tiles * p.H * d.most + (p.zero_outside ? kZeroBlocks : 0)), dim3(kThreads), lds,
                      s, d);
+  FLITE_HIP_CHECK(hipGetLastError());
+  if (d.most > 1)
+    hipLaunchKernelGGL(attn_lse_join_kernel<D>, dim3((unsigned)(((long)p.total_q * p.H * (D / 8) + kThreads - 1) / kThreads)),
+                       dim3(kThreads), 0, s, d);
   FLITE_HIP_CHECK(hipGetLastError());
   return 0;
 }
@@ -1479,7 +1613,13 @@ long attn_train_workspace_bytes(const AttnTrainParams& p) {
   return make_plan(p).total();
 }
 
-int attn_train_fwd(const AttnTrainParams& p, hipStream_t s) {
+long attn_train_fwd_workspace_bytes(const AttnTrainParams& p) {
+  if (check(p)) return -1;
+  const FwdPlan x = make_fwd_plan(p);
+  return x.o_bytes + x.ml_bytes;
+}
+
+int attn_train_fwd(const AttnTrainParams& p, void* ws, long ws_bytes, hipStream_t s) {
   if (int rc = check(p)) return rc;
   const bool any_q = p.total_q > 0, any_k = p.total_k > 0;
   if (int rc = check_rows(p.q, p.q_row, p.q_head, p.dim, any_q, "q")) return rc;
@@ -1488,9 +1628,16 @@ int attn_train_fwd(const AttnTrainParams& p, hipStream_t s) {
   if (int rc = check_rows(p.o, p.o_row, p.o_head, p.dim, any_q, "out")) return rc;
   FLITE_REQUIRE(p.lse || !any_q, "attention: missing lse");
   if (!any_q) return 0;
+  const FwdPlan x = make_fwd_plan(p);
+  FLITE_REQUIRE(x.most == 1 || (ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= x.o_bytes + x.ml_bytes),
+                "attention: workspace missing, not 256-byte aligned, or too small");
   TrainDev d{};
   d.p = p;
-  d.tiles_q = p.total_q / WROWS + p.B;
+  d.tiles = x.tiles;
+  d.most = x.most;
+  d.stages = x.stages;
+  d.part_o = (float*)ws;
+  d.part_ml = (float2*)((char*)ws + x.o_bytes);
   if (p.dim == 64) return launch_fwd<64>(d, s);
   if (p.dim == 128) return launch_fwd<128>(d, s);
   return launch_fwd<256>(d, s);

@@ -218,9 +218,17 @@ static AttnTrainParams attn_train_params(const flite_attn_train& a) {
   return p;
 }
 
-int flite_attn_lse_fwd(void* stream, const flite_attn_train* args) {
+long flite_attn_lse_fwd_workspace_bytes(const flite_attn_train* args) {
+  if (args == nullptr) {
+    set_last_error("flite: flite_attn_lse_fwd_workspace_bytes: null argument");
+    return -1;
+  }
+  return attn_train_fwd_workspace_bytes(attn_train_params(*args));
+}
+
+int flite_attn_lse_fwd(void* stream, const flite_attn_train* args, void* workspace, long workspace_bytes) {
   FLITE_REQUIRE(args, "flite_attn_lse_fwd: null argument");
-  return attn_train_fwd(attn_train_params(*args), (hipStream_t)stream);
+  return attn_train_fwd(attn_train_params(*args), workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 long flite_attn_lse_bwd_workspace_bytes(const flite_attn_train* args) {

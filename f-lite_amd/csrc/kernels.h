@@ -133,8 +133,9 @@ struct AttnTrainParams {
   float scale = 1.f;
   int zero_outside = 0;  // 1: rows that no sequence covers become zeros (lse: -inf); 0: they stay as they were
 };
-int attn_train_fwd(const AttnTrainParams& p, hipStream_t s);
-long attn_train_workspace_bytes(const AttnTrainParams& p);  // -1: the sizes are refused
+long attn_train_fwd_workspace_bytes(const AttnTrainParams& p);  // -1: the sizes are refused; 0: none is needed
+int attn_train_fwd(const AttnTrainParams& p, void* ws, long ws_bytes, hipStream_t s);
+long attn_train_workspace_bytes(const AttnTrainParams& p);  // the backward pass's
 int attn_train_bwd(const AttnTrainParams& p, void* ws, long ws_bytes, hipStream_t s);
 
 }  // namespace flite

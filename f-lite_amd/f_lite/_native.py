@@ -110,7 +110,8 @@ SIGNATURES = {
                                       _f, _vp, _l]),
     "flite_rmsnorm_modulate": (_i, [_vp, _vp, _i, _l, _vp, _l, _vp, _vp, _vp, _l, _l, _l, _i, _f]),
     "flite_rope_qknorm": (_i, [_vp, _vp, _l, _l, _i, _i, _vp, _vp, _l, _f]),
-    "flite_attn_lse_fwd": (_i, [_vp, _vp]),
+    "flite_attn_lse_fwd_workspace_bytes": (_l, [_vp]),
+    "flite_attn_lse_fwd": (_i, [_vp, _vp, _vp, _l]),
     "flite_attn_lse_bwd_workspace_bytes": (_l, [_vp]),
     "flite_attn_lse_bwd": (_i, [_vp, _vp, _vp, _l]),
     "flite_rope_axes_fwd": (_i, [_vp, _vp]),
@@ -609,7 +610,11 @@ def attn_varlen_lse(q, k, v, cu_q, cu_k, scale, out=None, lse=None):
     po, o0, o1 = _heads("out", out, torch.bfloat16, q.shape)
     args = _ATTN_TRAIN.pack(pq, pk, pv, po, _lse_ptr(lse, h, n), 0, 0, 0, 0, q0, q1, k0, k1, v0, v1, o0, o1, 0, 0, 0, 0,
                             0, 0, 0, 0, cu_q.data_ptr(), cu_k.data_ptr(), b, h, hk, d, n, nk, scale, new)
-    _call(dev, "flite_attn_lse_fwd", args)
+    size = (_lib or load()).flite_attn_lse_fwd_workspace_bytes(args)
+    if size < 0:
+        check(2, "flite_attn_lse_fwd_workspace_bytes")
+    ws = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
+    _call(dev, "flite_attn_lse_fwd", args, _ptr(ws), size)
     return out, lse
 
 

@@ -156,9 +156,10 @@ typedef struct flite_attn_train {
   int zero_outside;     /* rows outside all sequences: 1 = zeros in the outputs (lse: -inf), 0 = they stay as they are */
 } flite_attn_train;
 
-/* Writes out and lse. Training counterpart of
- * flash_attn_varlen_func (reference f_lite/model.py:203-210). */
-int flite_attn_lse_fwd(void* stream, const flite_attn_train* args);
+/* Workspace of the forward pass for these sizes (256-byte aligned device memory; 0: none); -1: the sizes are refused. */
+long flite_attn_lse_fwd_workspace_bytes(const flite_attn_train* args);
+/* Writes out and lse. Training counterpart of flash_attn_varlen_func (reference f_lite/model.py:203-210). */
+int flite_attn_lse_fwd(void* stream, const flite_attn_train* args, void* workspace, long workspace_bytes);
 /* Workspace of the backward pass for these sizes (256-byte aligned device memory); -1: the sizes are refused. */
 long flite_attn_lse_bwd_workspace_bytes(const flite_attn_train* args);
 /* dq, dk, dv of sum(out * dout), with the probabilities made again from q, k and lse. */

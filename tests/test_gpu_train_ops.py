@@ -54,15 +54,15 @@ def cu_of(lens, first=0):
 
 
 # ------------------------------------------------------------------------------------------------ attention
-def attn_ref(q, k, v, do, ql, kl, scale, q_first=0, k_first=0):
-    """out, lse, dq, dk, dv in 64 bits and an elementwise bound for each; rows outside stay 0 (lse -inf)."""
+def attn_ref(q, k, v, do, ql, kl, scale, q_first=0, k_first=0, f=F):
+    """out, lse, dq, dk, dv in 64 bits and an elementwise bound for each, with P off by f; rows outside stay 0 (lse -inf)."""
     n, h, d = q.shape
     hk = k.shape[1]
     Q, K, V, DO = (x.double() for x in (q, k, v, do))
     ref = {x: torch.zeros_like(t) for x, t in (("out", Q), ("dq", Q), ("dk", K), ("dv", V))}
     tol = {x: torch.zeros_like(t) for x, t in ref.items()}
     ref["lse"] = torch.full((h, n), -math.inf, device=DEV, dtype=torch.float64)
-    tol["lse"] = torch.full_like(ref["lse"], 2 * F)
+    tol["lse"] = torch.full_like(ref["lse"], 2 * f)
     a, b = q_first, k_first
     for nq, nk in zip(ql, kl):
         for i in range(h if nq and nk else 0):
@@ -75,20 +75,20 @@ def attn_ref(q, k, v, do, ql, kl, scale, q_first=0, k_first=0):
             o = p @ vi
             ref["lse"][i, qs] = lse[:, 0]
             ref["out"][qs, i] = o
-            o_err = U * o.abs() + (U + 3 * F) * (p @ vi.abs())
+            o_err = U * o.abs() + (U + 3 * f) * (p @ vi.abs())
             tol["out"][qs, i] = o_err
             dp = di @ vi.T
             delta = (di * o).sum(1, keepdim=True)
             ds = p * (dp - delta)
             d_err = (di.abs() * o_err).sum(1, keepdim=True)  # delta is made from the rounded out
             # dS: one rounding, the error of P, and that of dP - delta
-            ds_err = U * ds.abs() + 3 * F * p * (di.abs() @ vi.abs().T + delta.abs()) + p * d_err
+            ds_err = U * ds.abs() + 3 * f * p * (di.abs() @ vi.abs().T + delta.abs()) + p * d_err
             ref["dq"][qs, i] = scale * ds @ ki
-            tol["dq"][qs, i] = scale * ds_err @ ki.abs()
+            tol["dq"][qs, i] = abs(scale) * ds_err @ ki.abs()
             ref["dk"][ks, j] += scale * ds.T @ qi
-            tol["dk"][ks, j] += scale * ds_err.T @ qi.abs()
+            tol["dk"][ks, j] += abs(scale) * ds_err.T @ qi.abs()
             ref["dv"][ks, j] += p.T @ di
-            tol["dv"][ks, j] += (U + 3 * F) * (p.T @ di.abs())
+            tol["dv"][ks, j] += (U + 3 * f) * (p.T @ di.abs())
         a, b = a + nq, b + nk
     for x in ("dq", "dk", "dv"):
         tol[x] += U * ref[x].abs()
@@ -107,6 +107,10 @@ ATTN = [
     (128, 8, 1, [140], [70]),
     (64, 6, 2, [65, 1, 1, 190], [1, 130, 600, 31]),
     (64, 1, 1, [1], [2000]),   # one query over a long context: the sweep is cut and joined
+    (256, 2, 1, [9, 0, 130], [2500, 40, 33]),
+    (128, 4, 1, [257, 3], [1100, 1025]),
+    (64, 2, 2, [3000], [1600]),
+    (64, 2, 1, [1, 3, 0, 2] * 25, [2, 0, 5, 40] * 25),  # more sequences than a wave has lanes
     (64, 4, 4, [1500], [3]),
     (256, 12, 12, [700], [77]),
 ]
@@ -195,6 +199,26 @@ def test_attention_far_scores(d, sign):
     for x, g in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *grads)):
         assert torch.isfinite(g).all(), x
         close(g, ref[x], tol[x] * (1 + p_err[x] / U) + slack * F * (abs(ref[x]) if x == "lse" else 1e-9), x)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("scale", [1.0, -1.0, 0.0])
+def test_attention_scores_that_grow(d, scale):
+    """The largest score of some queries comes late and is far above the first ones (up to e^300); a negative scale turns
+    the order round, with a scale of zero all keys count alike."""
+    ql, kl = [70, 300], [500, 129]
+    q, k, v, do = attn_inputs(d, 2, 1, ql, kl, seed=12)
+    q, k = (q.float() * 0.05).to(BF), (k.float() * 0.05).to(BF)
+    q[..., 0] = 4.0
+    k[..., 0] = 0.0
+    k[400:, :, 0], k[490:, :, 0], k[600:, :, 0] = 40.0, 75.0, -30.0
+    cq, ck = cu_of(ql), cu_of(kl)
+    # scores of up to 300, one product of 300 and small ones that sum to under 2: off by at most d * 2^-24 * 302
+    ref, tol = attn_ref(q, k, v, do, ql, kl, scale, f=F + d * 2.0 ** -24 * 302)
+    out, lse = nat.attn_varlen_lse(q, k, v, cq, ck, scale)
+    grads = nat.attn_varlen_bwd(do, q, k, v, out, lse, cq, ck, scale)
+    for x, g in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *grads)):
+        close(g, ref[x], tol[x], x)
 
 
 def test_attention_gradients_against_differences():

@@ -47,7 +47,7 @@ BAD_ATTN_BWD = [(dict(dout=None), b"missing dout"), (dict(dq=None), b"missing dq
 
 @pytest.mark.parametrize("kw,msg", BAD_ATTN)
 def test_attention_forward_refuses(lib, kw, msg):
-    assert lib.flite_attn_lse_fwd(None, ctypes.byref(attn_args(**kw))) != 0
+    assert lib.flite_attn_lse_fwd(None, ctypes.byref(attn_args(**kw)), PTR, 1 << 40) != 0
     assert msg in lib.flite_last_error()
 
 
@@ -65,7 +65,15 @@ def test_attention_workspace(lib):
         assert b"workspace" in lib.flite_last_error()
     assert lib.flite_attn_lse_bwd_workspace_bytes(ctypes.byref(attn_args(head_dim=80))) == -1
     assert lib.flite_attn_lse_bwd_workspace_bytes(None) == -1
-    assert lib.flite_attn_lse_fwd(None, None) != 0 and lib.flite_attn_lse_bwd(None, None, None, 0) != 0
+    assert lib.flite_attn_lse_fwd_workspace_bytes(None) == -1
+    # one query over many keys: the sweep is cut
+    long_sweep = attn_args(total_q=1, total_k=8192)
+    n = lib.flite_attn_lse_fwd_workspace_bytes(ctypes.byref(long_sweep))
+    assert n > 0
+    for ws, size in ((None, 1 << 40), (PTR, n - 1), (PTR + 16, 1 << 40)):
+        assert lib.flite_attn_lse_fwd(None, ctypes.byref(long_sweep), ws, size) != 0
+        assert b"workspace" in lib.flite_last_error()
+    assert lib.flite_attn_lse_fwd(None, None, None, 0) != 0 and lib.flite_attn_lse_bwd(None, None, None, 0) != 0
 
 
 def rope_args(**kw):
