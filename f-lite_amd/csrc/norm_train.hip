@@ -8,7 +8,9 @@
 //   dshift[seg] = S0, dscale[seg] = w * S1 + b * S0, dw = sum_seg (1 + scale) * S1, db = sum_seg (1 + scale) * S0.
 //
 // Bound by HBM: x and dy are read once (mean and rstd are made again from the row in registers, so the forward pass
-// keeps nothing), dx is written once. One thread holds 8 consecutive columns of a row (16-B bf16 accesses).
+// keeps nothing), dx is written once. A wave holds a row of up to 3072 columns, 8 consecutive ones a lane and chunk (16-B
+// bf16 accesses), so that its sums need neither LDS nor barriers; longer rows take two or four waves. A workgroup of four
+// waves walks over a strip of rows, the next row of each wave on its way, and keeps what the rows share in LDS.
 #include <math.h>
 
 #include <algorithm>
@@ -20,13 +22,15 @@ namespace flite {
 
 namespace {
 
-constexpr int kMaxThreads = 512;  // threads per row: 8 columns each, so one pass covers 4096 columns
+constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxDim = 8192;
+constexpr int kFwdStrips = 1024, kBwdStrips = 512, kBwdRows = 8;
 
 struct NormTrainDev {
   NormTrainParams p;
-  int strips;      // row strips per segment (backward)
+  int strips;      // row strips per segment
   int strip_rows;  // rows per strip
+  int row_waves;   // waves per row: 1, 2 or 4
 };
 
 template <bool BF>
@@ -48,6 +52,27 @@ __device__ __forceinline__ void load8(const void* base, long off, float (&v)[8])
   }
 }
 
+// Eight values as they lie in memory
+template <bool BF>
+struct Raw8 {
+  u32x4 w[BF ? 1 : 2];
+  __device__ __forceinline__ void load(const void* base, long off) {
+    const char* at = (const char*)base + off * (BF ? 2 : 4);
+    w[0] = *(const u32x4*)at;
+    if constexpr (!BF) w[1] = *(const u32x4*)(at + 16);
+  }
+  __device__ __forceinline__ void zero() {
+    w[0] = u32x4{0, 0, 0, 0};
+    if constexpr (!BF) w[1] = w[0];
+  }
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (BF)
+      return __uint_as_float(j & 1 ? w[0][j >> 1] & 0xffff0000u : w[0][j >> 1] << 16);
+    else
+      return __uint_as_float(w[j >> 2][j & 3]);
+  }
+};
+
 template <bool BF>
 __device__ __forceinline__ void store8(void* base, long off, const float (&v)[8]) {
   if constexpr (BF) {
@@ -61,191 +86,315 @@ __device__ __forceinline__ void store8(void* base, long off, const float (&v)[8]
   }
 }
 
-// Sums of N values over the row's threads (all of the workgroup), the same on every thread: a wave sum, then one LDS
-// slot per wave. `buf` holds N * 8 floats; consecutive calls alternate between two of them, so one barrier per call
-// is enough (a wave can be at most one call ahead of the slowest reader).
+// Sum over a wave, the same on every lane: neighbours, pairs, quads and rows of 16 by lane moves of the vector unit (a
+// shuffle through LDS takes several times as long)
+template <int CTRL>
+__device__ __forceinline__ float lanes(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float sum64(float v) {
+  v += lanes<0xB1>(v);   // lane ^ 1
+  v += lanes<0x4E>(v);   // lane ^ 2
+  v += lanes<0x141>(v);  // mirrored within 8
+  v += lanes<0x140>(v);  // mirrored within 16
+  auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+
+// A thread's place: its row group of the workgroup, its place in the row
+struct Place {
+  int group, groups, t, threads;  // threads: per row
+  __device__ __forceinline__ Place(int row_waves) {
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    groups = kWaves / row_waves;
+    group = wave / row_waves;
+    threads = 64 * row_waves;
+    t = threadIdx.x - group * threads;
+  }
+  __device__ __forceinline__ int col(int c) const { return (c * threads + t) * 8; }
+};
+
+// Sums of N values over the row's threads, the same on each. Rows of several waves go through N LDS slots a wave;
+// consecutive calls alternate between two buffers, so one barrier per call is enough (a wave can be at most one call ahead
+// of the slowest reader). All waves of the workgroup make the same calls.
 template <int N>
-__device__ __forceinline__ void row_sums(float (&v)[N], float* buf, int waves) {
+__device__ __forceinline__ void row_sums(float (&v)[N], float* buf, int row_waves) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
-  if (waves == 1) return;
-  const int wave = threadIdx.x >> 6;
+  for (int i = 0; i < N; ++i) v[i] = sum64(v[i]);
+  if (row_waves == 1) return;
+  const int wave = threadIdx.x >> 6, first = wave & ~(row_waves - 1);
   if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) buf[i * 8 + wave] = v[i];
+    for (int i = 0; i < N; ++i) buf[wave * N + i] = v[i];
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float s = 0.f;
-    for (int w = 0; w < waves; ++w) s += buf[i * 8 + w];
-    v[i] = s;
-  }
+  for (int i = 0; i < N; ++i) v[i] = 0.f;
+  for (int w = 0; w < row_waves; ++w)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += buf[(first + w) * N + i];
 }
 
-// ---- forward: one workgroup per row (D <= 512: one wave) ----
-template <bool XBF, int NCH>
-__global__ __launch_bounds__(kMaxThreads) void layernorm_mod_kernel(NormTrainParams p) {
-  __shared__ float buf[2][8];
-  const int waves = blockDim.x >> 6;
-  const long row = blockIdx.x;
-  const long seg = p.seg_rows > 0 ? row / p.seg_rows : 0;
-  float x[NCH][8];
-  float s[1] = {0.f};
-#pragma unroll
-  for (int c = 0; c < NCH; ++c) {
-    const int col = (c * blockDim.x + threadIdx.x) * 8;
-    if (col < p.D) {
-      load8<XBF>(p.x, row * p.ldx + col, x[c]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[c][j] = 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s[0] += x[c][j];
+// Eight columns of a table in LDS: two planes of 16 B a lane, without bank conflicts
+struct Table {
+  float* base;
+  int threads, t;
+  __device__ __forceinline__ f32x4* at(int c, int half) const { return (f32x4*)base + (2 * c + half) * threads + t; }
+  __device__ __forceinline__ void put(int c, const float (&v)[8]) const {
+    *at(c, 0) = f32x4{v[0], v[1], v[2], v[3]};
+    *at(c, 1) = f32x4{v[4], v[5], v[6], v[7]};
   }
-  row_sums<1>(s, buf[0], waves);
-  const float mean = s[0] / (float)p.D;
-  s[0] = 0.f;
+  __device__ __forceinline__ void get(int c, float (&v)[8]) const {
+    const f32x4 a = *at(c, 0), b = *at(c, 1);
 #pragma unroll
-  for (int c = 0; c < NCH; ++c) {
-    const bool live = (c * (int)blockDim.x + (int)threadIdx.x) * 8 < p.D;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[c][j] = live ? x[c][j] - mean : 0.f;
-      s[0] += x[c][j] * x[c][j];
+    for (int j = 0; j < 4; ++j) {
+      v[j] = a[j];
+      v[4 + j] = b[j];
     }
   }
-  row_sums<1>(s, buf[1], waves);
-  const float r = 1.f / sqrtf(s[0] / (float)p.D + p.eps);
-#pragma unroll
-  for (int c = 0; c < NCH; ++c) {
-    const int col = (c * blockDim.x + threadIdx.x) * 8;
-    if (col >= p.D) continue;
-    float a[8], y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = x[c][j] * r;
-    if (p.w) {
-      load8<true>(p.w, col, a);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] *= a[j];
-    }
-    if (p.b) {
-      load8<true>(p.b, col, a);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] += a[j];
-    }
-    if (p.scale) {
-      load8<false>(p.scale, seg * p.mod_seg_stride + col, a);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] *= 1.f + a[j];
-    }
-    if (p.shift) {
-      load8<false>(p.shift, seg * p.mod_seg_stride + col, a);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] += a[j];
-    }
-    store8<true>(p.y, row * p.ldy + col, y);
-  }
-}
+};
 
-// ---- backward: one workgroup per strip of rows of one segment; S0 and S1 of the strip to the workspace ----
-template <bool XBF, bool RMS, int NCH, bool SUMS>
-__global__ __launch_bounds__(kMaxThreads) void norm_bwd_kernel(NormTrainDev d) {
-  const NormTrainParams& p = d.p;
-  __shared__ float buf[2][3 * 8];
-  const int waves = blockDim.x >> 6;
-  const int strip = blockIdx.x % d.strips;
-  const long seg = blockIdx.x / d.strips;
-  const long seg_rows = p.seg_rows > 0 ? p.seg_rows : p.rows;
-  const long seg_end = min((seg + 1) * seg_rows, p.rows);
-  const long r0 = seg * seg_rows + (long)strip * d.strip_rows;
-  const long r1 = min(r0 + d.strip_rows, seg_end);
+// Rows r0 .. r1 of the workgroup's strip
+struct Strip {
+  long seg, r0, r1;
+  __device__ __forceinline__ explicit Strip(const NormTrainDev& d) {
+    const NormTrainParams& p = d.p;
+    seg = blockIdx.x / d.strips;
+    const long seg_rows = p.seg_rows > 0 ? p.seg_rows : p.rows;
+    r0 = seg * seg_rows + (long)(blockIdx.x % d.strips) * d.strip_rows;
+    r1 = min(min(r0 + d.strip_rows, (seg + 1) * seg_rows), p.rows);
+  }
+};
 
-  float a[NCH][8], s0[NCH][8], s1[NCH][8];
+// a = w (1 + scale) of the eight columns at col
+__device__ __forceinline__ void factor8(const NormTrainParams& p, long seg, int col, float (&a)[8]) {
 #pragma unroll
-  for (int c = 0; c < NCH; ++c) {
-    const int col = (c * blockDim.x + threadIdx.x) * 8;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      a[c][j] = 1.f;
-      s0[c][j] = s1[c][j] = 0.f;
-    }
-    if (col >= p.D) continue;
+  for (int j = 0; j < 8; ++j) a[j] = 1.f;
+  if (p.w) load8<true>(p.w, col, a);
+  if (p.scale) {
     float t[8];
-    if (p.w) load8<true>(p.w, col, a[c]);
-    if (p.scale) {
-      load8<false>(p.scale, seg * p.mod_seg_stride + col, t);
+    load8<false>(p.scale, seg * p.mod_seg_stride + col, t);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a[c][j] *= 1.f + t[j];
-    }
+    for (int j = 0; j < 8; ++j) a[j] *= 1.f + t[j];
   }
-  const float inv_d = 1.f / (float)p.D;
-  for (long row = r0; row < r1; ++row) {
-    float x[NCH][8], dy[NCH][8];
-    float mean = 0.f;
+}
+
+// ---- forward: y = n a + c with a = w (1 + scale) and c = b (1 + scale) + shift of the segment ----
+template <bool XBF, int NCH>
+__global__ __launch_bounds__(kThreads) void layernorm_mod_kernel(NormTrainDev d) {
+  extern __shared__ __attribute__((aligned(16))) float smem[];
+  __shared__ float buf[2][kWaves];
+  const NormTrainParams& p = d.p;
+  const Place at(d.row_waves);
+  const Strip st(d);
+  if (st.r0 >= st.r1) return;
+  const Table ta{smem, at.threads, at.t}, tc{smem + at.threads * NCH * 8, at.threads, at.t};
+
+  Raw8<XBF> nx[NCH];
+  auto fetch = [&](long row) {
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const int col = (c * blockDim.x + threadIdx.x) * 8;
-      if (col < p.D) {
-        load8<XBF>(p.x, row * p.ldx + col, x[c]);
-        load8<true>(p.dy, row * p.lddy + col, dy[c]);
-      } else {
+      if (at.col(c) < p.D)
+        nx[c].load(p.x, row * p.ldx + at.col(c));
+      else
+        nx[c].zero();
+    }
+  };
+  fetch(min(st.r0 + at.group, st.r1 - 1));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[c][j] = dy[c][j] = 0.f;
+  for (int c = 0; c < NCH; ++c) {
+    const int col = at.col(c);
+    if (c % at.groups != at.group || col >= p.D) continue;  // the groups share the work
+    float a[8], b[8], t[8];
+    factor8(p, st.seg, col, a);
+    ta.put(c, a);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = 0.f;
+    if (p.b) {
+      load8<true>(p.b, col, b);
+      if (p.scale) {
+        load8<false>(p.scale, st.seg * p.mod_seg_stride + col, t);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] *= 1.f + t[j];
       }
     }
+    if (p.shift) {
+      load8<false>(p.shift, st.seg * p.mod_seg_stride + col, t);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b[j] += t[j];
+    }
+    tc.put(c, b);
+  }
+  __syncthreads();
+  const float inv_d = 1.f / (float)p.D;
+  for (long first = st.r0; first < st.r1; first += at.groups) {
+    const long row = first + at.group;
+    Raw8<XBF> x[NCH];
+    float s[1] = {0.f};
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      x[c] = nx[c];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[0] += x[c].get(j);
+    }
+    if (first + at.groups < st.r1) fetch(min(row + at.groups, st.r1 - 1));
+    row_sums<1>(s, buf[0], d.row_waves);
+    const float mean = s[0] * inv_d;
+    s[0] = 0.f;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const bool live = at.col(c) < p.D;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float v = live ? x[c].get(j) - mean : 0.f;
+        s[0] += v * v;
+      }
+    }
+    row_sums<1>(s, buf[1], d.row_waves);
+    const float r = 1.f / sqrtf(s[0] * inv_d + p.eps);
+    if (row >= st.r1) continue;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      if (at.col(c) >= p.D) continue;
+      float a[8], b[8], y[8];
+      ta.get(c, a);
+      tc.get(c, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = (x[c].get(j) - mean) * r * a[j] + b[j];
+      store8<true>(p.y, row * p.ldy + at.col(c), y);
+    }
+  }
+}
+
+// ---- backward: S0 and S1 of the strip to the workspace ----
+template <bool XBF, bool RMS, int NCH, bool SUMS>
+__global__ __launch_bounds__(kThreads, XBF ? 2 : 1) void norm_bwd_kernel(NormTrainDev d) {
+  extern __shared__ __attribute__((aligned(16))) float smem[];
+  __shared__ float buf[2][kWaves * 3];
+  const NormTrainParams& p = d.p;
+  const Place at(d.row_waves);
+  const Strip st(d);
+  const Table ta{smem, at.threads, at.t};
+
+  Raw8<XBF> nx[NCH];
+  Raw8<true> ndy[NCH];
+  auto fetch = [&](long row) {
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      if (at.col(c) < p.D) {
+        nx[c].load(p.x, row * p.ldx + at.col(c));
+        ndy[c].load(p.dy, row * p.lddy + at.col(c));
+      } else {
+        nx[c].zero();
+        ndy[c].zero();
+      }
+    }
+  };
+  if (st.r0 < st.r1) fetch(min(st.r0 + at.group, st.r1 - 1));
+  float s0[NCH][8], s1[NCH][8];
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s0[c][j] = s1[c][j] = 0.f;
+    if (c % at.groups != at.group || at.col(c) >= p.D) continue;  // the groups share the work
+    float a[8];
+    factor8(p, st.seg, at.col(c), a);
+    ta.put(c, a);
+  }
+  __syncthreads();
+  const float inv_d = 1.f / (float)p.D;
+  int turn = 0;
+  for (long first = st.r0; first < st.r1; first += at.groups) {
+    const long row = first + at.group;
+    Raw8<XBF> x[NCH];
+    Raw8<true> dy[NCH];
+    float mean = 0.f, m[1] = {0.f};
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      x[c] = nx[c];
+      dy[c] = ndy[c];
+      if constexpr (!RMS) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m[0] += x[c].get(j);
+      }
+    }
+    if (first + at.groups < st.r1) fetch(min(row + at.groups, st.r1 - 1));
     if constexpr (!RMS) {
-      float s[1] = {0.f};
-#pragma unroll
-      for (int c = 0; c < NCH; ++c)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[0] += x[c][j];
-      row_sums<1>(s, buf[0], waves);
-      mean = s[0] * inv_d;
+      row_sums<1>(m, buf[turn], d.row_waves);
+      turn ^= 1;
+      mean = m[0] * inv_d;
     }
     float s[3] = {0.f, 0.f, 0.f};  // sum (x - mean)^2, sum g, sum g (x - mean)
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const bool live = (c * (int)blockDim.x + (int)threadIdx.x) * 8 < p.D;
+      const bool live = at.col(c) < p.D;
+      float a[8];
+      if (live) {
+        ta.get(c, a);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if constexpr (!RMS) x[c][j] = live ? x[c][j] - mean : 0.f;
-        const float g = dy[c][j] * a[c][j];
-        s[0] += x[c][j] * x[c][j];
-        s[1] += g;
-        s[2] += g * x[c][j];
+        for (int j = 0; j < 8; ++j) {
+          const float v = x[c].get(j) - mean;
+          const float g = dy[c].get(j) * a[j];
+          s[0] += v * v;
+          if constexpr (!RMS) s[1] += g;
+          s[2] += g * v;
+        }
       }
     }
-    row_sums<3>(s, buf[RMS ? (int)(row & 1) : 1], waves);
+    row_sums<3>(s, buf[turn], d.row_waves);
+    turn ^= 1;
+    if (row >= st.r1) continue;
     const float r = 1.f / sqrtf(s[0] * inv_d + p.eps);
     const float c1 = RMS ? 0.f : s[1] * inv_d;
     const float c2 = s[2] * inv_d * r;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const int col = (c * blockDim.x + threadIdx.x) * 8;
-      if (col >= p.D) continue;
-      float o[8];
+      if (at.col(c) >= p.D) continue;
+      float a[8], o[8];
+      ta.get(c, a);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float n = x[c][j] * r;
+        const float n = (x[c].get(j) - mean) * r, g = dy[c].get(j);
         if constexpr (SUMS) {
-          s0[c][j] += dy[c][j];
-          s1[c][j] += dy[c][j] * n;
+          s0[c][j] += g;
+          s1[c][j] += g * n;
         }
-        o[j] = r * (dy[c][j] * a[c][j] - c1 - n * c2);
+        o[j] = r * (g * a[j] - c1 - n * c2);
       }
-      store8<XBF>(p.dx, row * p.lddx + col, o);
+      store8<XBF>(p.dx, row * p.lddx + at.col(c), o);
     }
   }
   if constexpr (SUMS) {
+    // the groups' sums, in group order, through the table's place
+    for (int g = 1; g < at.groups; ++g) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        __syncthreads();
+        if (at.group == g) {
+#pragma unroll
+          for (int c = 0; c < NCH; ++c) ta.put(c, k ? s1[c] : s0[c]);
+        }
+        __syncthreads();
+        if (at.group == 0) {
+#pragma unroll
+          for (int c = 0; c < NCH; ++c) {
+            float v[8];
+            ta.get(c, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) (k ? s1[c][j] : s0[c][j]) += v[j];
+          }
+        }
+      }
+    }
+    if (at.group != 0) return;
     float* ws = p.ws + (long)blockIdx.x * 2 * p.D;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const int col = (c * blockDim.x + threadIdx.x) * 8;
-      if (col >= p.D) continue;
-      store8<false>(ws, col, s0[c]);
-      store8<false>(ws, p.D + col, s1[c]);
+      if (at.col(c) >= p.D) continue;
+      store8<false>(ws, at.col(c), s0[c]);
+      store8<false>(ws, p.D + at.col(c), s1[c]);
     }
   }
 }
@@ -305,10 +454,17 @@ __global__ __launch_bounds__(RC* RL) void norm_sums_kernel(NormTrainDev d, long 
   }
 }
 
-int threads_of(int D, int* nch) {
-  *nch = D > kMaxThreads * 8 ? 2 : 1;
-  const int per = (D / 8 + *nch - 1) / *nch;
-  return (per + 63) / 64 * 64;
+// Waves per row and chunks per lane (1, 2, 4 or 6)
+struct Shape {
+  int row_waves, chunks, table;  // table: bytes of one table
+};
+Shape shape_of(int D) {
+  Shape x;
+  x.row_waves = D <= 64 * 48 ? 1 : D <= 128 * 48 ? 2 : 4;
+  const int need = (D + 512 * x.row_waves - 1) / (512 * x.row_waves);
+  x.chunks = need <= 2 ? need : need <= 4 ? 4 : 6;
+  x.table = 64 * x.row_waves * x.chunks * 8 * 4;
+  return x;
 }
 
 int check_common(const NormTrainParams& p) {
@@ -324,33 +480,40 @@ int check_common(const NormTrainParams& p) {
   return 0;
 }
 
-// Strips of the backward pass: enough workgroups for the chip (two per CU), none under 4 rows, one segment each.
-void plan(const NormTrainParams& p, long* segs, int* strips, int* strip_rows) {
+// Strips of one segment each: `want` workgroups in all, none under `least` rows
+void plan(const NormTrainParams& p, int wanted, int least, long* segs, int* strips, int* strip_rows) {
   const long seg_rows = p.seg_rows > 0 ? std::min(p.seg_rows, p.rows) : p.rows;
   *segs = p.rows > 0 ? (p.rows + seg_rows - 1) / seg_rows : 0;
   if (*segs == 0) {
     *strips = *strip_rows = 0;
     return;
   }
-  const long want = std::max(1L, 512 / *segs);
-  const long most = std::max(1L, seg_rows / 4);
+  const long want = std::max(1L, wanted / *segs);
+  const long most = std::max(1L, (seg_rows + least - 1) / least);
   const long n = std::min(want, most);
   *strip_rows = (int)((seg_rows + n - 1) / n);
   *strips = (int)((seg_rows + *strip_rows - 1) / *strip_rows);
 }
 
-using BwdKernel = void (*)(NormTrainDev);
-template <bool X, bool R, int N>
-BwdKernel pick(bool sums) {
-  return sums ? (BwdKernel)norm_bwd_kernel<X, R, N, true> : (BwdKernel)norm_bwd_kernel<X, R, N, false>;
+using Kernel = void (*)(NormTrainDev);
+template <bool X, bool R, bool S>
+Kernel pick(int chunks) {
+  return chunks == 1   ? (Kernel)norm_bwd_kernel<X, R, 1, S>
+         : chunks == 2 ? (Kernel)norm_bwd_kernel<X, R, 2, S>
+         : chunks == 4 ? (Kernel)norm_bwd_kernel<X, R, 4, S>
+                       : (Kernel)norm_bwd_kernel<X, R, 6, S>;
 }
-template <bool X, bool R>
-BwdKernel pick(int nch, bool sums) {
-  return nch == 1 ? pick<X, R, 1>(sums) : pick<X, R, 2>(sums);
+template <bool X>
+Kernel pick(int chunks, bool rms, bool sums) {
+  if (rms) return sums ? pick<X, true, true>(chunks) : pick<X, true, false>(chunks);
+  return sums ? pick<X, false, true>(chunks) : pick<X, false, false>(chunks);
 }
-BwdKernel bwd_kernel(bool x_bf16, bool rms, int nch, bool sums) {
-  if (x_bf16) return rms ? pick<true, true>(nch, sums) : pick<true, false>(nch, sums);
-  return rms ? pick<false, true>(nch, sums) : pick<false, false>(nch, sums);
+template <bool X>
+Kernel pick_fwd(int chunks) {
+  return chunks == 1   ? (Kernel)layernorm_mod_kernel<X, 1>
+         : chunks == 2 ? (Kernel)layernorm_mod_kernel<X, 2>
+         : chunks == 4 ? (Kernel)layernorm_mod_kernel<X, 4>
+                       : (Kernel)layernorm_mod_kernel<X, 6>;
 }
 
 }  // namespace
@@ -362,7 +525,7 @@ long norm_bwd_workspace_bytes(long rows, long seg_rows, int D) {
   p.seg_rows = seg_rows;
   long segs;
   int strips, strip_rows;
-  plan(p, &segs, &strips, &strip_rows);
+  plan(p, kBwdStrips, kBwdRows, &segs, &strips, &strip_rows);
   return segs * strips * 2 * D * 4;
 }
 
@@ -371,12 +534,17 @@ int layernorm_mod(const NormTrainParams& p, bool x_bf16, hipStream_t s) {
   FLITE_REQUIRE((p.y || p.rows == 0) && ((uintptr_t)p.y & 15) == 0 && p.ldy % 8 == 0 && p.ldy >= p.D,
                 "layernorm: y must be 16-byte aligned rows, their stride a multiple of 8 and at least dim");
   if (p.rows == 0) return 0;
-  int nch;
-  const dim3 block(threads_of(p.D, &nch)), grid((unsigned)p.rows);
-  if (x_bf16 && nch == 1) hipLaunchKernelGGL((layernorm_mod_kernel<true, 1>), grid, block, 0, s, p);
-  if (x_bf16 && nch == 2) hipLaunchKernelGGL((layernorm_mod_kernel<true, 2>), grid, block, 0, s, p);
-  if (!x_bf16 && nch == 1) hipLaunchKernelGGL((layernorm_mod_kernel<false, 1>), grid, block, 0, s, p);
-  if (!x_bf16 && nch == 2) hipLaunchKernelGGL((layernorm_mod_kernel<false, 2>), grid, block, 0, s, p);
+  const Shape x = shape_of(p.D);
+  NormTrainDev d;
+  d.p = p;
+  d.row_waves = x.row_waves;
+  long segs;
+  plan(p, kFwdStrips, kWaves / x.row_waves, &segs, &d.strips, &d.strip_rows);
+  FLITE_REQUIRE(segs * d.strips <= 0x7fffffffL, "layernorm: too many segments");
+  const Kernel k = x_bf16 ? pick_fwd<true>(x.chunks) : pick_fwd<false>(x.chunks);
+  if (2 * x.table > 48 * 1024)
+    FLITE_HIP_CHECK(hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * x.table));
+  hipLaunchKernelGGL(k, dim3((unsigned)(segs * d.strips)), dim3(kThreads), 2 * x.table, s, d);
   FLITE_HIP_CHECK(hipGetLastError());
   return 0;
 }
@@ -394,15 +562,16 @@ int norm_bwd(const NormTrainParams& p, bool x_bf16, bool rms, hipStream_t s) {
   NormTrainDev d;
   d.p = p;
   long segs;
-  plan(p, &segs, &d.strips, &d.strip_rows);
+  plan(p, kBwdStrips, kBwdRows, &segs, &d.strips, &d.strip_rows);
   FLITE_REQUIRE(!sums || p.rows == 0 || (p.ws && ((uintptr_t)p.ws & 15) == 0 &&
                                          p.ws_bytes >= norm_bwd_workspace_bytes(p.rows, p.seg_rows, p.D)),
                 "norm backward: workspace missing or too small");
   FLITE_REQUIRE(segs * d.strips <= 0x7fffffffL, "norm backward: too many segments");
   if (p.rows > 0) {
-    int nch;
-    const dim3 block(threads_of(p.D, &nch)), grid((unsigned)(segs * d.strips));
-    hipLaunchKernelGGL(bwd_kernel(x_bf16, rms, nch, sums), grid, block, 0, s, d);
+    const Shape x = shape_of(p.D);
+    d.row_waves = x.row_waves;
+    const Kernel k = x_bf16 ? pick<true>(x.chunks, rms, sums) : pick<false>(x.chunks, rms, sums);
+    hipLaunchKernelGGL(k, dim3((unsigned)(segs * d.strips)), dim3(kThreads), x.table, s, d);
     FLITE_HIP_CHECK(hipGetLastError());
   }
   if (sums) {
