@@ -559,7 +559,7 @@ struct TrAhead {
   }
 };
 
-// acc[n] (VGPRs) = stage rows . stationary block n. hook(s) after k-step s; last(): reads of the next phase
+// acc[n] (VGPRs) = stage rows . stationary block n. hook(m) after each of the D / 8 MFMAs; last(): reads of the next phase
 template <int D, typename Hook, typename Last>
 __device__ __forceinline__ void row_phase(const RowReader<D>& o, const RowAhead<D>& first,
                                           const bf16x8 (&f)[2][D / 16], f32x16 (&acc)[2], Hook hook, Last last) {
@@ -573,10 +573,11 @@ __device__ __forceinline__ void row_phase(const RowReader<D>& o, const RowAhead<
     FENCE();
     if (s + AHEAD < NS) a[s + AHEAD] = o.read(s + AHEAD);
     if (s + AHEAD == NS) last();
+    hook(2 * s);
     FENCE();
     acc[1] = mfma(a[s], f[1][s], s == 0 ? zero16() : acc[1]);
     FENCE();
-    hook(s);
+    hook(2 * s + 1);
     FENCE();
   }
 }
@@ -603,6 +604,18 @@ __device__ __forceinline__ void tr_phase(const TrReader<D>& o, const TrAhead<D>&
     hook(2 * m + 1);
     FENCE();
   }
+}
+
+// A softmax has 32 scores a lane and stage. With D = 256 they fit between the 32 MFMAs of the tr phase behind their row
+// phase. With fewer columns the last kLate of them get their exp2 between the MFMAs of the next row phase (which makes
+// the next stage's scores: their arguments move out of its way in the tr phase).
+template <int D>
+constexpr int kLate = D == 256 ? 0 : D == 128 ? 20 : 16;
+// MFMA of the tr phase that score e is done behind: 6 parts of work for a whole one, 1 for an argument
+template <int D>
+constexpr int slot_of(int e) {
+  constexpr int M = D / 8 - SKIP, T = 32 - kLate<D>, W = 6 * T + kLate<D>;
+  return SKIP + (e < T ? 6 * e : 6 * T + e - T) * M / W;
 }
 
 template <int ND>
@@ -754,9 +767,12 @@ __device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char
     auto none = [](int) {};
     auto nothing = []() {};
     // work behind MFMA m of the tr phase: copies of step i, and the 32 scores spread over the MFMAs m >= SKIP
-    auto spread = [&](int i, int m, auto one) {
+    auto spread_copies = [&](int i, int m) {
       constexpr int GAP = (4 * ND) / (2 * P + 1);
       if (m % GAP == 0 && m / GAP <= 2 * P) copy(i, m / GAP);
+    };
+    auto spread = [&](int i, int m, auto one) {
+      spread_copies(i, m);
 #pragma unroll
       for (int e = share(m, 4 * ND, 32); e < share(m + 1, 4 * ND, 32); ++e) one(e);
     };
@@ -770,31 +786,45 @@ __device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char
     if ((wave & 1) == 0) {
       // score e of stage j: group r4 = e >> 3 (rows 8 r4 + 4 hh + 0..3), block (e >> 2) & 1. Each call does the exp2 of
       // its score, the argument of the next and the stores of the ones before, so that nothing waits on the exp2
+      constexpr int LATE = kLate<D>, T = 32 - LATE;
       f32x4 lse, lse_n;
-      float x;
+      float x, late[LATE > 0 ? LATE : 1];
+      auto val = [&](int e) { return e < T ? s[(e >> 2) & 1][4 * (e >> 3) + (e & 3)] : late[e < T ? 0 : e - T]; };
       auto arg = [&](int j, int e) {
         const int r4 = e >> 3, nb = (e >> 2) & 1, i = e & 3;
         if ((e & 7) == 0) lse = lse_n;
-        x = __builtin_fmaf(s[nb][4 * r4 + i], sl2, -lse[i]);
+        const float y = __builtin_fmaf(s[nb][4 * r4 + i], sl2, -lse[i]);
+        if (e < T)
+          x = y;
+        else
+          late[e - T] = y;
         if ((e & 7) == 0 && r4 < 3)
           lse_n = *(const f32x4*)(smem + L::LSE + (j & 7) * 256 + (8 * (r4 + 1) + 4 * hh) * 4);
       };
       auto store = [&](int j, int e) {  // P of score e is there
         const int r4 = e >> 3, nb = (e >> 2) & 1, i = e & 3, r = 4 * r4 + i;
-        if (i & 1) bn[nb][r >> 3][(r & 7) >> 1] = pack_bf(s[nb][r - 1], s[nb][r]);
+        if (i & 1) bn[nb][r >> 3][(r & 7) >> 1] = pack_bf(val(e - 1), val(e));
         if (i == 3) {
           typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
           *(f16x4*)(xch + (j & 1) * L::PBYTES + (r4 * 2 + nb) * 512) =
-              f16x4{(_Float16)s[nb][r - 3], (_Float16)s[nb][r - 2], (_Float16)s[nb][r - 1], (_Float16)s[nb][r]};
+              f16x4{(_Float16)val(e - 3), (_Float16)val(e - 2), (_Float16)val(e - 1), (_Float16)val(e)};
         }
       };
       auto begin = [&](int j) { lse_n = *(const f32x4*)(smem + L::LSE + (j & 7) * 256 + 4 * hh * 4); };
-      auto prob = [&](int j, int e) {
+      auto prob = [&](int j, int e) {  // in the tr phase
         if (e == 0) arg(j, 0);
-        s[(e >> 2) & 1][4 * (e >> 3) + (e & 3)] = __builtin_amdgcn_exp2f(x);
+        if (e < T) s[(e >> 2) & 1][4 * (e >> 3) + (e & 3)] = __builtin_amdgcn_exp2f(x);
         if (e < 31) arg(j, e + 1);
-        if (e > 0) store(j, e - 1);
-        if (e == 31) store(j, 31);
+        if (e > 0 && e <= T) store(j, e - 1);
+        if (e == 31 && T == 32) store(j, 31);
+      };
+      auto prob_late = [&](int j, int m) {  // behind MFMA m of the next row phase
+#pragma unroll
+        for (int e = T + m * LATE / (D / 8); e < T + (m + 1) * LATE / (D / 8); ++e) {
+          late[e - T] = __builtin_amdgcn_exp2f(late[e - T]);
+          if (e > T) store(j, e - 1);
+          if (e == 31) store(j, 31);
+        }
       };
       rr.init(lane, lds0 + L::A);
       tr.init(lane, lds0 + L::B);
@@ -803,20 +833,29 @@ __device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char
       row_phase<D>(rr, ra, f, s, none, nothing);
 #pragma unroll
       for (int e = 0; e < 32; ++e) prob(0, e);
-      next();
+      if constexpr (LATE == 0) next();
       rr.move(SB);  // q stage i + 1
       ra.read(rr);
       for (int i = 0; i < n; ++i) {
         open();
         begin(i + 1);
-        row_phase<D>(rr, ra, f, s, none, [&]() { ta.read(tr); });
+        row_phase<D>(rr, ra, f, s, [&](int m) { prob_late(i, m); }, [&]() { ta.read(tr); });
+        if constexpr (LATE > 0) next();
         rr.move(next_a(qi + 1));
         if (wave == 0)
           step_sync<E*(2 * P + 1)>();
         else
           step_sync<E * 2 * P>();
-        tr_phase<D>(tr, ta, bc, acc, [&](int m) { spread(i, m, [&](int e) { prob(i + 1, e); }); }, [&]() { ra.read(rr); });
-        next();
+        tr_phase<D>(
+            tr, ta, bc, acc,
+            [&](int m) {
+              spread_copies(i, m);
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (slot_of<D>(e) == m) prob(i + 1, e);
+            },
+            [&]() { ra.read(rr); });
+        if constexpr (LATE == 0) next();
         tr.move(next_b(di));
         qi = wrap<L::RA>(qi + 1);
         di = wrap<L::RB>(di + 1);
@@ -1339,29 +1378,36 @@ __global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[nb][r] = 8 * (r >> 2) + 4 * hh + (r & 3) < left ? s[nb][r] : -INFINITY;
     };
-    // Softmax of a stage in 40 pieces: maxima of 4 scores (8), P of one score (32)
-    float sub[2], x;
+    constexpr int LATE = kLate<D>, T = 32 - LATE;
+    float sub[2], x, late[LATE > 0 ? LATE : 1];
+    auto val = [&](int e) { return e < T ? s[(e >> 2) & 1][4 * (e >> 3) + (e & 3)] : late[e < T ? 0 : e - T]; };
     auto arg = [&](int e) {
       const int nb = (e >> 2) & 1, r = 4 * (e >> 3) + (e & 3);
-      x = __builtin_fmaf(s[nb][r], sl2, -sub[nb]);
+      float& to = e < T ? x : late[e < T ? 0 : e - T];
+      to = __builtin_fmaf(s[nb][r], sl2, -sub[nb]);
     };
-    auto maxima = [&](int u) {
-      const int nb = u >> 2, r = 4 * (u & 3);
+    auto add = [&](int e) {  // P of score e is there
+      const int nb = (e >> 2) & 1, r = 4 * (e >> 3) + (e & 3);
+      l[nb] += val(e);
+      if (r & 1) bn[nb][r >> 3][(r & 7) >> 1] = pack_bf(val(e - 1), val(e));
+    };
+    auto maxima = [&](int u) {  // of scores 4 u .. 4 u + 3, before their exp2 takes their place
+      const int nb = u & 1, r = 4 * (u >> 1);
       most[nb] = fmaxf(most[nb], fmaxf(fmaxf(s[nb][r], s[nb][r + 1]), fmaxf(s[nb][r + 2], s[nb][r + 3])));
     };
-    auto prob = [&](int e) {
-      const int nb = (e >> 2) & 1, r = 4 * (e >> 3) + (e & 3);
+    auto prob = [&](int e) {  // in the tr phase
       if (e == 0) arg(0);
-      s[nb][r] = __builtin_amdgcn_exp2f(x);
+      if (e < T) s[(e >> 2) & 1][4 * (e >> 3) + (e & 3)] = __builtin_amdgcn_exp2f(x);
       if (e < 31) arg(e + 1);
-      if (e > 0) {
-        const int e1 = e - 1, n1 = (e1 >> 2) & 1, r1 = 4 * (e1 >> 3) + (e1 & 3);
-        l[n1] += s[n1][r1];
-        if (r1 & 1) bn[n1][r1 >> 3][(r1 & 7) >> 1] = pack_bf(s[n1][r1 - 1], s[n1][r1]);
-      }
-      if (e == 31) {
-        l[nb] += s[nb][r];
-        bn[nb][r >> 3][(r & 7) >> 1] = pack_bf(s[nb][r - 1], s[nb][r]);
+      if (e > 0 && e <= T) add(e - 1);
+      if (e == 31 && T == 32) add(31);
+    };
+    auto prob_late = [&](int m) {  // behind MFMA m of the next row phase
+#pragma unroll
+      for (int e = T + m * LATE / (D / 8); e < T + (m + 1) * LATE / (D / 8); ++e) {
+        late[e - T] = __builtin_amdgcn_exp2f(late[e - T]);
+        if (e > T) add(e - 1);
+        if (e == 31) add(31);
       }
     };
     // largest score of the query: the lane halves hold different keys
@@ -1384,12 +1430,13 @@ __global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
     }
 #pragma unroll
     for (int e = 0; e < 32; ++e) prob(e);
-    next();
+    if constexpr (LATE == 0) next();
     rr.move(SB);  // k stage i + 1
     ra.read(rr);
     for (int i = 0; i < n; ++i) {
       open();
-      row_phase<D>(rr, ra, f, s, none, [&]() { ta.read(tr); });
+      row_phase<D>(rr, ra, f, s, [&](int k) { prob_late(k); }, [&]() { ta.read(tr); });
+      if constexpr (LATE > 0) next();
       rr.move(move(ri + 1));
       mask(i + 1);
       step_sync<E * 2 * P>();
@@ -1399,10 +1446,14 @@ __global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
             constexpr int GAP = (4 * ND) / (2 * P);
             if (k % GAP == 0 && k / GAP < 2 * P) copy(k / GAP);
 #pragma unroll
-            for (int u = share(k, 4 * ND, 40); u < share(k + 1, 4 * ND, 40); ++u) u < 8 ? maxima(u) : prob(u - 8);
+            for (int u = 0; u < 8; ++u)
+              if (slot_of<D>(4 * u) == k) maxima(u);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (slot_of<D>(e) == k) prob(e);
           },
           [&]() { ra.read(rr); });
-      next();
+      if constexpr (LATE == 0) next();
       tr.move(move(ri));
       ri = wrap<L::R>(ri + 1);
     }
