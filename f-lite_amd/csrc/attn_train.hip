@@ -432,7 +432,8 @@ __device__ __forceinline__ void copy4(const i32x4& rsrc, unsigned voff, unsigned
 // A stream of 32-row stages over a tensor: descriptor of the next one, zeros after the last. One head's rows [0, len)
 // follow those of the head before; all in scalar registers.
 struct Stream {
-  const char* ptr;   // first byte of the next stage
+  i32x4 rs;          // descriptor of the current stage
+  const char* ptr;   // first byte of the next one
   int left;          // rows from there to the sequence end
   int stages;        // stages that are still to come
   int len, row_b;    // rows of a sequence, bytes of a row
@@ -450,15 +451,30 @@ struct Stream {
     ptr = (const char*)base + (long)h * head_bytes + (long)r * row_bytes;
   }
   // rows_of: bytes per row that the range counts (the whole stride: offsets are row * stride + column)
-  __device__ __forceinline__ i32x4 next() {
+  __device__ __forceinline__ void next() {
     const int live = stages > 0 ? min(left, 32) : 0;
-    const i32x4 rs = make_rsrc(ptr, (unsigned)(live * row_b));
+    rs = make_rsrc(ptr, (unsigned)(live * row_b));
     --stages;
     left -= 32;
     const bool w = left <= 0;
     ptr += stages > 0 ? (w ? wrap : step) : 0;
     left = w ? len : left;
-    return rs;
+  }
+};
+
+// Slots of a ring of N stages, in bytes: where a copy goes, or what moves a reader on
+template <int N, int BYTES>
+struct Ring {
+  int at;
+  __device__ __forceinline__ void next() {
+    at += BYTES;
+    at = at == N * BYTES ? 0 : at;
+  }
+  __device__ __forceinline__ int move() {
+    at += BYTES;
+    const bool end = at == N * BYTES;
+    at = end ? 0 : at;
+    return end ? (1 - N) * BYTES : BYTES;
   }
 };
 
@@ -661,12 +677,6 @@ __device__ __forceinline__ constexpr int share(int m, int M, int all) {
   return m <= SKIP ? 0 : ((m - SKIP) * all + (M - SKIP) - 1) / (M - SKIP);
 }
 
-// i mod M for i in [-M, 2 M)
-template <int M>
-__device__ __forceinline__ int wrap(int i) {
-  return i < 0 ? i + M : i >= M ? i - M : i;
-}
-
 // A key workgroup: dk and dv of 128 keys of K/V head hk. Step i: wave 0 makes S(i + 1), then (behind the barrier) adds
 // dout(i)^T P(i) to dv while it turns S(i + 1) into P(i + 1); wave 1 makes dP(i), then adds q(i - 1)^T dS(i - 1) to dk
 // while it makes dS(i) from dP(i) and P(i).
@@ -703,26 +713,23 @@ __device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char
     st_q.init(p.q + (long)q_start * p.q_row + h0 * p.q_head, t0, tiles, q_len, n, p.q_row * 2, p.q_head * 2);
     st_d.init(p.dout + (long)q_start * p.do_row + h0 * p.do_head, t0, tiles, q_len, n, p.do_row * 2, p.do_head * 2);
     st_x.init((wave == 0 ? d.lse2 : d.delta) + h0 * p.total_q + q_start, t0, tiles, q_len, n, 4, (long)p.total_q * 4);
-    i32x4 rq, rd, rx;
-    int qi = 0, di = 0;  // step mod RA, mod RB
+    Ring<L::RA, SB> to_a{(3 + E) * SB};  // where step i's copies go
+    Ring<L::RB, SB> to_b{(2 + E) * SB};
     // stages i + 3 + E of q and i + 2 + E of dout, in 2 P + 1 pieces: issued behind step i's barrier, in place E + 1
     // barriers later
     auto open = [&]() {
-      rq = st_q.next();
-      rd = st_d.next();
-      rx = st_x.next();
+      st_q.next();
+      st_d.next();
+      st_x.next();
     };
     auto copy = [&](int i, int k) {
       if (k < P)
-        copy16(rq, sq.src(k), wlds + L::A + wrap<L::RA>(qi + 3 + E) * SB + sq.dst(k));
+        copy16(st_q.rs, sq.src(k), wlds + L::A + to_a.at + sq.dst(k));
       else if (k < 2 * P)
-        copy16(rd, sd.src(k - P), wlds + L::B + wrap<L::RB>(di + 2 + E) * SB + sd.dst(k - P));
+        copy16(st_d.rs, sd.src(k - P), wlds + L::B + to_b.at + sd.dst(k - P));
       else if (k == 2 * P && wave < 2)
-        copy4(rx, ld_off, lds0 + (wave == 0 ? L::LSE + ((i + 3 + E) & 7) * 256 : L::DELTA + ((i + 2 + E) & 7) * 256));
+        copy4(st_x.rs, ld_off, lds0 + (wave == 0 ? L::LSE + ((i + 3 + E) & 7) * 256 : L::DELTA + ((i + 2 + E) & 7) * 256));
     };
-    // bytes from slot x of a ring to the next one
-    auto next_a = [&](int x) { return wrap<L::RA>(x) == L::RA - 1 ? (1 - L::RA) * SB : SB; };
-    auto next_b = [&](int x) { return wrap<L::RB>(x) == L::RB - 1 ? (1 - L::RB) * SB : SB; };
     RowReader<D> rr;
     TrReader<D> tr;
     // before step 0: q stages -1 (zeros: dk(-1) adds nothing), 0 .. 2 + E; dout stages 0 .. 1 + E
@@ -732,19 +739,19 @@ __device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char
       for (int k = 0; k < P; ++k) copy16(zero, sq.src(k), wlds + L::A + (L::RA - 1) * SB + sq.dst(k));
 #pragma unroll
       for (int j = 0; j < 3 + E; ++j) {
-        rq = st_q.next();
+        st_q.next();
 #pragma unroll
-        for (int k = 0; k < P; ++k) copy16(rq, sq.src(k), wlds + L::A + j * SB + sq.dst(k));
+        for (int k = 0; k < P; ++k) copy16(st_q.rs, sq.src(k), wlds + L::A + j * SB + sq.dst(k));
       }
 #pragma unroll
       for (int j = 0; j < 2 + E; ++j) {
-        rd = st_d.next();
+        st_d.next();
 #pragma unroll
-        for (int k = 0; k < P; ++k) copy16(rd, sd.src(k), wlds + L::B + j * SB + sd.dst(k));
+        for (int k = 0; k < P; ++k) copy16(st_d.rs, sd.src(k), wlds + L::B + j * SB + sd.dst(k));
       }
       for (int j = 0; j < (wave == 0 ? 3 : 2) + E; ++j) {
-        rx = st_x.next();
-        if (wave < 2) copy4(rx, ld_off, lds0 + (wave == 0 ? L::LSE : L::DELTA) + j * 256);
+        st_x.next();
+        if (wave < 2) copy4(st_x.rs, ld_off, lds0 + (wave == 0 ? L::LSE : L::DELTA) + j * 256);
       }
     }
     // stationary rows: k for wave 0, v for wave 1
@@ -836,12 +843,14 @@ __device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char
       if constexpr (LATE == 0) next();
       rr.move(SB);  // q stage i + 1
       ra.read(rr);
+      Ring<L::RA, SB> at_r{SB};
+      Ring<L::RB, SB> at_t{0};
       for (int i = 0; i < n; ++i) {
         open();
         begin(i + 1);
         row_phase<D>(rr, ra, f, s, [&](int m) { prob_late(i, m); }, [&]() { ta.read(tr); });
         if constexpr (LATE > 0) next();
-        rr.move(next_a(qi + 1));
+        rr.move(at_r.move());
         if (wave == 0)
           step_sync<E*(2 * P + 1)>();
         else
@@ -856,9 +865,9 @@ __device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char
             },
             [&]() { ra.read(rr); });
         if constexpr (LATE == 0) next();
-        tr.move(next_b(di));
-        qi = wrap<L::RA>(qi + 1);
-        di = wrap<L::RB>(di + 1);
+        tr.move(at_t.move());
+        to_a.next();
+        to_b.next();
       }
       step_sync();
     } else {
@@ -872,6 +881,8 @@ __device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char
       f32x4 del, del_n;
       typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
       f16x4 pr, pr_n;
+      Ring<L::RB, SB> at_r{0};
+      Ring<L::RA, SB> at_t{(L::RA - 1) * SB};
       for (int i = 0; i <= n; ++i) {
         auto rd = [&](int e) {  // delta and P of the 4 scores from e on
           const int r4 = e >> 3, nb = (e >> 2) & 1;
@@ -880,7 +891,7 @@ __device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char
         };
         open();  // after the last stage: zeros
         row_phase<D>(rr, ra, f, s, none, [&]() { ta.read(tr); });
-        rr.move(next_b(di));
+        rr.move(at_r.move());
         if (wave == 1)
           step_sync<E*(2 * P + 1)>();
         else
@@ -902,9 +913,9 @@ __device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char
             },
             [&]() { ra.read(rr); });
         next();
-        tr.move(next_a(qi - 1));
-        qi = wrap<L::RA>(qi + 1);
-        di = wrap<L::RB>(di + 1);
+        tr.move(at_t.move());
+        to_a.next();
+        to_b.next();
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may outlive the workgroup
@@ -958,26 +969,28 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
     st_k.init(p.k + (long)k_start * p.k_row + (long)hk * p.k_head, t0, all, k_len, n, p.k_row * 2, 0);
     st_v.init(p.v + (long)k_start * p.v_row + (long)hk * p.v_head, t0, all, k_len, n, p.v_row * 2, 0);
   }
-  i32x4 rk, rv;
-  int ki = 0, vi = 0;  // step mod RA, mod RB
+  // stages i + 3 + E of k and v
+  Ring<L::RA, SB> to_a{0};
+  Ring<L::RB, SB> to_b{0};
   auto open = [&]() {
-    rk = st_k.next();
-    rv = st_v.next();
+    st_k.next();
+    st_v.next();
   };
-  auto copy = [&](int j, int k) {  // piece k of k and v stage i + j
+  auto copy = [&](int k) {  // piece k
     if (k < P)
-      copy16(rk, sk.src(k), wlds + L::A + wrap<L::RA>(ki + j) * SB + sk.dst(k));
+      copy16(st_k.rs, sk.src(k), wlds + L::A + to_a.at + sk.dst(k));
     else if (k < 2 * P)
-      copy16(rv, sv.src(k - P), wlds + L::B + wrap<L::RB>(vi + (j == L::RB ? 0 : j)) * SB + sv.dst(k - P));
-  };
-  auto copy_all = [&](int j) {
-    open();
-#pragma unroll
-    for (int k = 0; k < 2 * P; ++k) copy(j, k);
+      copy16(st_v.rs, sv.src(k - P), wlds + L::B + to_b.at + sv.dst(k - P));
   };
   auto advance = [&]() {
-    ki = wrap<L::RA>(ki + 1);
-    vi = wrap<L::RB>(vi + 1);
+    to_a.next();
+    to_b.next();
+  };
+  auto copy_all = [&]() {
+    open();
+#pragma unroll
+    for (int k = 0; k < 2 * P; ++k) copy(k);
+    advance();
   };
 
   // dS of stage j: [j & 1][pair][block][r4][lane] f32x4
@@ -985,7 +998,7 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
   if ((wave & 1) == 0) {
     if (n <= 0) return;  // wave 1 stores the zeros
 #pragma unroll
-    for (int j = 0; j < 3 + E; ++j) copy_all(j);
+    for (int j = 0; j < 3 + E; ++j) copy_all();
     bf16x8 qf[2][NS], df[2][NS];
     float lse[2], del[2];
 #pragma unroll
@@ -1053,6 +1066,8 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
         }
       }
     };
+    Ring<L::RA, SB> at_k{SB};
+    Ring<L::RB, SB> at_v{SB};
     auto mask = [&](int j, f32x16 (&s)[2]) {  // keys past the end: P = 0 (their exp2(-lse) may overflow)
       const int left = k_len - (t0 + j) * 32;
       if (left >= 32) return;
@@ -1069,11 +1084,11 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
           [&](int m) {
 #pragma unroll
             for (int u = share(m, 4 * NS, 64); u < share(m + 1, 4 * NS, 64); ++u) ds_half(i, s, dp, u);
-            if ((m & 1) && (m >> 1) < 2 * P) copy(3 + E, m >> 1);
+            if ((m & 1) && (m >> 1) < 2 * P) copy(m >> 1);
           },
           [&]() {
-            kr.move(wrap<L::RA>(ki + 1) == L::RA - 1 ? (1 - L::RA) * SB : SB);
-            vr.move(wrap<L::RB>(vi + 1) == L::RB - 1 ? (1 - L::RB) * SB : SB);
+            kr.move(at_k.move());
+            vr.move(at_v.move());
             read_first();
           });
       advance();
@@ -1098,15 +1113,15 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
   acc_zero<ND>(acc);
   if (n > 0) {
 #pragma unroll
-    for (int j = 0; j < 3 + E; ++j) copy_all(j);
+    for (int j = 0; j < 3 + E; ++j) copy_all();
     step_sync();
     step_sync();
-    copy_all(3 + E);
+    copy_all();
     bf16x8 a[ND];
     TrReader<D> tr;  // k stage i - 1
     tr.init(lane, lds0 + L::A);
     auto rd = [&](int s, int dt) { a[dt] = tr.read(s, dt); };
-    advance();
+    Ring<L::RA, SB> at_t{0};
     step_sync<E * 2 * P>();
     for (int i = 1; i <= n; ++i) {
       open();  // after the last stage: zeros
@@ -1152,7 +1167,7 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
 #pragma unroll
           for (int q = 0; q < 8; ++q)
             if (s == 0 && q * ND / 4 == m) split_lo(0, q);
-          if (s == 1 && (m & 1)) copy(3 + E, P + (m >> 1));
+          if (s == 1 && (m & 1)) copy(P + (m >> 1));
           FENCE();
         }
         settle();
@@ -1169,11 +1184,11 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
               split_hi(1, q);
               split_lo(1, q);
             }
-          if (s == 0 && !(m & 1) && (m >> 1) < P) copy(3 + E, m >> 1);
+          if (s == 0 && !(m & 1) && (m >> 1) < P) copy(m >> 1);
           FENCE();
         }
       }
-      tr.move(wrap<L::RA>(ki - 1) == L::RA - 1 ? (1 - L::RA) * SB : SB);
+      tr.move(at_t.move());
       advance();
       if (i < n) step_sync<E * 2 * P>();
     }
@@ -1305,7 +1320,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
   const int per = (all + ranges - 1) / ranges, t0 = min(part * per, all), n = min(per, all - t0);
 
   f32x16 acc[2][ND];
-  float m[2] = {-INFINITY, -INFINITY}, l[2], most[2] = {-INFINITY, -INFINITY};
+  float m[2] = {-INFINITY, -INFINITY}, l[2], largest[2];
   bool again = false;
   do {
     acc_zero<ND>(acc);
@@ -1319,31 +1334,29 @@ __global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
     Stream st_k, st_v;
     st_k.init(p.k + (long)k_start * p.k_row + (long)hk * p.k_head, t0, all, k_len, n, p.k_row * 2, 0);
     st_v.init(p.v + (long)k_start * p.v_row + (long)hk * p.v_head, t0, all, k_len, n, p.v_row * 2, 0);
-    i32x4 rk, rv;
-    int ri = 0;  // step mod R
+    Ring<L::R, SB> to_a{0}, to_b{(L::R - 1) * SB}, at_r{SB}, at_t{0};
     // stages i + 3 + E of k and i + 2 + E of v: issued behind step i's barrier, in place E + 1 barriers later
     auto open = [&]() {
-      rk = st_k.next();
-      rv = st_v.next();
+      st_k.next();
+      st_v.next();
     };
     auto copy = [&](int k) {
       if (k < P)
-        copy16(rk, sk.src(k), wlds + L::A + ri * SB + sk.dst(k));
+        copy16(st_k.rs, sk.src(k), wlds + L::A + to_a.at + sk.dst(k));
       else if (k < 2 * P)
-        copy16(rv, sv.src(k - P), wlds + L::B + wrap<L::R>(ri - 1) * SB + sv.dst(k - P));
+        copy16(st_v.rs, sv.src(k - P), wlds + L::B + to_b.at + sv.dst(k - P));
     };
-    auto move = [&](int x) { return wrap<L::R>(x) == L::R - 1 ? (1 - L::R) * SB : SB; };
 #pragma unroll
     for (int j = 0; j < L::R; ++j) {
-      rk = st_k.next();
+      st_k.next();
 #pragma unroll
-      for (int k = 0; k < P; ++k) copy16(rk, sk.src(k), wlds + L::A + j * SB + sk.dst(k));
+      for (int k = 0; k < P; ++k) copy16(st_k.rs, sk.src(k), wlds + L::A + j * SB + sk.dst(k));
     }
 #pragma unroll
     for (int j = 0; j < L::R - 1; ++j) {
-      rv = st_v.next();
+      st_v.next();
 #pragma unroll
-      for (int k = 0; k < P; ++k) copy16(rv, sv.src(k), wlds + L::B + j * SB + sv.dst(k));
+      for (int k = 0; k < P; ++k) copy16(st_v.rs, sv.src(k), wlds + L::B + j * SB + sv.dst(k));
     }
     bf16x8 f[2][D / 16];
 #pragma unroll
@@ -1379,21 +1392,25 @@ __global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
         for (int r = 0; r < 16; ++r) s[nb][r] = 8 * (r >> 2) + 4 * hh + (r & 3) < left ? s[nb][r] : -INFINITY;
     };
     constexpr int LATE = kLate<D>, T = 32 - LATE;
-    float sub[2], x, late[LATE > 0 ? LATE : 1];
+    float most[2];  // largest exponent (score less m)
+    float sub[2], x, last, late[LATE > 0 ? LATE : 1];
     auto val = [&](int e) { return e < T ? s[(e >> 2) & 1][4 * (e >> 3) + (e & 3)] : late[e < T ? 0 : e - T]; };
     auto arg = [&](int e) {
       const int nb = (e >> 2) & 1, r = 4 * (e >> 3) + (e & 3);
-      float& to = e < T ? x : late[e < T ? 0 : e - T];
-      to = __builtin_fmaf(s[nb][r], sl2, -sub[nb]);
+      const float y = __builtin_fmaf(s[nb][r], sl2, -sub[nb]);
+      if (e < T)
+        x = y;
+      else
+        late[e - T] = y;
+      if (e & 1)
+        most[nb] = fmaxf(fmaxf(most[nb], last), y);
+      else
+        last = y;
     };
     auto add = [&](int e) {  // P of score e is there
       const int nb = (e >> 2) & 1, r = 4 * (e >> 3) + (e & 3);
       l[nb] += val(e);
       if (r & 1) bn[nb][r >> 3][(r & 7) >> 1] = pack_bf(val(e - 1), val(e));
-    };
-    auto maxima = [&](int u) {  // of scores 4 u .. 4 u + 3, before their exp2 takes their place
-      const int nb = u & 1, r = 4 * (u >> 1);
-      most[nb] = fmaxf(most[nb], fmaxf(fmaxf(s[nb][r], s[nb][r + 1]), fmaxf(s[nb][r + 2], s[nb][r + 3])));
     };
     auto prob = [&](int e) {  // in the tr phase
       if (e == 0) arg(0);
@@ -1406,6 +1423,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
 #pragma unroll
       for (int e = T + m * LATE / (D / 8); e < T + (m + 1) * LATE / (D / 8); ++e) {
         late[e - T] = __builtin_amdgcn_exp2f(late[e - T]);
+        asm volatile("" : "+v"(late[e - T]));  // not behind the branch of the mask
         if (e > T) add(e - 1);
         if (e == 31) add(31);
       }
@@ -1419,14 +1437,16 @@ __global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
     ra.read(rr);
     row_phase<D>(rr, ra, f, s, none, nothing);
     mask(0);
-    if (!again) {
-#pragma unroll
-      for (int u = 0; u < 8; ++u) maxima(u);
-    }
 #pragma unroll
     for (int nb = 0; nb < 2; ++nb) {
-      m[nb] = both(most[nb]) * sl2;
+      if (!again) {
+        float x = s[nb][0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) x = fmaxf(x, s[nb][r]);
+        m[nb] = both(x) * sl2;
+      }
       sub[nb] = m[nb] == -INFINITY ? 0.f : m[nb];  // only -inf scores so far: P = exp2(-inf) = 0
+      most[nb] = -INFINITY;
     }
 #pragma unroll
     for (int e = 0; e < 32; ++e) prob(e);
@@ -1437,7 +1457,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
       open();
       row_phase<D>(rr, ra, f, s, [&](int k) { prob_late(k); }, [&]() { ta.read(tr); });
       if constexpr (LATE > 0) next();
-      rr.move(move(ri + 1));
+      rr.move(at_r.move());
       mask(i + 1);
       step_sync<E * 2 * P>();
       tr_phase<D>(
@@ -1446,23 +1466,32 @@ __global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
             constexpr int GAP = (4 * ND) / (2 * P);
             if (k % GAP == 0 && k / GAP < 2 * P) copy(k / GAP);
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-              if (slot_of<D>(4 * u) == k) maxima(u);
-#pragma unroll
             for (int e = 0; e < 32; ++e)
               if (slot_of<D>(e) == k) prob(e);
           },
           [&]() { ra.read(rr); });
       if constexpr (LATE == 0) next();
-      tr.move(move(ri));
-      ri = wrap<L::R>(ri + 1);
+      tr.move(at_t.move());
+      to_a.next();
+      to_b.next();
     }
     // a score far above m in any wave (all copies land here, too: none may outlive the sweep)
-    const bool far = __any(both(most[0]) * sl2 > m[0] + 40.f || both(most[1]) * sl2 > m[1] + 40.f);
+    bool far = false;
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+      const float x = both(most[nb]);
+      far |= x > 40.f || (m[nb] == -INFINITY && x > m[nb]);
+      largest[nb] = x + sub[nb];
+    }
+    far = __any(far);
     volatile LDS_AS unsigned char* flag = (volatile LDS_AS unsigned char*)(unsigned long)(lds0 + L::FLAG);
     if (lane == 0) flag[wave] = far && !again;
     step_sync();
     again = (flag[0] | flag[1] | flag[2] | flag[3]) != 0;
+    if (again) {
+      m[0] = largest[0];
+      m[1] = largest[1];
+    }
     step_sync();
   } while (again);
   acc_fence<ND>(acc);
