@@ -79,33 +79,6 @@ __device__ __forceinline__ void seq_range(const int* cu, int b, int total, int* 
   *len = e - s;
 }
 
-// Tile t of R rows of the packed batch -> (sequence, first row); false past the last one. Tiles number the sequences'
-// pieces in order.
-template <int R>
-__device__ __forceinline__ bool find_tile(const int* cu, int B, int total, int t, int* b, int* row0) {
-  const int lane = threadIdx.x & 63;
-  for (int base = 0; base < B; base += 64) {
-    int s, len = 0;
-    if (base + lane < B) seq_range(cu, base + lane, total, &s, &len);
-    const int n = (len + R - 1) / R;
-    int sum = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int up = __shfl_up(sum, o, 64);
-      if (lane >= o) sum += up;
-    }
-    const unsigned long long hit = __ballot(t < sum);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      *b = base + l;
-      *row0 = (t - (__shfl(sum, l, 64) - __shfl(n, l, 64))) * R;
-      return true;
-    }
-    t -= __shfl(sum, 63, 64);
-  }
-  return false;
-}
-
 // Sequence that holds `row`, -1: none
 __device__ __forceinline__ int find_seq(const int* cu, int B, int total, int row) {
   int lo = 0, hi = B;  // the last b with cu[b] <= row
@@ -1290,33 +1263,84 @@ struct FwdLds {
   static constexpr int R = 3 + E, A = 0, B = R * Stage<D>::BYTES, FLAG = 2 * R * Stage<D>::BYTES, TOTAL = FLAG + 16;
 };
 
+// The forward pass's units: a tile of 256 queries and a range of its sequence's keys, tiles in order, ranges within
+__device__ __forceinline__ int units_of(const TrainDev& d, int b, int* ranges) {
+  const AttnTrainParams& p = d.p;
+  *ranges = 1;
+  if (b >= p.B) return 0;
+  int s, q_len, k_len;
+  seq_range(p.cu_q, b, p.total_q, &s, &q_len);
+  seq_range(p.cu_k, b, p.total_k, &s, &k_len);
+  *ranges = ranges_of((k_len + 31) / 32, d.stages, d.most);
+  return (q_len + 255) / 256 * *ranges;
+}
+// Block v -> its unit, heads in turn; false: nothing to do. The launch has an upper bound of blocks, and those without
+// a unit come last (between the others they kept units from starting: ragged batch 63 -> 55 us).
+struct FwdUnit {
+  int b, h, row0, part, ranges;
+};
+__device__ __forceinline__ bool find_fwd_unit(const TrainDev& d, FwdUnit* u) {
+  const int lane = threadIdx.x & 63, B = d.p.B;
+  auto chunk = [&](int base, int* n, int* own) {  // units up to and with sequence base + lane
+    *n = units_of(d, base + lane, own);
+    int sum = *n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += up;
+    }
+    return sum;
+  };
+  int n, own, sum = chunk(0, &n, &own);
+  int units = __builtin_amdgcn_readlane(sum, 63);
+  for (int base = 64; base < B; base += 64) {
+    int n1, own1;
+    units += __builtin_amdgcn_readlane(chunk(base, &n1, &own1), 63);
+  }
+  units = min(units, d.tiles * d.most);  // more: the cumulative lengths are wrong
+  int v = blockIdx.x;
+  if (v >= units * d.p.H) return false;
+  v = xcd_remap(v, units * d.p.H);
+  u->h = v / units;
+  v %= units;
+  for (int base = 0;;) {
+    const unsigned long long hit = __ballot(v < sum);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      v -= __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l);
+      u->b = base + l;
+      u->ranges = __builtin_amdgcn_readlane(own, l);
+      u->row0 = v / u->ranges * 256;
+      u->part = v % u->ranges;
+      return true;
+    }
+    v -= __builtin_amdgcn_readlane(sum, 63);
+    base += 64;
+    if (base >= B) return false;
+    sum = chunk(base, &n, &own);
+  }
+}
+
 template <int D>
-__global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d) {
+__global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d, int blocks) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const AttnTrainParams& p = d.p;
+  if ((int)blockIdx.x >= blocks) {
+    zero_outside(p.o, p.o_row, p.o_head, p.cu_q, p.B, p.total_q, p.H, D, p.lse, blockIdx.x - blocks, gridDim.x - blocks);
+    return;
+  }
+  FwdUnit u;
+  if (!find_fwd_unit(d, &u)) return;
+  const int b = u.b, h = u.h, row0 = u.row0, part = u.part, ranges = u.ranges;
   using L = FwdLds<D>;
   constexpr int ND = D / 32, SB = Stage<D>::BYTES, P = Stage<D>::PIECES, E = L::E;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lq = lane & 31, hh = lane >> 5;
-  const int n_units = d.tiles * p.H * d.most;
-  if ((int)blockIdx.x >= n_units) {
-    zero_outside(p.o, p.o_row, p.o_head, p.cu_q, p.B, p.total_q, p.H, D, p.lse, blockIdx.x - n_units, gridDim.x - n_units);
-    return;
-  }
-  int v = xcd_remap(blockIdx.x, n_units);
-  const int part = v % d.most;
-  v /= d.most;
-  const int h = v / d.tiles;
-  int b, row0;
-  if (!find_tile<256>(p.cu_q, p.B, p.total_q, v % d.tiles, &b, &row0)) return;
-  b = __builtin_amdgcn_readfirstlane(b);
-  row0 = __builtin_amdgcn_readfirstlane(row0);
   int q_start, q_len, k_start, k_len;
   seq_range(p.cu_q, b, p.total_q, &q_start, &q_len);
   seq_range(p.cu_k, b, p.total_k, &k_start, &k_len);
   const int hk = h / (p.H / p.HK);
-  const int all = (k_len + 31) / 32, ranges = ranges_of(all, d.stages, d.most);
-  if (part >= ranges) return;
+  const int all = (k_len + 31) / 32;
   const int per = (all + ranges - 1) / ranges, t0 = min(part * per, all), n = min(per, all - t0);
 
   f32x16 acc[2][ND];
@@ -1652,8 +1676,8 @@ int launch_fwd(const TrainDev& d, hipStream_t s) {
   static std::atomic<unsigned long long> done{0};
   if (lds_limit(attn_lse_kernel<D>, lds, done)) return 1;
   const AttnTrainParams& p = d.p;
-  hipLaunchKernelGGL(attn_lse_kernel<D>, dim3(d.tiles * p.H * d.most + (p.zero_outside ? kZeroBlocks : 0)), dim3(kThreads), lds,
-                     s, d);
+  const int blocks = d.tiles * p.H * d.most;
+  hipLaunchKernelGGL(attn_lse_kernel<D>, dim3(blocks + (p.zero_outside ? kZeroBlocks : 0)), dim3(kThreads), lds, s, d, blocks);
   FLITE_HIP_CHECK(hipGetLastError());
   if (d.most > 1)
     hipLaunchKernelGGL(attn_lse_join_kernel<D>, dim3((unsigned)(((long)p.total_q * p.H * (D / 8) + kThreads - 1) / kThreads)),
