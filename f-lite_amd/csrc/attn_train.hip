@@ -359,7 +359,7 @@ __global__ __launch_bounds__(kThreads) void attn_delta_kernel(TrainDev d, int n)
 // with D = 256, 0.4 with 128, 0.2 with 64, and LDS has room for more stages where they are small (D = 128, ragged batch:
 // 1.37 us a step without).
 template <int D>
-constexpr int kExtra = D == 256 ? 0 : D == 128 ? 2 : 4;
+constexpr int kExtra = D == 256 ? 0 : D == 128 ? 2 : 1;
 
 template <int D>
 struct Stage {
@@ -1322,7 +1322,7 @@ __device__ __forceinline__ bool find_fwd_unit(const TrainDev& d, FwdUnit* u) {
 }
 
 template <int D>
-__global__ __launch_bounds__(kThreads, 1) void attn_lse_kernel(TrainDev d, int blocks) {
+__global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attn_lse_kernel(TrainDev d, int blocks) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const AttnTrainParams& p = d.p;
   if ((int)blockIdx.x >= blocks) {
