@@ -633,6 +633,28 @@ __device__ __forceinline__ unsigned pack_bf(float lo, float hi) {
   return __builtin_bit_cast(unsigned, v);
 }
 
+// What bf16 dropped of the pair whose rounded halves are `hi`, as bf16
+__device__ __forceinline__ unsigned dropped(float a, float b, unsigned hi) {
+  return pack_bf(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+}
+
+// P and dS are rounded to bf16 for their products. Over many roundings and results that averages out: dv, dk and out are
+// sqrt(2) times as far (in the mean square) from the exact ones as one rounding of the result is. Where a sequence has few
+// of them, or few that matter, chance takes that far up (one query's P rounds alike for all columns: up to 2), so there a
+// second run of MFMAs adds what the rounding dropped. Few: for out at most 2048 P or 8192 results, for dk and dv, whose
+// terms vary more, 2^17 P or 32768 results. In 800 batches of up to five sequences of 1 to 4720 tokens, with keys that
+// many queries share: out 1.43 at most, dk and dv 1.50, against 1.46 and 1.54 in 100 without.
+__device__ __forceinline__ bool few(long pairs, long results, bool gradient) {
+  return pairs <= (gradient ? 1 << 17 : 2048) || results <= (gradient ? 32768 : 8192);
+}
+
+// VALU write -> asm MFMA read (the compiler does not look into asm): two wait states before a run of MFMAs
+__device__ __forceinline__ void settle() {
+  FENCE();
+  asm volatile("s_nop 1");
+  FENCE();
+}
+
 // LDS of a key workgroup: q ring of 5 stages, dout ring of 3, P double-buffered, lse and delta rings; of a query
 // workgroup: k ring of 5, v ring of 3, dS double-buffered (D = 256: all 160 KB). Rings are kExtra stages longer.
 template <int D>
@@ -640,8 +662,8 @@ struct Lds {
   static constexpr int RA = 5 + kExtra<D>, RB = 3 + kExtra<D>;
   static constexpr int A = 0, B = RA * Stage<D>::BYTES, X = B + RB * Stage<D>::BYTES;
   static constexpr int PBYTES = 8192, SBYTES = 16384;  // one buffer of P, of dS
-  static constexpr int LSE = X + 2 * PBYTES, DELTA = LSE + 8 * 256, TOTAL = X + 2 * SBYTES;
-  static_assert(DELTA + 8 * 256 <= TOTAL, "lse and delta lie behind P, where a query workgroup has its dS");
+  static constexpr int LSE = X + 2 * PBYTES, DELTA = LSE + 8 * 256, LOW = DELTA + 8 * 256, TOTAL = X + 2 * SBYTES;
+  static_assert(LOW + PBYTES <= TOTAL, "lse, delta and the low parts of dS lie behind P, where a query workgroup has dS");
   static_assert(TOTAL <= 160 * 1024 && 3 + kExtra<D> < 8, "LDS of a CU; the rings of lse and delta");
 };
 
@@ -653,7 +675,7 @@ __device__ __forceinline__ constexpr int share(int m, int M, int all) {
 // A key workgroup: dk and dv of 128 keys of K/V head hk. Step i: wave 0 makes S(i + 1), then (behind the barrier) adds
 // dout(i)^T P(i) to dv while it turns S(i + 1) into P(i + 1); wave 1 makes dP(i), then adds q(i - 1)^T dS(i - 1) to dk
 // while it makes dS(i) from dP(i) and P(i).
-template <int D>
+template <int D, bool FEW>
 __device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char* smem) {
   const AttnTrainParams& p = d.p;
   using L = Lds<D>;
@@ -837,6 +859,21 @@ __device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char
                 if (slot_of<D>(e) == m) prob(i + 1, e);
             },
             [&]() { ra.read(rr); });
+        if constexpr (FEW) {  // P(i) lies in LDS with three more bits
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            const int nb = g & 1, ks = g >> 2, w = g & 2;
+            typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
+            const f16x4 y = *(const f16x4*)(xch + (i & 1) * L::PBYTES + g * 512);
+            u32x4 b = __builtin_bit_cast(u32x4, bc[nb][ks]);
+            b[w] = dropped((float)y[0], (float)y[1], b[w]);
+            b[w + 1] = dropped((float)y[2], (float)y[3], b[w + 1]);
+            bc[nb][ks] = __builtin_bit_cast(bf16x8, b);
+          }
+          ta.read(tr);
+          settle();
+          tr_phase<D>(tr, ta, bc, acc, none, nothing);
+        }
         if constexpr (LATE == 0) next();
         tr.move(at_t.move());
         to_a.next();
@@ -856,6 +893,11 @@ __device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char
       f16x4 pr, pr_n;
       Ring<L::RB, SB> at_r{0};
       Ring<L::RA, SB> at_t{(L::RA - 1) * SB};
+      char* const low = smem + L::LOW + pair * (L::PBYTES / 2) + lane * 16;  // of dS(i - 1): [block][k-step][lane] 16 B
+      if constexpr (FEW) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) *(u32x4*)(low + g * 1024) = u32x4{0u, 0u, 0u, 0u};
+      }
       for (int i = 0; i <= n; ++i) {
         auto rd = [&](int e) {  // delta and P of the 4 scores from e on
           const int r4 = e >> 3, nb = (e >> 2) & 1;
@@ -885,6 +927,21 @@ __device__ __forceinline__ void key_block(const TrainDev& d, const Unit& u, char
               });
             },
             [&]() { ra.read(rr); });
+        if constexpr (FEW) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int nb = g >> 1, ks = g & 1;
+            bc[nb][ks] = *(const bf16x8*)(low + g * 1024);
+            u32x4 w;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              w[c] = dropped(s[nb][8 * ks + 2 * c], s[nb][8 * ks + 2 * c + 1], bn[nb][ks][c]);
+            *(u32x4*)(low + g * 1024) = w;
+          }
+          ta.read(tr);
+          settle();
+          tr_phase<D>(tr, ta, bc, acc, none, nothing);
+        }
         next();
         tr.move(at_t.move());
         to_a.next();
@@ -1122,12 +1179,6 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
 #pragma unroll
       for (int q = 0; q < 8; ++q) split_hi(0, q);
       FENCE();
-      // VALU write -> asm MFMA read (the compiler does not look into asm): two wait states before each run of MFMAs
-      auto settle = []() {
-        FENCE();
-        asm volatile("s_nop 1");
-        FENCE();
-      };
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         settle();
@@ -1188,10 +1239,16 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_kernel(TrainDev d) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   Unit u;
   if (!find_unit(d, blockIdx.x, &u)) return;
+  const AttnTrainParams& p = d.p;
+  int start, q_len, k_len;
+  seq_range(p.cu_q, u.b, p.total_q, &start, &q_len);
+  seq_range(p.cu_k, u.b, p.total_k, &start, &k_len);
   if (u.query)
     query_block<D>(d, u, smem);
+  else if (few((long)q_len * k_len * p.H, (long)k_len * p.HK * D, true))
+    key_block<D, true>(d, u, smem);
   else
-    key_block<D>(d, u, smem);
+    key_block<D, false>(d, u, smem);
 }
 
 // Adds the ranges' partial gradients in order: one item = 8 columns of a row and head, of all rows (full tiles) or of the
@@ -1260,7 +1317,8 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(TrainDev d, JoinIte
 template <int D>
 struct FwdLds {
   static constexpr int E = D == 256 ? 1 : D == 128 ? 3 : 4;  // steps that a copy may take beyond its own
-  static constexpr int R = 3 + E, A = 0, B = R * Stage<D>::BYTES, FLAG = 2 * R * Stage<D>::BYTES, TOTAL = FLAG + 16;
+  static constexpr int R = 3 + E, A = 0, B = R * Stage<D>::BYTES, LOW = 2 * R * Stage<D>::BYTES, FLAG = LOW + 16384,
+                       TOTAL = FLAG + 16;
 };
 
 // The forward pass's units: a tile of 256 queries and a range of its sequence's keys, tiles in order, ranges within
@@ -1321,16 +1379,9 @@ __device__ __forceinline__ bool find_fwd_unit(const TrainDev& d, FwdUnit* u) {
   }
 }
 
-template <int D>
-__global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attn_lse_kernel(TrainDev d, int blocks) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+template <int D, bool FEW>
+__device__ __forceinline__ void lse_unit(const TrainDev& d, const FwdUnit& u, char* smem) {
   const AttnTrainParams& p = d.p;
-  if ((int)blockIdx.x >= blocks) {
-    zero_outside(p.o, p.o_row, p.o_head, p.cu_q, p.B, p.total_q, p.H, D, p.lse, blockIdx.x - blocks, gridDim.x - blocks);
-    return;
-  }
-  FwdUnit u;
-  if (!find_fwd_unit(d, &u)) return;
   const int b = u.b, h = u.h, row0 = u.row0, part = u.part, ranges = u.ranges;
   using L = FwdLds<D>;
   constexpr int ND = D / 32, SB = Stage<D>::BYTES, P = Stage<D>::PIECES, E = L::E;
@@ -1474,12 +1525,24 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attn_lse_kernel(Tra
     }
 #pragma unroll
     for (int e = 0; e < 32; ++e) prob(e);
+    // what bf16 drops of P, in 4s of scores: [wave][group][lane] 8 B
+    char* const low = smem + L::LOW + wave * 4096 + lane * 8;
+    auto save = [&](int from, int to) {
+#pragma unroll
+      for (int e = from; e < to; e += 4) {
+        const int nb = (e >> 2) & 1, r = 4 * (e >> 3), w = (r & 7) >> 1;
+        *(uint2*)(low + (e >> 2) * 512) = make_uint2(dropped(val(e), val(e + 1), bn[nb][r >> 3][w]),
+                                                     dropped(val(e + 2), val(e + 3), bn[nb][r >> 3][w + 1]));
+      }
+    };
+    if constexpr (FEW) save(0, T);
     if constexpr (LATE == 0) next();
     rr.move(SB);  // k stage i + 1
     ra.read(rr);
     for (int i = 0; i < n; ++i) {
       open();
       row_phase<D>(rr, ra, f, s, [&](int k) { prob_late(k); }, [&]() { ta.read(tr); });
+      if constexpr (FEW && LATE > 0) save(T, 32);
       if constexpr (LATE > 0) next();
       rr.move(at_r.move());
       mask(i + 1);
@@ -1494,6 +1557,20 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attn_lse_kernel(Tra
               if (slot_of<D>(e) == k) prob(e);
           },
           [&]() { ra.read(rr); });
+      if constexpr (FEW) {
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          const uint2 y = *(const uint2*)(low + g * 512);
+          u32x4 b = __builtin_bit_cast(u32x4, bc[g & 1][g >> 2]);
+          b[g & 2] = y.x;
+          b[(g & 2) + 1] = y.y;
+          bc[g & 1][g >> 2] = __builtin_bit_cast(bf16x8, b);
+        }
+        save(0, T);
+        ta.read(tr);
+        settle();
+        tr_phase<D>(tr, ta, bc, acc, none, nothing);
+      }
       if constexpr (LATE == 0) next();
       tr.move(at_t.move());
       to_a.next();
@@ -1533,6 +1610,25 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attn_lse_kernel(Tra
     store_row<D>(p.o + rc * p.o_row + (long)h * p.o_head, acc[nb], sum == 0.f ? 0.f : 1.f / sum, hh, live);
     if (live && hh == 0) p.lse[(long)h * p.total_q + rc] = sum == 0.f ? -INFINITY : (m[nb] + log2f(sum)) * kLn2;
   }
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void attn_lse_kernel(TrainDev d, int blocks) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const AttnTrainParams& p = d.p;
+  if ((int)blockIdx.x >= blocks) {
+    zero_outside(p.o, p.o_row, p.o_head, p.cu_q, p.B, p.total_q, p.H, D, p.lse, blockIdx.x - blocks, gridDim.x - blocks);
+    return;
+  }
+  FwdUnit u;
+  if (!find_fwd_unit(d, &u)) return;
+  int start, q_len, k_len;
+  seq_range(p.cu_q, u.b, p.total_q, &start, &q_len);
+  seq_range(p.cu_k, u.b, p.total_k, &start, &k_len);
+  if (few((long)q_len * k_len * p.H, (long)q_len * p.H * D, false))
+    lse_unit<D, true>(d, u, smem);
+  else
+    lse_unit<D, false>(d, u, smem);
 }
 
 // Joins the ranges of rows that were cut: out and lse from their sums, in range order

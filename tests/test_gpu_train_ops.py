@@ -54,8 +54,8 @@ def cu_of(lens, first=0):
 
 
 # ------------------------------------------------------------------------------------------------ attention
-def attn_ref(q, k, v, do, ql, kl, scale, q_first=0, k_first=0, f=F):
-    """out, lse, dq, dk, dv in 64 bits and an elementwise bound for each, with P off by f; rows outside stay 0 (lse -inf)."""
+def attn_ref(q, k, v, do, ql, kl, scale, q_first=0, k_first=0, f=F, u=U):
+    """out, lse, dq, dk, dv in 64 bits and an elementwise bound for each, with P off by f, P and dS rounded by u; rows outside stay 0 (lse -inf)."""
     n, h, d = q.shape
     hk = k.shape[1]
     Q, K, V, DO = (x.double() for x in (q, k, v, do))
@@ -75,20 +75,20 @@ def attn_ref(q, k, v, do, ql, kl, scale, q_first=0, k_first=0, f=F):
             o = p @ vi
             ref["lse"][i, qs] = lse[:, 0]
             ref["out"][qs, i] = o
-            o_err = U * o.abs() + (U + 3 * f) * (p @ vi.abs())
+            o_err = U * o.abs() + (u + 3 * f) * (p @ vi.abs())
             tol["out"][qs, i] = o_err
             dp = di @ vi.T
             delta = (di * o).sum(1, keepdim=True)
             ds = p * (dp - delta)
             d_err = (di.abs() * o_err).sum(1, keepdim=True)  # delta is made from the rounded out
             # dS: one rounding, the error of P, and that of dP - delta
-            ds_err = U * ds.abs() + 3 * f * p * (di.abs() @ vi.abs().T + delta.abs()) + p * d_err
+            ds_err = u * ds.abs() + 3 * f * p * (di.abs() @ vi.abs().T + delta.abs()) + p * d_err
             ref["dq"][qs, i] = scale * ds @ ki
             tol["dq"][qs, i] = abs(scale) * ds_err @ ki.abs()
             ref["dk"][ks, j] += scale * ds.T @ qi
             tol["dk"][ks, j] += abs(scale) * ds_err.T @ qi.abs()
             ref["dv"][ks, j] += p.T @ di
-            tol["dv"][ks, j] += (U + 3 * f) * (p.T @ di.abs())
+            tol["dv"][ks, j] += (u + 3 * f) * (p.T @ di.abs())
         a, b = a + nq, b + nk
     for x in ("dq", "dk", "dv"):
         tol[x] += U * ref[x].abs()
@@ -219,6 +219,28 @@ def test_attention_scores_that_grow(d, scale):
     grads = nat.attn_varlen_bwd(do, q, k, v, out, lse, cq, ck, scale)
     for x, g in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *grads)):
         close(g, ref[x], tol[x], x)
+
+
+@pytest.mark.parametrize("d,h,hk,ql,kl", [
+    (64, 1, 1, [1], [3]), (128, 1, 1, [2], [5]), (256, 1, 1, [1], [2]),
+    (64, 4, 2, [1, 3, 0, 7, 16], [2, 90, 5, 33, 31]),
+    (128, 2, 1, [32, 1, 31], [32, 33, 3]),
+    (256, 4, 2, [1, 3, 0, 7, 16], [2, 90, 5, 33, 31]),
+    (64, 2, 1, [128], [512]), (64, 2, 1, [2000], [5]), (128, 1, 1, [64], [40]), (256, 2, 2, [1], [4000]),
+])
+def test_attention_of_few_rows(d, h, hk, ql, kl):
+    """Few probabilities or results: P and dS count with what bf16 drops of them (fp16, or two bf16 parts)."""
+    cq, ck, scale = cu_of(ql), cu_of(kl), d ** -0.5
+    for seed in range(4):
+        q, k, v, do = attn_inputs(d, h, hk, ql, kl, seed=30 + 10 * seed)
+        ref, tol = attn_ref(q, k, v, do, ql, kl, scale, u=2.0 ** -12)
+        out, lse = nat.attn_varlen_lse(q, k, v, cq, ck, scale)
+        grads = nat.attn_varlen_bwd(do, q, k, v, out, lse, cq, ck, scale)
+        pairs = max(a * b for a, b in zip(ql, kl)) * h
+        for x, g in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *grads)):
+            few = pairs <= 2048 or max(ql) * h * d <= 8192 if x == "out" else pairs <= 2 ** 17 or max(kl) * hk * d <= 32768
+            if few or x in ("lse", "dq"):
+                close(g, ref[x], tol[x], x)
 
 
 def test_attention_gradients_against_differences():
