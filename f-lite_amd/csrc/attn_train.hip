@@ -62,6 +62,7 @@ struct TrainDev {
   int most, stages;        // ranges of a sweep, at most; stages of a range
   float* part_o;           // [most][total_q][H][D] with most > 1: sums of 2^(S - m) v
   float2* part_ml;         // [most][H][total_q]: m and the sum of 2^(S - m), S in units of log2
+  int* starts;             // [B + 1] units of a head before each sequence, for batches of more than 64
   // backward
   Cut q, k;
   int* target;             // stages per range: of a full tile, of a part; [2]: groups, [3]: blocks that have work
@@ -96,6 +97,20 @@ __device__ __forceinline__ int ranges_of(int stages, int target, int most) {
   return min(max((stages + target - 1) / target, 1), most);
 }
 
+// The last of `start`'s n ascending entries (STEP ints apart) that is at most v; start[0] is. A wave looks at 64 at a time.
+template <int STEP>
+__device__ __forceinline__ int last_at_most(const int* start, int n, int v) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64, at = lo + lane * step;
+    const int found = __popcll(__ballot(at < hi && start[(long)min(at, hi - 1) * STEP] <= v));
+    lo += max(found - 1, 0) * step;
+    hi = min(lo + step, hi);
+  }
+  return lo;
+}
+
 // The backward pass's work list: groups of equal units (the full tiles of a sequence, or its part, as keys or as queries),
 // the longest ranges first. Made on the device, which alone knows the lengths; the launch has an upper bound of blocks.
 struct Group {
@@ -111,32 +126,21 @@ struct Unit {
 };
 // Block v -> its unit; false: nothing to do
 __device__ __forceinline__ bool find_unit(const TrainDev& d, int v, Unit* u) {
-  const int lane = threadIdx.x & 63;
   const int n = d.target[2], blocks = d.target[3];
   if (v >= blocks) return false;
-  for (int base = 0; base < n; base += 64) {
-    // the group of v is the last one that starts at or before it; the entry behind it tells its size
-    const int4 g = d.groups[min(base + lane, n - 1)];
-    const int next = base + lane + 1 < n ? d.groups[base + lane + 1].x : blocks;
-    const unsigned long long hit = __ballot(base + lane < n && g.x <= v && v < next);
-    if (hit == 0) continue;
-    const int l = __builtin_ctzll(hit);
-    const int first = __builtin_amdgcn_readfirstlane(__shfl(g.x, l, 64));
-    const int size = __builtin_amdgcn_readfirstlane(__shfl(next, l, 64)) - first;
-    const int id = __builtin_amdgcn_readfirstlane(__shfl(g.y, l, 64));
-    const int tiles = __builtin_amdgcn_readfirstlane(__shfl(g.w, l, 64));
-    u->ranges = __builtin_amdgcn_readfirstlane(__shfl(g.z, l, 64));
-    u->b = id >> 2;
-    u->full = !(id & Group::PART);
-    u->query = (id & Group::QUERY) != 0;
-    v = xcd_remap(v - first, size);  // neighbours in the group (tiles of a head) on one XCD
-    u->part = v % u->ranges;
-    v /= u->ranges;
-    u->tile = v % tiles;
-    u->h = v / tiles;
-    return true;
-  }
-  return false;
+  const int e = __builtin_amdgcn_readfirstlane(last_at_most<4>((const int*)d.groups, n, v));
+  const int4 g = d.groups[e];
+  const int size = (e + 1 < n ? d.groups[e + 1].x : blocks) - g.x;
+  u->ranges = g.z;
+  u->b = g.y >> 2;
+  u->full = !(g.y & Group::PART);
+  u->query = (g.y & Group::QUERY) != 0;
+  v = xcd_remap(v - g.x, size);  // neighbours in the group (tiles of a head) on one XCD
+  u->part = v % g.z;
+  v /= g.z;
+  u->tile = v % g.w;
+  u->h = v / g.w;
+  return true;
 }
 
 // Row `row` of sequence b, head h, range 0 in the partial gradients; *step: floats from range to range
@@ -1339,44 +1343,66 @@ struct FwdUnit {
 };
 __device__ __forceinline__ bool find_fwd_unit(const TrainDev& d, FwdUnit* u) {
   const int lane = threadIdx.x & 63, B = d.p.B;
-  auto chunk = [&](int base, int* n, int* own) {  // units up to and with sequence base + lane
-    *n = units_of(d, base + lane, own);
-    int sum = *n;
+  int v = blockIdx.x, units, own;
+  if (B <= 64) {
+    const int n = units_of(d, lane, &own);
+    int sum = n;  // units up to and with sequence `lane`
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int up = __shfl_up(sum, o, 64);
       if (lane >= o) sum += up;
     }
-    return sum;
-  };
-  int n, own, sum = chunk(0, &n, &own);
-  int units = __builtin_amdgcn_readlane(sum, 63);
-  for (int base = 64; base < B; base += 64) {
-    int n1, own1;
-    units += __builtin_amdgcn_readlane(chunk(base, &n1, &own1), 63);
+    units = min(__builtin_amdgcn_readlane(sum, 63), d.tiles * d.most);  // more: the cumulative lengths are wrong
+    if (v >= units * d.p.H) return false;
+    v = xcd_remap(v, units * d.p.H);
+    u->h = v / units;
+    v %= units;
+    u->b = __builtin_ctzll(__ballot(v < sum));
+    v -= __builtin_amdgcn_readlane(sum, u->b) - __builtin_amdgcn_readlane(n, u->b);
+    u->ranges = __builtin_amdgcn_readlane(own, u->b);
+  } else {
+    units = min(__builtin_amdgcn_readfirstlane(d.starts[B]), d.tiles * d.most);
+    if (v >= units * d.p.H) return false;
+    v = xcd_remap(v, units * d.p.H);
+    u->h = v / units;
+    v %= units;
+    u->b = __builtin_amdgcn_readfirstlane(last_at_most<1>(d.starts, B, v));
+    v -= __builtin_amdgcn_readfirstlane(d.starts[u->b]);
+    units_of(d, u->b, &own);
+    u->ranges = __builtin_amdgcn_readfirstlane(own);
   }
-  units = min(units, d.tiles * d.most);  // more: the cumulative lengths are wrong
-  int v = blockIdx.x;
-  if (v >= units * d.p.H) return false;
-  v = xcd_remap(v, units * d.p.H);
-  u->h = v / units;
-  v %= units;
-  for (int base = 0;;) {
-    const unsigned long long hit = __ballot(v < sum);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      v -= __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(n, l);
-      u->b = base + l;
-      u->ranges = __builtin_amdgcn_readlane(own, l);
-      u->row0 = v / u->ranges * 256;
-      u->part = v % u->ranges;
-      return true;
+  u->row0 = v / u->ranges * 256;
+  u->part = v % u->ranges;
+  return true;
+}
+
+// Units before each sequence, in one workgroup: a block that counted them itself would read all lengths (1024 sequences
+// of 64 tokens, 16 heads: 702 us)
+__global__ __launch_bounds__(kThreads) void attn_lse_units_kernel(TrainDev d) {
+  __shared__ int waves[kThreads / 64];
+  const int tid = threadIdx.x;
+  int before = 0;
+  for (int base = 0; base < d.p.B; base += kThreads) {
+    int own;
+    const int n = units_of(d, base + tid, &own);
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(sum, o, 64);
+      if ((tid & 63) >= o) sum += up;
     }
-    v -= __builtin_amdgcn_readlane(sum, 63);
-    base += 64;
-    if (base >= B) return false;
-    sum = chunk(base, &n, &own);
+    if ((tid & 63) == 63) waves[tid >> 6] = sum;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < kThreads / 64; ++w) {
+      if (w < (tid >> 6)) sum += waves[w];
+      all += waves[w];
+    }
+    if (base + tid < d.p.B) d.starts[base + tid] = before + sum - n;
+    before += all;
+    __syncthreads();
   }
+  if (tid == 0) d.starts[d.p.B] = before;
 }
 
 template <int D, bool FEW>
@@ -1718,7 +1744,8 @@ Plan make_plan(const AttnTrainParams& p) {
 constexpr int kFwdRange = 16;
 struct FwdPlan {
   int tiles, most, stages;
-  long o_bytes, ml_bytes;
+  long o_bytes, ml_bytes, starts_bytes;
+  long total() const { return o_bytes + ml_bytes + starts_bytes; }
 };
 FwdPlan make_fwd_plan(const AttnTrainParams& p) {
   FwdPlan x;
@@ -1730,6 +1757,7 @@ FwdPlan make_fwd_plan(const AttnTrainParams& p) {
   auto pad = [](long n) { return (n + 255) / 256 * 256; };
   x.o_bytes = x.most > 1 ? pad((long)x.most * p.total_q * p.H * p.dim * 4) : 0;
   x.ml_bytes = x.most > 1 ? pad((long)x.most * p.total_q * p.H * 8) : 0;
+  x.starts_bytes = p.B > 64 ? pad((p.B + 1L) * 4) : 0;
   return x;
 }
 
@@ -1773,6 +1801,8 @@ int launch_fwd(const TrainDev& d, hipStream_t s) {
   if (lds_limit(attn_lse_kernel<D>, lds, done)) return 1;
   const AttnTrainParams& p = d.p;
   const int blocks = d.tiles * p.H * d.most;
+  if (p.B > 64) hipLaunchKernelGGL(attn_lse_units_kernel, dim3(1), dim3(kThreads), 0, s, d);
+  FLITE_HIP_CHECK(hipGetLastError());
   hipLaunchKernelGGL(attn_lse_kernel<D>, dim3(blocks + (p.zero_outside ? kZeroBlocks : 0)), dim3(kThreads), lds, s, d, blocks);
   FLITE_HIP_CHECK(hipGetLastError());
   if (d.most > 1)
@@ -1815,8 +1845,7 @@ long attn_train_workspace_bytes(const AttnTrainParams& p) {
 
 long attn_train_fwd_workspace_bytes(const AttnTrainParams& p) {
   if (check(p)) return -1;
-  const FwdPlan x = make_fwd_plan(p);
-  return x.o_bytes + x.ml_bytes;
+  return make_fwd_plan(p).total();
 }
 
 int attn_train_fwd(const AttnTrainParams& p, void* ws, long ws_bytes, hipStream_t s) {
@@ -1829,7 +1858,7 @@ int attn_train_fwd(const AttnTrainParams& p, void* ws, long ws_bytes, hipStream_
   FLITE_REQUIRE(p.lse || !any_q, "attention: missing lse");
   if (!any_q) return 0;
   const FwdPlan x = make_fwd_plan(p);
-  FLITE_REQUIRE(x.most == 1 || (ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= x.o_bytes + x.ml_bytes),
+  FLITE_REQUIRE(x.total() == 0 || (ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= x.total()),
                 "attention: workspace missing, not 256-byte aligned, or too small");
   TrainDev d{};
   d.p = p;
@@ -1838,6 +1867,7 @@ int attn_train_fwd(const AttnTrainParams& p, void* ws, long ws_bytes, hipStream_
   d.stages = x.stages;
   d.part_o = (float*)ws;
   d.part_ml = (float2*)((char*)ws + x.o_bytes);
+  d.starts = (int*)((char*)ws + x.o_bytes + x.ml_bytes);
   if (p.dim == 64) return launch_fwd<64>(d, s);
   if (p.dim == 128) return launch_fwd<128>(d, s);
   return launch_fwd<256>(d, s);

@@ -111,6 +111,7 @@ ATTN = [
     (128, 4, 1, [257, 3], [1100, 1025]),
     (64, 2, 2, [3000], [1600]),
     (64, 2, 1, [1, 3, 0, 2] * 25, [2, 0, 5, 40] * 25),  # more sequences than a wave has lanes
+    (64, 1, 1, [1, 3, 0, 130, 2] * 210, [2, 0, 5, 140, 1] * 210),  # work lists of more than 64 x 64 entries
     (64, 4, 4, [1500], [3]),
     (256, 12, 12, [700], [77]),
 ]
