@@ -1066,6 +1066,15 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
     f32x16 sa[2], da[2], sb[2], db[2];
     // Half u of the 64 that make stage j's dS from its S and dP: element e = u >> 1 (block e >> 4, score e & 15); even
     // halves do an exp2 and the next one's argument, odd ones the product
+    // dP starts from -delta where there are registers for it: a subtraction less per score
+    constexpr bool FROM = D < 256;
+    f32x16 from[FROM ? 2 : 1];
+    if constexpr (FROM) {
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) from[nb][r] = -del[nb];
+    }
     float x, pe;
     auto ds_half = [&](int j, f32x16 (&s)[2], f32x16 (&dp)[2], int u) {
       const int e = u >> 1, nb = e >> 4, r = e & 15;
@@ -1074,7 +1083,7 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
         pe = __builtin_amdgcn_exp2f(x);
         if (e < 31) x = __builtin_fmaf(s[(e + 1) >> 4][(e + 1) & 15], sl2, -lse[(e + 1) >> 4]);
       } else {
-        s[nb][r] = pe * (dp[nb][r] - del[nb]);
+        s[nb][r] = pe * (FROM ? dp[nb][r] : dp[nb][r] - del[nb]);
         if ((r & 3) == 3)
           *(f32x4*)(xch + (j & 1) * L::SBYTES + (nb * 4 + (r >> 2)) * 1024) =
               f32x4{s[nb][r - 3], s[nb][r - 2], s[nb][r - 1], s[nb][r]};
@@ -1101,7 +1110,7 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb) {
           const bf16x8& f = m & 1 ? df[nb][m >> 1] : qf[nb][m >> 1];
-          acc[nb] = mfma(a[m], f, m < 2 ? zero16() : acc[nb]);
+          acc[nb] = mfma(a[m], f, m == 1 && FROM ? from[FROM ? nb : 0] : m < 2 ? zero16() : acc[nb]);
           FENCE();
           if (nb == 0 && m + AHEAD < 2 * NS) a[m + AHEAD] = rd(m + AHEAD);
           if (nb == 0 && m + AHEAD == 2 * NS) last();
