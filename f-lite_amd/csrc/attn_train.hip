@@ -6,16 +6,26 @@
 //   delta = sum_d dout * out,  dP = dout v^T,  dS = P * (dP - delta)
 //   dv = P^T dout,  dk = scale dS^T q,  dq = scale dS k
 //
-// Backward = three launches. (1) delta and lse * log2(e) per query row. (2) Two kinds of workgroups in one launch: a
-// "key" workgroup owns 128 keys of one K/V head and sweeps the queries of its group of heads (4 products: S, dP, dv,
-// dk); a "query" workgroup owns 128 queries of one head and sweeps the keys (3 products: S, dP, dq). S and dP are made
-// twice (7 products instead of 5), and in return every gradient is summed by one workgroup in registers, in a fixed
-// order: no atomics, no fp32 gradient in memory. (3) Where too few workgroups would run, the sweeps are cut into
-// ranges whose fp32 partial gradients a last kernel adds in range order.
+// Forward: a workgroup owns 256 queries of one head and sweeps the keys, two products; where units are few or long, the
+// sweeps are cut into ranges and joined (attn_lse_kernel).
 //
-// A wave owns 32 of the workgroup's rows ("stationary": fragments in registers, row on the lane) and reads tiles of
-// the swept rows from LDS: row-wise (ds_read_b128, A operand of S and dP) and transposed (ds_read_b64_tr_b16, A operand
-// of the gradients). P and dS go from the S accumulators straight into the B operand: no LDS round trip.
+// Backward = three launches. (1) delta and lse * log2(e) per query row, and the work list. (2) Two kinds of workgroups in
+// one launch: a "key" workgroup owns 128 keys of one K/V head and sweeps the queries of its group of heads (4 products:
+// S, dP, dv, dk); a "query" workgroup owns 128 queries of one head and sweeps the keys (S, dP, and dq twice: its dS counts
+// in two bf16 parts). That is 8 products, where 5 would do if S and dP were made once; in return every gradient is summed
+// by one workgroup in registers, in a fixed order: no atomics, no fp32 dq in memory. (3) Where too few workgroups would
+// run, the sweeps are cut into ranges whose fp32 partial gradients a last kernel adds in range order.
+//
+// Two waves share 64 of the workgroup's rows ("stationary": fragments in registers, row on the lane) and split the
+// products between them: an accumulator of 64 x 256 takes 256 registers, so a wave of its 512 holds one. They read tiles
+// of 32 swept rows from LDS, where copies bring them several steps ahead: row-wise (ds_read_b128, A operand of S and dP)
+// and transposed (ds_read_b64_tr_b16, A operand of the gradients); P and dS go straight into the B operand of their own
+// wave, and through LDS to the other.
+//
+// Bound by the matrix cores. Measured: backward of 2 x 4112 tokens, 12 heads of 256 (8 products, 1.66 TFLOP): 1377 us =
+// 1.2 PFLOP/s, where an 8192^3 matrix product reaches 1.38 and the card lowers its clock to 1.65 GHz under either. With
+// head size 128 (4 x 4096 tokens, 16 heads) 1956 us = 1.12 PFLOP/s, with 64 1480 us = 0.74: the scores' exp2 and products
+// take as long as the MFMAs there. Forward, two products: 390 us = 1.07, 510 = 1.08 and 325 = 0.85 PFLOP/s.
 #include <math.h>
 
 #include <algorithm>
@@ -321,7 +331,7 @@ __device__ __forceinline__ void make_groups(const TrainDev& d) {
 }
 
 // First launch of the backward pass: lse * log2 e and delta of every query row (those outside all sequences are read by
-// nobody); the ranges' length; zeros outside
+// nobody); the work list; zeros outside. Bound by HBM: 101 MB (8224 rows, 12 heads of 256) in 23 us = 4.4 TB/s.
 template <int D>
 __global__ __launch_bounds__(kThreads) void attn_delta_kernel(TrainDev d, int n) {  // the first n workgroups: the rest
   const AttnTrainParams& p = d.p;
@@ -367,11 +377,15 @@ __global__ __launch_bounds__(kThreads) void attn_delta_kernel(TrainDev d, int n)
 //
 // Everything is made a step (32 swept rows) or more ahead, so that between two barriers no wave waits: a step's tiles
 // have been in LDS for a whole step, the first fragments of a step are read before its barrier, scores are turned into
-// P or dS in the step after their products. What a step costs beyond its 2048 MFMA cycles is the barrier.
+// P or dS in the step after their products. Measured (one sequence of 4096, 4 heads): 2870 cycles a step of a key workgroup
+// and 3160 of a query workgroup with D = 256, of which the MFMAs take 2048; 1840 and 2080 with D = 128 (1024), 1525 and
+// 1640 with 64 (512). The scores' vector work, about 900 cycles, hides behind D = 256's MFMAs; what is left is the barrier
+// and the waits on LDS behind it. A workgroup starts in 5.4 us with D = 128 and 7.5 with 256 (stationary rows: 32 rows a
+// load, 32 B of each) and ends in 3.4 and 9.
 
-// Steps that a copy may take beyond the one it is issued in. A copy takes 1.2 to 2 us (L2 or HBM), a step 0.9 us and more
-// with D = 256, 0.4 with 128, 0.2 with 64, and LDS has room for more stages where they are small (D = 128, ragged batch:
-// 1.37 us a step without).
+// Steps that a copy may take beyond the one it is issued in. A copy takes 1.2 to 2 us (L2 or HBM), a step 1.6 us with
+// D = 256, 1.0 with 128 and 0.8 with 64, and LDS has room for more stages where they are small. Without one more a step of
+// D = 64 takes 3 % longer (4 x 4096 tokens, 16 heads: 1550 us against 1500), with four as long; D = 128: 1 to 3 alike.
 template <int D>
 constexpr int kExtra = D == 256 ? 0 : D == 128 ? 2 : 1;
 
@@ -1275,7 +1289,7 @@ __global__ __launch_bounds__(kThreads, 1) void attn_bwd_kernel(TrainDev d) {
 }
 
 // Adds the ranges' partial gradients in order: one item = 8 columns of a row and head, of all rows (full tiles) or of the
-// 128-row slots of the sequences' parts
+// 128-row slots of the sequences' parts. Bound by memory: three ranges of 589 keys, 12 heads of 256, and their like 15 us.
 struct JoinItems {
   int q_full, q_part, k_full, k_part;  // workgroups; 0: that kind has no ranges
 };
@@ -1336,7 +1350,10 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(TrainDev d, JoinIte
 // transposed, as a key workgroup's wave 0 does. P = 2^(S - m) with m the largest score of the query's first 32 keys: any m
 // will do while P and the sums stay in fp32's range, which they do up to S = m + 40 (bf16 rounds P to the same relative
 // 2^-9 there), so the accumulators are never scaled anew. Where a later score is larger still, the workgroup sweeps its
-// keys once more, with m the largest score of them all, which it then knows.
+// keys once more, with m the largest score of them all, which it then knows. (Scaling the accumulators where a maximum
+// grows took 300 registers' spills: a branch that multiplies pulls them out of the AGPRs.) Measured: 2970 cycles a step
+// with D = 256 (2048 of MFMAs), 1900 with 128 (1024), 1500 with 64 (512), where two workgroups share a CU instead: 4 x 4096
+// tokens, 16 heads 384 -> 321 us.
 template <int D>
 struct FwdLds {
   static constexpr int E = D == 256 ? 1 : D == 128 ? 3 : 4;  // steps that a copy may take beyond its own

@@ -11,6 +11,9 @@
 // keeps nothing), dx is written once. A wave holds a row of up to 3072 columns, 8 consecutive ones a lane and chunk (16-B
 // bf16 accesses), so that its sums need neither LDS nor barriers; longer rows take two or four waves. A workgroup of four
 // waves walks over a strip of rows, the next row of each wave on its way, and keeps what the rows share in LDS.
+// Measured at 8224 x 3072 bf16, two segments: forward 24.8 us (101 MB, 4.1 TB/s; a workgroup per row, which reads the
+// shared rows anew, 32.4), backward 37 us (151 MB, 4.1 TB/s; a workgroup per row at a time 59.6, four at a time 66) and
+// 8.4 for the sums of its 12.6 MB of partial sums. A large copy reaches 5.2 TB/s.
 #include <math.h>
 
 #include <algorithm>
@@ -24,6 +27,8 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxDim = 8192;
+// Workgroups wanted, and rows of a strip at least. Backward, both kernels: 256 strips 48.5 us, 384 46.5, 512 46.2, 1024 57
+// (each strip writes 2 D partial sums, which the second kernel reads); forward 256 to 2056: the same.
 constexpr int kFwdStrips = 1024, kBwdStrips = 512, kBwdRows = 8;
 
 struct NormTrainDev {
@@ -269,6 +274,7 @@ __global__ __launch_bounds__(kThreads) void layernorm_mod_kernel(NormTrainDev d)
 }
 
 // ---- backward: S0 and S1 of the strip to the workspace ----
+// (two waves a SIMD for bf16: with one, where it takes 264 registers, 8224 x 3072 take 56 us in place of 46)
 template <bool XBF, bool RMS, int NCH, bool SUMS>
 __global__ __launch_bounds__(kThreads, XBF ? 2 : 1) void norm_bwd_kernel(NormTrainDev d) {
   extern __shared__ __attribute__((aligned(16))) float smem[];

@@ -55,7 +55,8 @@ def cu_of(lens, first=0):
 
 # ------------------------------------------------------------------------------------------------ attention
 def attn_ref(q, k, v, do, ql, kl, scale, q_first=0, k_first=0, f=F, u=U):
-    """out, lse, dq, dk, dv in 64 bits and an elementwise bound for each, with P off by f, P and dS rounded by u; rows outside stay 0 (lse -inf)."""
+    """out, lse, dq, dk, dv in 64 bits and an elementwise bound for each, with P off by f, P and dS rounded by u; rows outside
+    stay 0 (lse -inf)."""
     n, h, d = q.shape
     hk = k.shape[1]
     Q, K, V, DO = (x.double() for x in (q, k, v, do))
