@@ -1144,6 +1144,7 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
         for (int r = 0; r < 16; ++r) s[nb][r] = 8 * (r >> 2) + 4 * hh + (r & 3) < left ? s[nb][r] : -INFINITY;
     };
     auto step = [&](int i, f32x16 (&s)[2], f32x16 (&dp)[2], f32x16 (&s2)[2], f32x16 (&dp2)[2]) {
+      read_first();  // behind the barrier: before it, the stage's copies had a step less to arrive
       open();
       mask(i, s);
       products(
@@ -1156,17 +1157,15 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
           [&]() {
             kr.move(at_k.move());
             vr.move(at_v.move());
-            read_first();
           });
       advance();
-      step_sync<E * 2 * P>();
+      step_sync<(E + 1) * 2 * P>();
     };
     step_sync();
     read_first();
     products(sa, da, [](int) {}, []() {});
     kr.move(SB);
     vr.move(SB);
-    read_first();
     step_sync();
     int i = 0;
     for (; i + 1 < n; i += 2) {
@@ -1174,6 +1173,7 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
       step(i + 1, sb, db, sa, da);
     }
     if (i < n) step(i, sa, da, sb, db);
+    step_sync();  // wave 1's last one; no copy may outlive the workgroup
     return;
   }
   f32x16 acc[2][ND];
@@ -1189,69 +1189,76 @@ __device__ __forceinline__ void query_block(const TrainDev& d, const Unit& u, ch
     tr.init(lane, lds0 + L::A);
     auto rd = [&](int s, int dt) { a[dt] = tr.read(s, dt); };
     Ring<L::RA, SB> at_t{0};
-    step_sync<E * 2 * P>();
-    for (int i = 1; i <= n; ++i) {
-      open();  // after the last stage: zeros
-      const char* x = xch + ((i - 1) & 1) * L::SBYTES;
-      f32x4 w[2][4];
+    f32x4 w[2][4];
+    u32x4 hi[2][2], lo[2][2];
+    auto load = [&](int j) {  // dS of stage j
+      const char* x = xch + (j & 1) * L::SBYTES;
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4)
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb) w[nb][r4] = *(const f32x4*)(x + (nb * 4 + r4) * 1024);
+    };
+    auto split_hi = [&](int s, int q) {  // pair q of 8: block q >> 2, scores 8 s + 2 (q & 3), + 1
+      const int nb = q >> 2, c = q & 3;
+      const f32x4& y = w[nb][2 * s + (c >> 1)];
+      hi[nb][s][c] = pack_bf(y[2 * (c & 1)], y[2 * (c & 1) + 1]);
+    };
+    auto split_lo = [&](int s, int q) {
+      const int nb = q >> 2, c = q & 3;
+      const f32x4& y = w[nb][2 * s + (c >> 1)];
+      lo[nb][s][c] = dropped(y[2 * (c & 1)], y[2 * (c & 1) + 1], hi[nb][s][c]);
+    };
+    // 2 ND MFMAs with one half of the stage's rows; hook(m) behind each
+    auto run = [&](const u32x4 (&b)[2][2], int s, auto hook) {
+      settle();
 #pragma unroll
-      for (int dt = 0; dt < ND; ++dt) rd(0, dt);
-      u32x4 hi[2][2], lo[2][2];
-      auto split_hi = [&](int s, int q) {  // pair q of 8: block q >> 2, scores 8 s + 2 (q & 3), + 1
-        const int nb = q >> 2, c = q & 3;
-        const f32x4& y = w[nb][2 * s + (c >> 1)];
-        hi[nb][s][c] = pack_bf(y[2 * (c & 1)], y[2 * (c & 1) + 1]);
-      };
-      auto split_lo = [&](int s, int q) {
-        const int nb = q >> 2, c = q & 3;
-        const f32x4& y = w[nb][2 * s + (c >> 1)];
-        const unsigned h2 = hi[nb][s][c];
-        lo[nb][s][c] = pack_bf(y[2 * (c & 1)] - __uint_as_float(h2 << 16),
-                               y[2 * (c & 1) + 1] - __uint_as_float(h2 & 0xffff0000u));
-      };
+      for (int m = 0; m < 2 * ND; ++m) {
+        bf16x8 bb = __builtin_bit_cast(bf16x8, b[m & 1][s]);
+        mfma_o<false>(acc[m & 1][m >> 1], a[m >> 1], bb);
+        FENCE();
+        hook(m);
+        FENCE();
+      }
+    };
+    auto begin = [&]() {
 #pragma unroll
       for (int q = 0; q < 8; ++q) split_hi(0, q);
       FENCE();
+    };
+    step_sync<(E + 1) * 2 * P>();
+    load(0);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        settle();
-        // hi: 2 ND MFMAs; beside them the low parts
+    for (int dt = 0; dt < ND; ++dt) rd(0, dt);
+    begin();
+    for (int i = 1; i <= n; ++i) {
+      open();  // after the last stage: zeros
+      run(hi, 0, [&](int m) {
 #pragma unroll
-        for (int m = 0; m < 2 * ND; ++m) {
-          bf16x8 bb = __builtin_bit_cast(bf16x8, hi[m & 1][s]);
-          mfma_o<false>(acc[m & 1][m >> 1], a[m >> 1], bb);
-          FENCE();
+        for (int q = 0; q < 8; ++q)
+          if (q * ND / 4 == m) split_lo(0, q);
+        if (m & 1) copy(m >> 1);
+      });
+      // the fragments once more, then their place takes the next half's; beside them the next half's split
+      run(lo, 0, [&](int m) {
+        if (m & 1) rd(1, m >> 1);
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (s == 0 && q * ND / 4 == m) split_lo(0, q);
-          if (s == 1 && (m & 1)) copy(P + (m >> 1));
-          FENCE();
-        }
-        settle();
-        // lo: the fragments once more, then their place takes the next half's; beside them the next half's split
-#pragma unroll
-        for (int m = 0; m < 2 * ND; ++m) {
-          bf16x8 bb = __builtin_bit_cast(bf16x8, lo[m & 1][s]);
-          mfma_o<false>(acc[m & 1][m >> 1], a[m >> 1], bb);
-          FENCE();
-          if (s == 0 && (m & 1)) rd(1, m >> 1);
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (s == 0 && q * ND / 4 == m) {
-              split_hi(1, q);
-              split_lo(1, q);
-            }
-          if (s == 0 && !(m & 1) && (m >> 1) < P) copy(m >> 1);
-          FENCE();
-        }
-      }
-      tr.move(at_t.move());
+        for (int q = 0; q < 8; ++q)
+          if (q * ND / 4 == m) {
+            split_hi(1, q);
+            split_lo(1, q);
+          }
+      });
+      run(hi, 1, [](int) {});
+      // The barrier stands before the last MFMAs, which cover the next step's first reads (behind the last one they are
+      // of no use; wave 0 has one barrier more for it)
       advance();
-      if (i < n) step_sync<E * 2 * P>();
+      tr.move(at_t.move());
+      step_sync<(E + 1) * 2 * P>();
+      load(i);
+      run(lo, 1, [&](int m) {
+        if (m & 1) rd(0, m >> 1);
+      });
+      begin();
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may outlive the workgroup
   }
