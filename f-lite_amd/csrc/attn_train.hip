@@ -22,10 +22,10 @@
 // and transposed (ds_read_b64_tr_b16, A operand of the gradients); P and dS go straight into the B operand of their own
 // wave, and through LDS to the other.
 //
-// Bound by the matrix cores. Measured: backward of 2 x 4112 tokens, 12 heads of 256 (8 products, 1.66 TFLOP): 1377 us =
-// 1.2 PFLOP/s, where an 8192^3 matrix product reaches 1.38 and the card lowers its clock to 1.65 GHz under either. With
-// head size 128 (4 x 4096 tokens, 16 heads) 1956 us = 1.12 PFLOP/s, with 64 1480 us = 0.74: the scores' exp2 and products
-// take as long as the MFMAs there. Forward, two products: 390 us = 1.07, 510 = 1.08 and 325 = 0.85 PFLOP/s.
+// Bound by the matrix cores. Measured: backward of 2 x 4112 tokens, 12 heads of 256 (8 products, 1.66 TFLOP): 1340 us =
+// 1.24 PFLOP/s, where an 8192^3 matrix product reaches 1.38 and the card lowers its clock under either. With head size 128
+// (4 x 4096 tokens, 16 heads) 1921 us = 1.14 PFLOP/s, with 64 1490 us = 0.74: the scores' exp2 and products take as long
+// as the MFMAs there. Forward, two products: 390 us = 1.07, 510 = 1.08 and 325 = 0.85 PFLOP/s.
 #include <math.h>
 
 #include <algorithm>
@@ -376,12 +376,13 @@ __global__ __launch_bounds__(kThreads) void attn_delta_kernel(TrainDev d, int n)
 // from the exact gradient as one final rounding to bf16 is, against 1.4 for dk and dv).
 //
 // Everything is made a step (32 swept rows) or more ahead, so that between two barriers no wave waits: a step's tiles
-// have been in LDS for a whole step, the first fragments of a step are read before its barrier, scores are turned into
-// P or dS in the step after their products. Measured (one sequence of 4096, 4 heads): 2870 cycles a step of a key workgroup
-// and 3160 of a query workgroup with D = 256, of which the MFMAs take 2048; 1840 and 2080 with D = 128 (1024), 1525 and
-// 1640 with 64 (512). The scores' vector work, about 900 cycles, hides behind D = 256's MFMAs; what is left is the barrier
-// and the waits on LDS behind it. A workgroup starts in 5.4 us with D = 128 and 7.5 with 256 (stationary rows: 32 rows a
-// load, 32 B of each) and ends in 3.4 and 9.
+// have been in LDS before its barrier, the first fragments of a step are read where MFMAs cover them, scores are turned
+// into P or dS in the step after their products. Measured (one sequence of 4096, 4 heads): 3140 cycles a step of a key
+// workgroup and 2710 of a query workgroup with D = 256, of which the MFMAs take 2048; 2090 and 1770 with D = 128 (1024),
+// 1650 and 1400 with 64 (512). The scores' vector work, about 900 cycles, hides behind D = 256's MFMAs; what is left is
+// the barrier and the waits on LDS and on copies around it. A workgroup starts in 5.1 us with D = 128 and 7.5 with 256
+// (stationary rows: 32 rows a load, 32 B of each) and ends in 3.5 and 9. Of a whole launch shorter waits give back less:
+// the card lowers its clock under this load (query steps 6 % shorter: 2 x 4112 tokens 1349 -> 1330 us).
 
 // Steps that a copy may take beyond the one it is issued in. A copy takes 1.2 to 2 us (L2 or HBM), a step 1.6 us with
 // D = 256, 1.0 with 128 and 0.8 with 64, and LDS has room for more stages where they are small. Without one more a step of

@@ -725,3 +725,72 @@ def test_attention_branch_in_graphs_and_on_streams():
     torch.cuda.synchronize()
     for res in got:
         assert all(torch.equal(r, e) for r, e in zip(res, expect[1]))
+
+
+def test_offsets_past_32_bits():
+    """Rows 2^22 elements apart, the last ones more than 2^31 elements behind the first: the results of packed rows."""
+    rows, far = 600, 1 << 22
+    buf = torch.empty(rows, far, device=DEV, dtype=BF)
+    at = iter(range(0, far, 1024))
+
+    def spread(like, fill=True):
+        c, width = next(at), like[0].numel()
+        v = buf[:, c:c + width].unflatten(1, like.shape[1:])
+        return v.copy_(like) if fill else v
+
+    q, k, v, do = attn_inputs(64, 2, 1, [rows], [rows], seed=70)
+    cu, scale = cu_of([rows]), 64 ** -0.5
+    out, lse = nat.attn_varlen_lse(q, k, v, cu, cu, scale)
+    grads = nat.attn_varlen_bwd(do, q, k, v, out, lse, cu, cu, scale)
+    Q, K, V, DO, O = spread(q), spread(k), spread(v), spread(do), spread(q, False)
+    L = torch.empty_like(lse)
+    nat.attn_varlen_lse(Q, K, V, cu, cu, scale, O, L)
+    into = [spread(t, False) for t in (q, k, v)]
+    nat.attn_varlen_bwd(DO, Q, K, V, O, L, cu, cu, scale, *into)
+    assert torch.equal(O, out) and torch.equal(L, lse)
+    assert all(torch.equal(a, b) for a, b in zip(into, grads))
+    pos = torch.arange(2 * rows, device=DEV, dtype=torch.int32).view(rows, 2)
+    y, r = nat.rope_axes(q, pos, (16, 16), norm=True)
+    Y, R = nat.rope_axes(Q, pos, (16, 16), norm=True, out=spread(q, False))
+    assert torch.equal(Y, y) and torch.equal(R, r)
+    back = nat.rope_axes_bwd(DO, pos, (16, 16), y=Y, rstd=R, out=spread(q, False))
+    assert torch.equal(back, nat.rope_axes_bwd(do, pos, (16, 16), y=y, rstd=r))
+    x, w, b, shift, sc, dy = norm_inputs(rows, 640, 250, True, "rows", BF, False)
+    x = x.contiguous()
+    X, DY = spread(x), spread(dy)
+    assert torch.equal(nat.layernorm_modulate(X, w, b, shift, sc, 250, out=spread(x, False)),
+                       nat.layernorm_modulate(x, w, b, shift, sc, 250))
+    got = nat.norm_modulate_bwd(DY, X, w, b, sc, 250, dx=spread(x, False))
+    assert all(torch.equal(a, e) for a, e in zip(got, nat.norm_modulate_bwd(dy, x, w, b, sc, 250)))
+
+
+def test_long_rows_and_many_sequences_in_a_graph():
+    """What takes other launches than the branch above: norms of 8192 columns, and more than 64 sequences, whose work
+    lists are made on the device; replayed with other lengths than captured."""
+    x, w, b, shift, sc, dy = norm_inputs(6, 8192, 4, True, "rows", torch.float32, False)
+    x = x.contiguous()
+    ql, kl = [1, 9, 0, 4] * 20, [2, 0, 70, 5] * 20
+    q, k, v, do = attn_inputs(64, 2, 2, ql, kl, seed=80)
+    cq, ck = cu_of(ql), cu_of(kl)
+
+    def run():
+        y = nat.layernorm_modulate(x, w, b, shift, sc, 4)
+        out, lse = nat.attn_varlen_lse(q, k, v, cq, ck, 0.125)
+        return (y, *nat.norm_modulate_bwd(dy, x, w, b, sc, 4), out, lse,
+                *nat.attn_varlen_bwd(do, q, k, v, out, lse, cq, ck, 0.125))
+
+    run()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        res = run()
+    for turn in range(3):
+        if turn:
+            cq.copy_(cu_of(ql[turn:] + ql[:turn]))
+            ck.copy_(cu_of(kl[turn:] + kl[:turn]))
+        for t in res:
+            t.zero_()
+        g.replay()
+        expect = run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, e) for a, e in zip(res, expect))
